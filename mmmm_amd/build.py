@@ -20,7 +20,10 @@ LIB_PATH = LIB_DIR / 'libvividmed_hip.so'
 HIPCC = os.environ.get('HIPCC', '/opt/rocm/bin/hipcc')
 ARCH = 'gfx950'
 # VM_BUILD_DEFINES: extra -D flags of diagnostic builds (VM_GEMM_DEBUG_BUILD: the GEMM timing-experiment branches, tools/README.md)
+# packed fp32 off: hipcc -O3 forms v_pk_add / mul / fma_f32 from ordinary float code and some of their operand forms have returned wrong
+# results on these parts; the scalar forms compute the same values (the host pass does not know the feature and says so: harmless)
 CFLAGS = ['-O3', '-std=c++17', '-fPIC', f'--offload-arch={ARCH}', '-Wall', '-Wno-unused-function', '-DVM_KEEP_DENORMS',
+          '-Xclang', '-target-feature', '-Xclang', '-packed-fp32-ops',
           *os.environ.get('VM_BUILD_DEFINES', '').split()]
 
 

@@ -31,6 +31,7 @@ __device__ __forceinline__ void stv_nt(T* p, typename Elem<T>::vec_t v) {
 }
 
 // ---------------------------------------------------------------- RMSNorm
+// (the fused multiply-adds of the norms are written out: left to the compiler they are formed in one kernel form and not in the other)
 template <typename T>
 __global__ __launch_bounds__(ROW_THREADS) void rmsnorm_fwd_k(
     const T* __restrict__ x, const T* __restrict__ w, T* __restrict__ y, float* __restrict__ rstd_out,
@@ -46,7 +47,7 @@ __global__ __launch_bounds__(ROW_THREADS) void rmsnorm_fwd_k(
   for (int c = lane * V; c < cols; c += 64 * V) {
     auto v = ldv<T>(xr + c);
 #pragma unroll
-    for (int i = 0; i < V; ++i) { float f = Elem<T>::ld(v[i]); ss += f * f; }
+    for (int i = 0; i < V; ++i) { float f = Elem<T>::ld(v[i]); ss = fmaf(f, f, ss); }
   }
   ss = wave_sum(ss);
   const float r = rsqrtf(ss / (float)cols + eps);
@@ -81,7 +82,7 @@ __global__ __launch_bounds__(ROW_THREADS) void rmsnorm_bwd_k(
   for (int c = lane * V; c < cols; c += 64 * V) {
     auto xv = ldv<T>(xr + c); auto gv = ldv<T>(dyr + c); auto wv = ldv<T>(w + c);
 #pragma unroll
-    for (int i = 0; i < V; ++i) dot += Elem<T>::ld(wv[i]) * Elem<T>::ld(gv[i]) * (Elem<T>::ld(xv[i]) * r);
+    for (int i = 0; i < V; ++i) dot = fmaf(Elem<T>::ld(wv[i]) * Elem<T>::ld(gv[i]), Elem<T>::ld(xv[i]) * r, dot);
   }
   dot = wave_sum(dot) / (float)cols;
   for (int c = lane * V; c < cols; c += 64 * V) {
@@ -91,7 +92,7 @@ __global__ __launch_bounds__(ROW_THREADS) void rmsnorm_bwd_k(
 #pragma unroll
     for (int i = 0; i < V; ++i) {
       const float xh = Elem<T>::ld(xv[i]) * r;
-      o[i] = Elem<T>::st(r * (Elem<T>::ld(wv[i]) * Elem<T>::ld(gv[i]) - xh * dot) + (addr ? Elem<T>::ld(av[i]) : 0.f));
+      o[i] = Elem<T>::st(fmaf(r, fmaf(-xh, dot, Elem<T>::ld(wv[i]) * Elem<T>::ld(gv[i])), addr ? Elem<T>::ld(av[i]) : 0.f));
     }
     stv<T>(dxr + c, o);
   }
@@ -170,7 +171,7 @@ __global__ __launch_bounds__(ROW_THREADS) void layernorm_fwd_k(
   for (int c = lane * V; c < cols; c += 64 * V) {
     auto v = ldv<T>(xr + c);
 #pragma unroll
-    for (int i = 0; i < V; ++i) { const float d = Elem<T>::ld(v[i]) - mu; ss += d * d; }
+    for (int i = 0; i < V; ++i) { const float d = Elem<T>::ld(v[i]) - mu; ss = fmaf(d, d, ss); }
   }
   const float r = rsqrtf(wave_sum(ss) / (float)cols + eps);
   if (lane == 0) { if (mean_out) mean_out[row] = mu; if (rstd_out) rstd_out[row] = r; }
@@ -186,8 +187,9 @@ __global__ __launch_bounds__(ROW_THREADS) void layernorm_fwd_k(
 #pragma unroll
     for (int i = 0; i < V; ++i) {
       float f = (Elem<T>::ld(v[i]) - mu) * r;
-      if (w) f *= Elem<T>::ld(wv[i]);
-      if (b) f += Elem<T>::ld(bv[i]);
+      if (w && b) f = fmaf(f, Elem<T>::ld(wv[i]), Elem<T>::ld(bv[i]));
+      else if (w) f *= Elem<T>::ld(wv[i]);
+      else if (b) f += Elem<T>::ld(bv[i]);
       // torch rounds LN's output to the storage dtype before the residual add
       if (rr) f = Elem<T>::ld(Elem<T>::st(f)) + Elem<T>::ld(rv[i]);
       o[i] = Elem<T>::st(f);
@@ -218,7 +220,7 @@ __global__ __launch_bounds__(ROW_THREADS) void layernorm_bwd_k(
     for (int i = 0; i < V; ++i) {
       const float xh = (Elem<T>::ld(xv[i]) - mu) * r, g = Elem<T>::ld(gv[i]);
       const float wg = w ? Elem<T>::ld(wv[i]) * g : g;
-      s1 += wg; s2 += wg * xh;
+      s1 += wg; s2 = fmaf(wg, xh, s2);
     }
   }
   s1 = wave_sum(s1) / (float)cols; s2 = wave_sum(s2) / (float)cols;
@@ -231,7 +233,7 @@ __global__ __launch_bounds__(ROW_THREADS) void layernorm_bwd_k(
     for (int i = 0; i < V; ++i) {
       const float xh = (Elem<T>::ld(xv[i]) - mu) * r, g = Elem<T>::ld(gv[i]);
       const float wg = w ? Elem<T>::ld(wv[i]) * g : g;
-      o[i] = Elem<T>::st(r * (wg - s1 - xh * s2) + (addr ? Elem<T>::ld(av[i]) : 0.f));
+      o[i] = Elem<T>::st(fmaf(r, fmaf(-xh, s2, wg - s1), addr ? Elem<T>::ld(av[i]) : 0.f));
     }
     stv<T>(dxr + c, o);
   }
@@ -260,7 +262,7 @@ __global__ __launch_bounds__(ROW_THREADS) void rmsnorm_fwd_r_k(
   float ss = 0.f;
   VM_ROW_LOOP(j, c) {
 #pragma unroll
-    for (int i = 0; i < V; ++i) { float f = Elem<T>::ld(xv[j][i]); ss += f * f; }
+    for (int i = 0; i < V; ++i) { float f = Elem<T>::ld(xv[j][i]); ss = fmaf(f, f, ss); }
   }
   ss = wave_sum(ss);
   const float r = rsqrtf(ss / (float)cols + eps);
@@ -295,7 +297,7 @@ __global__ __launch_bounds__(ROW_THREADS) void rmsnorm_bwd_r_k(
   VM_ROW_LOOP(j, c) {
     auto wv = ldv<T>(w + c);
 #pragma unroll
-    for (int i = 0; i < V; ++i) dot += Elem<T>::ld(wv[i]) * Elem<T>::ld(gv[j][i]) * (Elem<T>::ld(xv[j][i]) * r);
+    for (int i = 0; i < V; ++i) dot = fmaf(Elem<T>::ld(wv[i]) * Elem<T>::ld(gv[j][i]), Elem<T>::ld(xv[j][i]) * r, dot);
   }
   dot = wave_sum(dot) / (float)cols;
   VM_ROW_LOOP(j, c) {
@@ -305,7 +307,7 @@ __global__ __launch_bounds__(ROW_THREADS) void rmsnorm_bwd_r_k(
 #pragma unroll
     for (int i = 0; i < V; ++i) {
       const float xh = Elem<T>::ld(xv[j][i]) * r;
-      o[i] = Elem<T>::st(r * (Elem<T>::ld(wv[i]) * Elem<T>::ld(gv[j][i]) - xh * dot) + (addr ? Elem<T>::ld(av[i]) : 0.f));
+      o[i] = Elem<T>::st(fmaf(r, fmaf(-xh, dot, Elem<T>::ld(wv[i]) * Elem<T>::ld(gv[j][i])), addr ? Elem<T>::ld(av[i]) : 0.f));
     }
     stv<T>(dxr + c, o);
   }
@@ -332,7 +334,7 @@ __global__ __launch_bounds__(ROW_THREADS) void layernorm_fwd_r_k(
   float ss = 0.f;
   VM_ROW_LOOP(j, c) {
 #pragma unroll
-    for (int i = 0; i < V; ++i) { const float d = Elem<T>::ld(xv[j][i]) - mu; ss += d * d; }
+    for (int i = 0; i < V; ++i) { const float d = Elem<T>::ld(xv[j][i]) - mu; ss = fmaf(d, d, ss); }
   }
   const float r = rsqrtf(wave_sum(ss) / (float)cols + eps);
   if (lane == 0) { if (mean_out) mean_out[row] = mu; if (rstd_out) rstd_out[row] = r; }
@@ -347,8 +349,9 @@ __global__ __launch_bounds__(ROW_THREADS) void layernorm_fwd_r_k(
 #pragma unroll
     for (int i = 0; i < V; ++i) {
       float f = (Elem<T>::ld(xv[j][i]) - mu) * r;
-      if (w) f *= Elem<T>::ld(wv[i]);
-      if (b) f += Elem<T>::ld(bv[i]);
+      if (w && b) f = fmaf(f, Elem<T>::ld(wv[i]), Elem<T>::ld(bv[i]));
+      else if (w) f *= Elem<T>::ld(wv[i]);
+      else if (b) f += Elem<T>::ld(bv[i]);
       if (rr) f = Elem<T>::ld(Elem<T>::st(f)) + Elem<T>::ld(rv[i]);
       o[i] = Elem<T>::st(f);
     }
@@ -379,7 +382,7 @@ __global__ __launch_bounds__(ROW_THREADS) void layernorm_bwd_r_k(
     for (int i = 0; i < V; ++i) {
       const float xh = (Elem<T>::ld(xv[j][i]) - mu) * r, g = Elem<T>::ld(gv[j][i]);
       const float wg = w ? Elem<T>::ld(wv[i]) * g : g;
-      s1 += wg; s2 += wg * xh;
+      s1 += wg; s2 = fmaf(wg, xh, s2);
     }
   }
   s1 = wave_sum(s1) / (float)cols; s2 = wave_sum(s2) / (float)cols;
@@ -391,7 +394,7 @@ __global__ __launch_bounds__(ROW_THREADS) void layernorm_bwd_r_k(
     for (int i = 0; i < V; ++i) {
       const float xh = (Elem<T>::ld(xv[j][i]) - mu) * r, g = Elem<T>::ld(gv[j][i]);
       const float wg = w ? Elem<T>::ld(wv[i]) * g : g;
-      o[i] = Elem<T>::st(r * (wg - s1 - xh * s2) + (addr ? Elem<T>::ld(av[i]) : 0.f));
+      o[i] = Elem<T>::st(fmaf(r, fmaf(-xh, s2, wg - s1), addr ? Elem<T>::ld(av[i]) : 0.f));
     }
     stv<T>(dxr + c, o);
   }

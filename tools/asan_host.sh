@@ -5,7 +5,7 @@ R=$(cd "$(dirname "$0")/.." && pwd)
 OUT=${1:-/tmp/vm_asan}
 mkdir -p $OUT
 HIPCC=${HIPCC:-/opt/rocm/bin/hipcc}
-FLAGS="-O1 -g -std=c++17 -fPIC --offload-arch=gfx950 -DVM_KEEP_DENORMS -fsanitize=address -shared-libsan -Wno-option-ignored"
+FLAGS="-O1 -g -std=c++17 -fPIC --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -DVM_KEEP_DENORMS -fsanitize=address -shared-libsan -Wno-option-ignored"
 pids=()
 for f in gemm gemm256 rowwise lora instance_loss; do
   $HIPCC $FLAGS -c $R/mmmm_amd/csrc/$f.hip -o $OUT/$f.o > $OUT/$f.log 2>&1 &

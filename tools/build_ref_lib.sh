@@ -8,7 +8,7 @@ T=$(mktemp -d)
 git -C /root/repo archive $REV mmmm_amd/csrc include mmmm_amd/build.py | tar -x -C $T
 cd $T
 for f in mmmm_amd/csrc/*.hip; do
-  /opt/rocm/bin/hipcc -O3 -std=c++17 -fPIC --offload-arch=gfx950 -Wall -Wno-unused-function -DVM_KEEP_DENORMS -c $f -o ${f%.hip}.o &
+  /opt/rocm/bin/hipcc -O3 -std=c++17 -fPIC --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -Wall -Wno-unused-function -DVM_KEEP_DENORMS -c $f -o ${f%.hip}.o &
 done
 wait
 /opt/rocm/bin/hipcc -shared -fPIC --offload-arch=gfx950 -o /root/repo/mmmm_amd/lib/libvividmed_hip_$NAME.so mmmm_amd/csrc/*.o

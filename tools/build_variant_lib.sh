@@ -6,7 +6,7 @@ NAME=$1; shift
 T=$(mktemp -d)
 R=$(cd "$(dirname "$0")/.." && pwd)
 for f in $R/mmmm_amd/csrc/*.hip; do
-  /opt/rocm/bin/hipcc -O3 -std=c++17 -fPIC --offload-arch=gfx950 -Wall -Wno-unused-function -DVM_KEEP_DENORMS "$@" -I$R/mmmm_amd/csrc -c $f -o $T/$(basename ${f%.hip}).o &
+  /opt/rocm/bin/hipcc -O3 -std=c++17 -fPIC --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -Wall -Wno-unused-function -DVM_KEEP_DENORMS "$@" -I$R/mmmm_amd/csrc -c $f -o $T/$(basename ${f%.hip}).o &
 done
 wait
 /opt/rocm/bin/hipcc -shared -fPIC --offload-arch=gfx950 -o $R/mmmm_amd/lib/libvividmed_hip_$NAME.so $T/*.o
