@@ -44,7 +44,7 @@ extern "C" {
 #define VM_ACT_RELU 2
 
 /* library / device info --------------------------------------------------- */
-int vm_version(void);   /* 600 = round 6 (vm_attn_f32_args grew by causal / row_of_pos; head width 112); 510 = VM_TN_GROUP_MAX 24 -> 32; 500 = round 5 (vm_gemm_args grew by workspace / workspace_bytes; vm_gemm_workspace_bytes added; vm_lora_down_fused removed), 400 = round 4
+int vm_version(void);   /* 700 = vm_paged_kv / vm_attn_paged_args added; 600 = round 6 (vm_attn_f32_args grew by causal / row_of_pos; head width 112); 510 = VM_TN_GROUP_MAX 24 -> 32; 500 = round 5 (vm_gemm_args grew by workspace / workspace_bytes; vm_gemm_workspace_bytes added; vm_lora_down_fused removed), 400 = round 4
                           * (vm_attn_args grew by workspace / workspace_bytes). The argument structs below only ever GROW at their end; a caller built against an older
                           * header must be rebuilt when this number changes (there is no struct_size field). */
 /* fills name[0..len) with the gcnArchName of the current device */
@@ -507,6 +507,72 @@ int vm_attn_decode_workspace(int batch, int n_heads, int head_dim, int max_len, 
 int vm_attn_decode_bf16(const void* q, int64_t ldq, const void* k_cache, const void* v_cache, int64_t ld_row, int64_t ld_seq,
                         const int32_t* kv_lens_dev, void* out, int64_t ldo, int batch, int n_heads, int head_dim, int max_len,
                         float scale, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* ---- Paged KV cache (generation path): conversations that go on, caches of different lengths in one pool, a bound on their memory.
+ * k_pages / v_pages: bf16, element (page, kv head, row, d) at page * ld_page + (kv_head * page_size + row) * head_dim + d; token j of
+ * sample b lies in page block_table[b * ld_table + j / page_size], row j % page_size. page_size 16 .. 1024, a power of two; head_dim
+ * 32 / 64 / 128. A table entry outside [0, n_pages) is a page that is not there: its tokens are masked, nothing is read or written through
+ * it. Pages may be shared by samples as long as nobody appends to a shared one. */
+typedef struct vm_paged_kv {
+  void* k_pages;
+  void* v_pages;
+  int64_t ld_page;
+  int32_t n_pages, page_size;
+  const int32_t* block_table; /* int32[n_seq][ld_table], max_pages entries used */
+  int64_t ld_table;
+  int32_t max_pages, n_seq;
+  int32_t n_kv_heads, head_dim;
+} vm_paged_kv;
+
+/* New tokens into the cache, rotary positions of q and k included (modeling_cogvlm.py:246-262). qkv rows are
+ * [n_heads | n_kv_heads | n_kv_heads] x head_dim; row r is token row_index[r] of sample row_seq[r] (either out of range: the row's K / V are
+ * not stored) at rotary position row_pos[r] (clamped to [0, n_pos)); cos / sin fp32 [n_pos, head_dim] as in vm_rope_inplace. The rotated q
+ * goes to q_out[rows][n_heads * head_dim]; qkv itself is not changed. Rows at or behind *nrows_dev are left alone. Two rows that name the
+ * same token are a race. */
+int vm_kv_append_paged_bf16(const vm_paged_kv* cache_host, const void* qkv, int64_t ld, const int32_t* row_seq, const int32_t* row_index,
+                            const int32_t* row_pos, const float* cos_tab, const float* sin_tab, int n_pos, int rows, int n_heads,
+                            void* q_out, int64_t ldq, const int32_t* nrows_dev, void* stream);
+
+/* Attention of a chunk of new tokens over the paged cache that already holds them (modeling_cogvlm.py:113-141 for one token, a prompt, or
+ * anything between). Positions cu_q[b] .. cu_q[b + 1] - 1 are the n_b new tokens of sample b, the last n_b of its kv_lens[b] cached ones:
+ * the i-th sees the tokens j <= kv_lens[b] - n_b + i. Query head h reads kv head h / (n_heads / n_kv_heads). Scores and softmax in fp32 (no
+ * rounding of the scores), probabilities rounded to bf16 for the P V product. A query that sees nothing gets zeros and lse = -inf.
+ * row_of_pos (may be NULL: identity) is the packed row of a position in q and out; lse[h * ld_lse + position]. Rows of no position are left
+ * as they were. max_q / max_kv: host upper bounds of n_b and of kv_lens (no device -> host sync).
+ * weights_out (may be NULL): weights_out[b][kv head][j] = weights[b][kv head][j] + the sum of the probabilities that token j gets from this
+ * call's queries of the heads of that kv head, for j < kv_lens[b]; fp32, fixed order of summation; weights may be the same buffer. */
+typedef struct vm_attn_paged_args {
+  vm_paged_kv cache;
+  const void* q;
+  int64_t ldq;
+  const int32_t* cu_q;
+  const int32_t* kv_lens;
+  const int32_t* row_of_pos;
+  void* out;
+  int64_t ldo;
+  float* lse;
+  int64_t ld_lse;
+  int32_t n_rows;
+  int32_t max_q, max_kv;
+  int32_t n_heads;
+  float scale;
+  int32_t w_cols;
+  const float* weights;
+  float* weights_out;
+  int64_t ldw_seq, ldw_head, ldwo_seq, ldwo_head;
+  void* workspace;
+  int64_t workspace_bytes;
+} vm_attn_paged_args;
+int vm_attn_paged_workspace(const vm_attn_paged_args* args_host, int64_t* bytes_host);
+int vm_attn_paged_bf16(const vm_attn_paged_args* args_host, void* stream);
+
+/* Eviction: of every sample and kv head the `budget` tokens stay that are among the `recent` newest or have the largest weight (ties: the
+ * older one; NaN counts as least; tokens of absent pages never stay). They keep their order and go to the pages of new_table, which nothing
+ * else may use; the old pages are not changed. new_lens[b] = how many stayed, new_weights their weights with zeros behind,
+ * kept[b][kv head][budget] their old indices with -1 behind. */
+int vm_kv_evict_paged_bf16(const vm_paged_kv* cache_host, const float* weights, int64_t ldw_seq, int64_t ldw_head, int w_cols,
+                           const int32_t* kv_lens, const int32_t* new_table, int64_t ld_new_table, int new_pages, int budget, int recent,
+                           float* new_weights, int64_t ldn_seq, int64_t ldn_head, int32_t* new_lens, int32_t* kept, void* stream);
 
 /* fp32 attention (SAM ViT-B encoder image_encoder.py:126-136 hd 64; two-way
  * transformer transformer.py:224-239 hd 96/48, tiny Lq or tiny Lk).

@@ -502,7 +502,7 @@ extern "C" int vm_prof_end2_(int kind, void* stream, void* tok, double flops, do
 
 extern "C" {
 
-int vm_version(void) { return 600; }      /* 600: round 6 (vm_attn_f32_args.causal / row_of_pos, head width 112); 510: VM_TN_GROUP_MAX 24 -> 32 (vm_tn_skinny_group_bf16 takes up to 32 items); 500: round 5 (vm_gemm_args.workspace / workspace_bytes, vm_gemm_workspace_bytes); 400: round 4 (vm_attn_args.workspace / workspace_bytes); 300: round 3 (vm_gemm_args.b_nn / f32_split, vm_attn_f32_args.f32_split) */
+int vm_version(void) { return 700; }      /* 700: the paged cache entry points (vm_paged_kv, vm_attn_paged_args); 600: round 6 (vm_attn_f32_args.causal / row_of_pos, head width 112); 510: VM_TN_GROUP_MAX 24 -> 32 (vm_tn_skinny_group_bf16 takes up to 32 items); 500: round 5 (vm_gemm_args.workspace / workspace_bytes, vm_gemm_workspace_bytes); 400: round 4 (vm_attn_args.workspace / workspace_bytes); 300: round 3 (vm_gemm_args.b_nn / f32_split, vm_attn_f32_args.f32_split) */
 
 int vm_device_arch(char* name_host, int len) {
   int dev = 0;

@@ -1,0 +1,263 @@
+// Paged KV cache of the generation path: storing new tokens (with the rotary positions of q and k) and eviction by received attention
+// weight. Replaces, for a paged cache, the rotary call and the torch.cat of /root/reference/mmmm/models/cogvlm/modeling_cogvlm.py:246-262.
+#include "paged.hpp"
+
+namespace {
+
+// ----------------------------------------------------------------------------- append
+// q'[t] = R(pos_t) q[t], K[page, row] = R(pos_t) k[t], V[page, row] = v[t];  R on the halves (x1, x2): (x1 c1 - x2 s1, x2 c2 + x1 s2),
+// fp32, rounded to bf16 once. HBM-bound: every qkv element is read once and written once. One workgroup takes 256 / tpr rows; a thread
+// owns one 8-element chunk index of the half head and walks the heads, so its 32 table values are loaded once per row and not per head.
+struct AppendP {
+  const unsigned short* qkv; int64_t ld;
+  const int32_t* row_seq; const int32_t* row_index; const int32_t* row_pos;
+  const float* cos; const float* sin; int n_pos;
+  const int32_t* nrows_dev; int rows;
+  int n_heads, n_seq;
+  unsigned short* q_out; int64_t ldq;
+  int tpr;                    // threads per row (power of two, <= 256)
+  PagedKV c;
+};
+
+template <int HD>
+__global__ __launch_bounds__(256) void kv_append_k(const AppendP p) {
+  constexpr int CPH = HD / 16;                    // 8-element chunks of a half head
+  int rows = p.rows;
+  if (p.nrows_dev) rows = min(rows, *p.nrows_dev);
+  const int row = blockIdx.x * (256 / p.tpr) + threadIdx.x / p.tpr;
+  if (row >= rows) return;
+  const int t = threadIdx.x & (p.tpr - 1);
+  const int ch = t & (CPH - 1), hl = t / CPH, hstep = p.tpr / CPH;
+  const int pos = max(0, min(p.row_pos[row], p.n_pos - 1));
+  const int seq = p.row_seq[row], idx = p.row_index[row];
+  int64_t dst = -1;                               // element offset of (page, head 0, row), or -1: nothing is stored
+  if ((unsigned)seq < (unsigned)p.n_seq && idx >= 0 && (idx >> p.c.shift) < p.c.max_pages) {
+    const int page = p.c.table[seq * p.c.ld_table + (idx >> p.c.shift)];
+    if (page_ok(page, p.c.n_pages)) dst = page_row(page, p.c.ld_page, 0, idx & p.c.mask, p.c.shift, HD);
+  }
+  const int64_t head_ld = (int64_t)HD << p.c.shift;
+  float c1[8], s1[8], c2[8], s2[8];
+  {
+    const float* cr = p.cos + (int64_t)pos * HD + ch * 8;
+    const float* sr = p.sin + (int64_t)pos * HD + ch * 8;
+#pragma unroll
+    for (int e = 0; e < 8; e += 4) {
+      *reinterpret_cast<f32x4_t*>(c1 + e) = *reinterpret_cast<const f32x4_t*>(cr + e);
+      *reinterpret_cast<f32x4_t*>(s1 + e) = *reinterpret_cast<const f32x4_t*>(sr + e);
+      *reinterpret_cast<f32x4_t*>(c2 + e) = *reinterpret_cast<const f32x4_t*>(cr + HD / 2 + e);
+      *reinterpret_cast<f32x4_t*>(s2 + e) = *reinterpret_cast<const f32x4_t*>(sr + HD / 2 + e);
+    }
+  }
+  const unsigned short* src = p.qkv + (int64_t)row * p.ld + ch * 8;
+  const int H = p.n_heads, Hk = p.c.n_kv_heads, total = H + 2 * Hk;
+  for (int h = hl; h < total; h += hstep) {
+    const u16x8_t a = *reinterpret_cast<const u16x8_t*>(src + h * HD);
+    const u16x8_t b = *reinterpret_cast<const u16x8_t*>(src + h * HD + HD / 2);
+    u16x8_t oa = a, ob = b;
+    if (h < H + Hk) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float x1 = bf2f(a[e]), x2 = bf2f(b[e]);
+        oa[e] = f2bf(x1 * c1[e] - x2 * s1[e]);
+        ob[e] = f2bf(x2 * c2[e] + x1 * s2[e]);
+      }
+    }
+    unsigned short* d;
+    if (h < H) {
+      d = p.q_out + (int64_t)row * p.ldq + h * HD;
+    } else {
+      if (dst < 0) continue;
+      const bool is_v = h >= H + Hk;
+      d = const_cast<unsigned short*>(is_v ? p.c.v : p.c.k) + dst + (h - H - (is_v ? Hk : 0)) * head_ld;
+    }
+    *reinterpret_cast<u16x8_t*>(d + ch * 8) = oa;
+    *reinterpret_cast<u16x8_t*>(d + HD / 2 + ch * 8) = ob;
+  }
+}
+
+// ----------------------------------------------------------------------------- eviction
+// One workgroup per (sample, kv head) picks the tokens that stay: the `budget` best by (key descending, index ascending), where the key
+// is 2^32 - 1 for the `recent` newest tokens, an order-preserving image of the weight for the others (NaN lowest, -0 = +0) and 0 for
+// tokens of absent pages, which never stay. The threshold key is found digit by digit (8 bits a pass, histogram in LDS) — exact, whatever
+// the distribution — and a last pass in index order emits the survivors, the first few of those AT the threshold included.
+constexpr int EV_THREADS = 1024, EV_WAVES = EV_THREADS / 64;
+
+__device__ __forceinline__ unsigned weight_key(float w) {
+  if (w != w) return 1u;
+  if (w == 0.f) w = 0.f;
+  const unsigned u = __builtin_bit_cast(unsigned, w);
+  return (u >> 31) ? ~u : u | 0x80000000u;
+}
+
+struct EvictP {
+  const float* w; float* w_new; int64_t ldw_seq, ldw_head, ldn_seq, ldn_head; int w_cols;
+  const int32_t* lens; int32_t* new_lens;
+  const int32_t* new_table; int64_t ld_new; int new_pages;
+  int32_t* kept; int budget, recent;
+  PagedKV c;
+};
+
+__device__ __forceinline__ unsigned evict_key(const EvictP& p, const float* w, const int32_t* table, int j, int newest) {
+  if (!page_ok(table[j >> p.c.shift], p.c.n_pages)) return 0u;
+  return j >= newest ? 0xFFFFFFFFu : weight_key(w[j]);
+}
+
+__global__ __launch_bounds__(EV_THREADS) void kv_evict_select_k(const EvictP p) {
+  __shared__ unsigned hist[256];
+  __shared__ unsigned sh[4];
+  __shared__ unsigned wsum[2][EV_WAVES];
+  const int hk = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int cap = (int)min((int64_t)p.c.max_pages << p.c.shift, (int64_t)p.w_cols);
+  const int n = max(0, min(p.lens[b], cap));
+  const int newest = n - min(p.recent, n);
+  const float* w = p.w + b * p.ldw_seq + hk * p.ldw_head;
+  float* wn = p.w_new + b * p.ldn_seq + hk * p.ldn_head;
+  const int32_t* table = p.c.table + b * p.c.ld_table;
+  int32_t* kept = p.kept + ((int64_t)b * p.c.n_kv_heads + hk) * p.budget;
+  // ---- threshold
+  unsigned prefix = 0, pmask = 0;
+  int want = 0, keep = 0;                         // how many of the keys that share the prefix stay
+  for (int pass = 0; pass < 4; ++pass) {
+    const int sh_bits = 24 - 8 * pass;
+    for (int i = tid; i < 256; i += EV_THREADS) hist[i] = 0;
+    if (tid == 0) sh[2] = 0;
+    __syncthreads();
+    unsigned present = 0;
+    for (int j = tid; j < n; j += EV_THREADS) {
+      const unsigned key = evict_key(p, w, table, j, newest);
+      if (key != 0) {
+        ++present;
+        if ((key & pmask) == prefix) atomicAdd(&hist[(key >> sh_bits) & 255], 1u);
+      }
+    }
+    if (pass == 0 && present) atomicAdd(&sh[2], present);
+    __syncthreads();
+    if (pass == 0) keep = want = min((int)sh[2], p.budget);
+    if (tid == 0) {                               // the digit whose bin holds the want-th largest key
+      unsigned above = 0;
+      int d = 255;
+      for (; d > 0; --d) {
+        if (above + hist[d] >= (unsigned)want) break;
+        above += hist[d];
+      }
+      sh[0] = (unsigned)d;
+      sh[1] = above;
+    }
+    __syncthreads();
+    prefix |= sh[0] << sh_bits;
+    pmask |= 0xFFu << sh_bits;
+    want -= (int)sh[1];
+    __syncthreads();
+  }
+  // ---- survivors in index order
+  int out0 = 0, eq0 = 0;
+  for (int j0 = 0; j0 < n && out0 < keep; j0 += EV_THREADS) {
+    const int j = j0 + tid;
+    const unsigned key = j < n ? evict_key(p, w, table, j, newest) : 0u;
+    const bool eq = key != 0 && key == prefix, gt = key > prefix;
+    const uint64_t beq = __ballot(eq);
+    if (lane == 0) wsum[0][wave] = __popcll(beq);
+    __syncthreads();
+    int eq_before = eq0 + __popcll(beq & ((1ull << lane) - 1)), eq_all = 0;
+    for (int i = 0; i < EV_WAVES; ++i) {
+      if (i < wave) eq_before += wsum[0][i];
+      eq_all += wsum[0][i];
+    }
+    const bool stay = gt || (eq && eq_before < want);
+    const uint64_t bst = __ballot(stay);
+    if (lane == 0) wsum[1][wave] = __popcll(bst);
+    __syncthreads();
+    int at = out0 + __popcll(bst & ((1ull << lane) - 1)), all = 0;
+    for (int i = 0; i < EV_WAVES; ++i) {
+      if (i < wave) at += wsum[1][i];
+      all += wsum[1][i];
+    }
+    if (stay && at < keep) {
+      kept[at] = j;
+      if (at < p.w_cols) wn[at] = w[j];
+    }
+    out0 += all;
+    eq0 += eq_all;
+    __syncthreads();
+  }
+  for (int j = keep + tid; j < p.budget; j += EV_THREADS) kept[j] = -1;
+  for (int j = keep + tid; j < p.w_cols; j += EV_THREADS) wn[j] = 0.f;      // the next tokens of this sample start at zero
+  if (hk == 0 && tid == 0) p.new_lens[b] = keep;
+}
+
+// the rows that stay, K and V, into the sample's new pages: HD / 8 lanes per row, 16 bytes each
+template <int HD>
+__global__ __launch_bounds__(256) void kv_evict_move_k(const EvictP p) {
+  constexpr int LPR = HD / 8, RPB = 256 / LPR;
+  const int hk = blockIdx.y, b = blockIdx.z;
+  const int j = blockIdx.x * RPB + threadIdx.x / LPR, e = (threadIdx.x & (LPR - 1)) * 8;
+  if (j >= p.budget) return;
+  const int i = p.kept[((int64_t)b * p.c.n_kv_heads + hk) * p.budget + j];
+  if (i < 0 || (j >> p.c.shift) >= p.new_pages) return;
+  const int src = p.c.table[b * p.c.ld_table + (i >> p.c.shift)], dst = p.new_table[b * p.ld_new + (j >> p.c.shift)];
+  if (!page_ok(src, p.c.n_pages) || !page_ok(dst, p.c.n_pages)) return;
+  const int64_t s = page_row(src, p.c.ld_page, hk, i & p.c.mask, p.c.shift, HD) + e, d = page_row(dst, p.c.ld_page, hk, j & p.c.mask, p.c.shift, HD) + e;
+  if (s == d) return;
+  const u16x8_t kv = *reinterpret_cast<const u16x8_t*>(p.c.k + s), vv = *reinterpret_cast<const u16x8_t*>(p.c.v + s);
+  *reinterpret_cast<u16x8_t*>(const_cast<unsigned short*>(p.c.k) + d) = kv;
+  *reinterpret_cast<u16x8_t*>(const_cast<unsigned short*>(p.c.v) + d) = vv;
+}
+
+}  // namespace
+
+extern "C" {
+
+int vm_kv_append_paged_bf16(const vm_paged_kv* cache_host, const void* qkv, int64_t ld, const int32_t* row_seq, const int32_t* row_index,
+                            const int32_t* row_pos, const float* cos_tab, const float* sin_tab, int n_pos, int rows, int n_heads,
+                            void* q_out, int64_t ldq, const int32_t* nrows_dev, void* stream) {
+  AppendP p;
+  const int rc = paged_cache(cache_host, p.c);
+  if (rc != VM_OK) return rc;
+  if (rows < 0 || n_heads <= 0 || n_pos <= 0) return VM_ERR_BAD_ARG;
+  if (rows == 0 || cache_host->n_seq == 0) return VM_OK;
+  if (!qkv || !row_seq || !row_index || !row_pos || !cos_tab || !sin_tab || !q_out) return VM_ERR_BAD_ARG;
+  const int hd = cache_host->head_dim, total = n_heads + 2 * p.c.n_kv_heads;
+  if (misaligned16(qkv) || misaligned16(q_out) || misaligned16(cos_tab) || misaligned16(sin_tab) || (ld & 7) || (ldq & 7)) return VM_ERR_BAD_ARG;
+  if (ld < (int64_t)total * hd || ldq < (int64_t)n_heads * hd) return VM_ERR_BAD_ARG;
+  p.qkv = (const unsigned short*)qkv; p.ld = ld; p.row_seq = row_seq; p.row_index = row_index; p.row_pos = row_pos;
+  p.cos = cos_tab; p.sin = sin_tab; p.n_pos = n_pos; p.nrows_dev = nrows_dev; p.rows = rows; p.n_heads = n_heads; p.n_seq = cache_host->n_seq;
+  p.q_out = (unsigned short*)q_out; p.ldq = ldq;
+  p.tpr = hd / 16;
+  while (p.tpr < 256 && p.tpr < total * (hd / 16)) p.tpr *= 2;
+  const dim3 grid((rows + 256 / p.tpr - 1) / (256 / p.tpr));
+  hipStream_t st = (hipStream_t)stream;
+  if (hd == 128) hipLaunchKernelGGL(kv_append_k<128>, grid, dim3(256), 0, st, p);
+  else if (hd == 64) hipLaunchKernelGGL(kv_append_k<64>, grid, dim3(256), 0, st, p);
+  else hipLaunchKernelGGL(kv_append_k<32>, grid, dim3(256), 0, st, p);
+  VM_LAUNCH_CHECK();
+  return VM_OK;
+}
+
+int vm_kv_evict_paged_bf16(const vm_paged_kv* cache_host, const float* weights, int64_t ldw_seq, int64_t ldw_head, int w_cols,
+                           const int32_t* kv_lens, const int32_t* new_table, int64_t ld_new_table, int new_pages, int budget, int recent,
+                           float* new_weights, int64_t ldn_seq, int64_t ldn_head, int32_t* new_lens, int32_t* kept, void* stream) {
+  EvictP p;
+  const int rc = paged_cache(cache_host, p.c);
+  if (rc != VM_OK) return rc;
+  if (budget <= 0 || recent < 0 || recent > budget || w_cols <= 0 || new_pages <= 0 || ld_new_table < new_pages) return VM_ERR_BAD_ARG;
+  if (ldw_head < w_cols || ldn_head < w_cols || ldw_seq < 0 || ldn_seq < 0) return VM_ERR_BAD_ARG;
+  if (cache_host->n_seq == 0) return VM_OK;
+  if (cache_host->n_seq > 65535 || p.c.n_kv_heads > 65535) return VM_ERR_UNSUPPORTED;
+  if (!weights || !kv_lens || !new_table || !new_weights || !new_lens || !kept) return VM_ERR_BAD_ARG;
+  if (weights == new_weights || kv_lens == new_lens || cache_host->block_table == new_table) return VM_ERR_BAD_ARG;      // out of place
+  p.w = weights; p.w_new = new_weights; p.ldw_seq = ldw_seq; p.ldw_head = ldw_head; p.ldn_seq = ldn_seq; p.ldn_head = ldn_head; p.w_cols = w_cols;
+  p.lens = kv_lens; p.new_lens = new_lens; p.new_table = new_table; p.ld_new = ld_new_table; p.new_pages = new_pages;
+  p.kept = kept; p.budget = budget; p.recent = recent;
+  hipStream_t st = (hipStream_t)stream;
+  hipLaunchKernelGGL(kv_evict_select_k, dim3(p.c.n_kv_heads, cache_host->n_seq), dim3(EV_THREADS), 0, st, p);
+  VM_LAUNCH_CHECK();
+  const int hd = cache_host->head_dim, rpb = 256 / (hd / 8);
+  const dim3 grid((budget + rpb - 1) / rpb, p.c.n_kv_heads, cache_host->n_seq);
+  if (hd == 128) hipLaunchKernelGGL(kv_evict_move_k<128>, grid, dim3(256), 0, st, p);
+  else if (hd == 64) hipLaunchKernelGGL(kv_evict_move_k<64>, grid, dim3(256), 0, st, p);
+  else hipLaunchKernelGGL(kv_evict_move_k<32>, grid, dim3(256), 0, st, p);
+  VM_LAUNCH_CHECK();
+  return VM_OK;
+}
+
+}  // extern "C"

@@ -1,0 +1,50 @@
+// The paged KV cache of the generation path: what its kernels share.
+//
+// k_pages / v_pages: bf16 [n_pages][n_kv_heads][page_size][head_dim], pages `ld_page` elements apart. The rows of one head of one page are
+// contiguous (page_size * head_dim * 2 bytes: 16 KiB for 64 tokens of width 128), so a key tile of the attention kernels is one straight
+// piece of memory. Token j of sample b lies in page block_table[b][j / page_size], row j % page_size; page_size is a power of two >= 16.
+// A table entry outside [0, n_pages) is a page that is not there: nothing is read or written through it and its tokens are masked.
+#pragma once
+#include "vm_common.hpp"
+
+struct PagedKV {
+  const unsigned short* k;
+  const unsigned short* v;
+  int64_t ld_page;
+  const int32_t* table;
+  int64_t ld_table;
+  int n_pages, max_pages;
+  int shift, mask;            // page_size = 1 << shift = mask + 1
+  int n_kv_heads;
+};
+
+__device__ __forceinline__ bool page_ok(int page, int n_pages) { return (unsigned)page < (unsigned)n_pages; }
+
+// element offset of row `row` of head `hk` of page `page` (64 bits: a pool may hold more than 2^31 elements)
+__device__ __forceinline__ int64_t page_row(int page, int64_t ld_page, int hk, int row, int shift, int head_dim) {
+  return (int64_t)page * ld_page + (((int64_t)hk << shift) + row) * head_dim;
+}
+
+inline int paged_shift(int page_size) {          // log2 of a legal page size, -1 otherwise
+  for (int s = 4; s <= 10; ++s)
+    if (page_size == 1 << s) return s;
+  return -1;
+}
+
+inline bool misaligned16(const void* a) { return ((uintptr_t)a & 15) != 0; }
+
+// the checks that every entry on the cache shares; fills `c`
+inline int paged_cache(const vm_paged_kv* a, PagedKV& c) {
+  if (!a || !a->k_pages || !a->v_pages || !a->block_table) return VM_ERR_BAD_ARG;
+  if (a->n_pages <= 0 || a->max_pages <= 0 || a->n_kv_heads <= 0 || a->n_seq < 0) return VM_ERR_BAD_ARG;
+  if (a->head_dim != 32 && a->head_dim != 64 && a->head_dim != 128) return VM_ERR_UNSUPPORTED;
+  const int shift = paged_shift(a->page_size);
+  if (shift < 0) return VM_ERR_UNSUPPORTED;
+  if (misaligned16(a->k_pages) || misaligned16(a->v_pages) || (a->ld_page & 7)) return VM_ERR_BAD_ARG;
+  if (a->ld_page < (((int64_t)a->n_kv_heads << shift) * a->head_dim) || a->ld_table < a->max_pages) return VM_ERR_BAD_ARG;
+  if (((int64_t)a->max_pages << shift) > 0x7FFFFFFF - 4096) return VM_ERR_UNSUPPORTED;
+  c.k = (const unsigned short*)a->k_pages; c.v = (const unsigned short*)a->v_pages; c.ld_page = a->ld_page;
+  c.table = a->block_table; c.ld_table = a->ld_table;
+  c.n_pages = a->n_pages; c.max_pages = a->max_pages; c.shift = shift; c.mask = a->page_size - 1; c.n_kv_heads = a->n_kv_heads;
+  return VM_OK;
+}

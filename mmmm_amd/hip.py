@@ -86,6 +86,33 @@ class AttnF32Args(C.Structure):
     ]
 
 
+class PagedKVArgs(C.Structure):
+    """vm_paged_kv (include/vividmed_hip.h)"""
+    _fields_ = [
+        ('k_pages', C.c_void_p), ('v_pages', C.c_void_p), ('ld_page', C.c_int64),
+        ('n_pages', C.c_int32), ('page_size', C.c_int32),
+        ('block_table', C.c_void_p), ('ld_table', C.c_int64),
+        ('max_pages', C.c_int32), ('n_seq', C.c_int32),
+        ('n_kv_heads', C.c_int32), ('head_dim', C.c_int32),
+    ]
+
+
+class AttnPagedArgs(C.Structure):
+    """vm_attn_paged_args (include/vividmed_hip.h)"""
+    _fields_ = [
+        ('cache', PagedKVArgs),
+        ('q', C.c_void_p), ('ldq', C.c_int64),
+        ('cu_q', C.c_void_p), ('kv_lens', C.c_void_p), ('row_of_pos', C.c_void_p),
+        ('out', C.c_void_p), ('ldo', C.c_int64),
+        ('lse', C.c_void_p), ('ld_lse', C.c_int64),
+        ('n_rows', C.c_int32), ('max_q', C.c_int32), ('max_kv', C.c_int32), ('n_heads', C.c_int32),
+        ('scale', C.c_float), ('w_cols', C.c_int32),
+        ('weights', C.c_void_p), ('weights_out', C.c_void_p),
+        ('ldw_seq', C.c_int64), ('ldw_head', C.c_int64), ('ldwo_seq', C.c_int64), ('ldwo_head', C.c_int64),
+        ('workspace', C.c_void_p), ('workspace_bytes', C.c_int64),
+    ]
+
+
 TN_GROUP_MAX = 32
 
 

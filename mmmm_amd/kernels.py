@@ -819,6 +819,134 @@ def attn_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k
     return out
 
 
+def _paged_cache(k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: torch.Tensor) -> hip.PagedKVArgs:
+    """checked vm_paged_kv of a paged cache: k_pages / v_pages bf16 [pages, kv heads, page size, head dim] (page stride free),
+    block_table int32 [samples, pages per sample]"""
+    assert k_pages.dim() == 4 and k_pages.shape == v_pages.shape and k_pages.stride() == v_pages.stride(), (k_pages.shape, v_pages.shape)
+    assert k_pages.dtype == torch.bfloat16 and v_pages.dtype == torch.bfloat16, 'the paged cache is bf16'
+    n, hk, ps, hd = k_pages.shape
+    assert k_pages.stride()[1:] == (ps * hd, hd, 1), 'a page is contiguous: [kv heads, page size, head dim]'
+    assert hd in (32, 64, 128), f'head_dim {hd}: 32, 64 or 128'
+    assert 16 <= ps <= 1024 and ps & (ps - 1) == 0, f'page size {ps}: a power of two in 16 .. 1024'
+    assert block_table.dtype == torch.int32 and block_table.dim() == 2 and block_table.stride(1) == 1 and block_table.shape[1] > 0
+    assert k_pages.device == v_pages.device == block_table.device
+    c = hip.PagedKVArgs()
+    c.k_pages, c.v_pages, c.ld_page = ptr(k_pages), ptr(v_pages), k_pages.stride(0) if n > 1 else hk * ps * hd
+    c.n_pages, c.page_size, c.n_kv_heads, c.head_dim = n, ps, hk, hd
+    c.block_table, c.max_pages, c.n_seq = ptr(block_table), block_table.shape[1], block_table.shape[0]
+    c.ld_table = block_table.stride(0) if block_table.shape[0] > 1 else block_table.shape[1]
+    assert k_pages.device.index == torch.cuda.current_device(), 'the cache lies on another device than the current one'
+    return c
+
+
+def _i32(t: torch.Tensor, n: int, like: torch.Tensor) -> torch.Tensor:
+    assert t.dtype == torch.int32 and t.is_contiguous() and t.numel() >= n and t.device == like.device, (t.dtype, t.shape, n)
+    return t
+
+
+def kv_append_paged(qkv: torch.Tensor, row_seq: torch.Tensor, row_index: torch.Tensor, block_table: torch.Tensor, k_pages: torch.Tensor,
+                    v_pages: torch.Tensor, row_pos: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, n_heads: int, *,
+                    nrows: torch.Tensor | None = None, q_out: torch.Tensor | None = None) -> torch.Tensor:
+    """new tokens into a paged cache, rotary positions included (vm_kv_append_paged_bf16). qkv [T, (n_heads + 2 kv heads) hd] bf16, not
+    changed; row r is token row_index[r] of sample row_seq[r] (out of range, e.g. -1: not stored) at position row_pos[r]; all int32.
+    -> rotated q [T, n_heads hd]"""
+    T = qkv.shape[0]
+    _, hk, _, hd = k_pages.shape
+    assert qkv.dim() == 2 and qkv.dtype == torch.bfloat16 and qkv.stride(1) == 1 and qkv.shape[1] == (n_heads + 2 * hk) * hd, (qkv.shape, n_heads, hk, hd)
+    assert qkv.device == k_pages.device and n_heads > 0
+    assert cos.dtype == torch.float32 and sin.dtype == torch.float32 and cos.is_contiguous() and sin.is_contiguous()
+    assert cos.shape == sin.shape and cos.dim() == 2 and cos.shape[1] == hd and cos.device == sin.device == qkv.device
+    if q_out is None:
+        q_out = torch.empty(T, n_heads * hd, dtype=qkv.dtype, device=qkv.device)
+    assert q_out.shape == (T, n_heads * hd) and q_out.dtype == qkv.dtype and q_out.stride(1) == 1 and q_out.device == qkv.device
+    for t in (row_seq, row_index, row_pos):
+        _i32(t, T, qkv)
+    c = _paged_cache(k_pages, v_pages, block_table)
+    if T:
+        hip.call('vm_kv_append_paged_bf16', C.addressof(c), ptr(qkv), _ld(qkv), ptr(row_seq), ptr(row_index), ptr(row_pos), ptr(cos), ptr(sin),
+                 cos.shape[0], T, n_heads, ptr(q_out), _ld(q_out), ptr(_i32(nrows, 1, qkv)) if nrows is not None else None, stream())
+    return q_out
+
+
+def _weights_view(w: torch.Tensor, n_seq: int, n_kv_heads: int, like: torch.Tensor) -> torch.Tensor:
+    assert w.dtype == torch.float32 and w.dim() == 3 and w.shape[:2] == (n_seq, n_kv_heads) and w.stride(2) == 1 and w.device == like.device, w.shape
+    assert w.shape[2] > 0 and (n_kv_heads == 1 or w.stride(1) >= w.shape[2])
+    return w
+
+
+def attn_paged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: torch.Tensor, cu_q: torch.Tensor,
+               kv_lens: torch.Tensor, scale: float, max_q: int, max_kv: int, *, row_of_pos: torch.Tensor | None = None,
+               weights: torch.Tensor | None = None, weights_out: torch.Tensor | None = None, out: torch.Tensor | None = None):
+    """attention of the newest tokens of every sample over its paged cache, which already holds them (vm_attn_paged_bf16).
+    q [rows, heads hd] bf16 (rotated); positions cu_q[b] .. cu_q[b+1]-1 are the last tokens of the kv_lens[b] cached ones (int32, device);
+    row_of_pos: packed row of a position. max_q / max_kv: host upper bounds of the new and of the cached tokens of a sample.
+    weights [samples, kv heads, >= max_kv] fp32: the attention weight every token has received so far; with this call's added it goes to
+    weights_out (default: in place). -> (out [rows, heads hd], lse fp32 [heads, rows] by position)"""
+    rows = q.shape[0]
+    n_seq = block_table.shape[0]
+    _, hk, _, hd = k_pages.shape
+    assert q.dim() == 2 and q.dtype == torch.bfloat16 and q.stride(1) == 1 and q.shape[1] % hd == 0 and q.device == k_pages.device
+    n_heads = q.shape[1] // hd
+    assert n_heads > 0 and n_heads % hk == 0, f'{n_heads} query heads over {hk} kv heads'
+    assert math.isfinite(scale) and scale > 0 and max_q >= 0 and max_kv >= 0
+    a = hip.AttnPagedArgs()
+    a.cache = _paged_cache(k_pages, v_pages, block_table)
+    if out is None:
+        out = torch.empty(rows, n_heads * hd, dtype=q.dtype, device=q.device)
+    assert out.shape == q.shape and out.dtype == q.dtype and out.stride(1) == 1 and out.device == q.device
+    lse = torch.empty(n_heads, rows, dtype=torch.float32, device=q.device)
+    a.q, a.ldq, a.out, a.ldo = ptr(q), _ld(q), ptr(out), _ld(out)
+    a.cu_q, a.kv_lens = ptr(_i32(cu_q, n_seq + 1, q)), ptr(_i32(kv_lens, n_seq, q))
+    if row_of_pos is not None:
+        a.row_of_pos = ptr(_i32(row_of_pos, rows, q))
+    a.lse, a.ld_lse = ptr(lse), rows
+    a.n_rows, a.max_q, a.max_kv, a.n_heads, a.scale = rows, max_q, max_kv, n_heads, scale
+    if weights is not None:
+        w_out = weights if weights_out is None else weights_out
+        _weights_view(weights, n_seq, hk, q), _weights_view(w_out, n_seq, hk, q)
+        assert w_out.shape == weights.shape and weights.shape[2] >= min(max_kv, block_table.shape[1] * k_pages.shape[2])
+        a.weights, a.weights_out, a.w_cols = ptr(weights), ptr(w_out), weights.shape[2]
+        a.ldw_seq, a.ldw_head, a.ldwo_seq, a.ldwo_head = weights.stride(0), _w_head(weights), w_out.stride(0), _w_head(w_out)
+    else:
+        assert weights_out is None
+    need = C.c_int64(0)
+    hip.call('vm_attn_paged_workspace', C.addressof(a), C.addressof(need))
+    if need.value:
+        ws = torch.empty(need.value, dtype=torch.uint8, device=q.device)
+        a.workspace, a.workspace_bytes = ptr(ws), need.value
+    hip.call('vm_attn_paged_bf16', C.addressof(a), stream())
+    return out, lse
+
+
+def _w_head(w: torch.Tensor) -> int:
+    return w.stride(1) if w.shape[1] > 1 else max(w.stride(1), w.shape[2])
+
+
+def kv_evict_paged(k_pages: torch.Tensor, v_pages: torch.Tensor, weights: torch.Tensor, block_table: torch.Tensor, kv_lens: torch.Tensor,
+                   new_block_table: torch.Tensor, budget: int, recent: int):
+    """of every sample and kv head the `budget` tokens stay that are among the `recent` newest or have received the most attention weight
+    (weights fp32 [samples, kv heads, cols]; ties: the older token), in their order, in the pages of new_block_table — pages that nothing
+    else uses; the old ones are not changed (vm_kv_evict_paged_bf16). -> (new weights, new lens int32 [samples], kept int32 [samples,
+    kv heads, budget]: old indices, -1 behind the last)"""
+    n_seq = block_table.shape[0]
+    _, hk, ps, _ = k_pages.shape
+    c = _paged_cache(k_pages, v_pages, block_table)
+    _weights_view(weights, n_seq, hk, k_pages)
+    _i32(kv_lens, n_seq, k_pages)
+    assert 0 < budget and 0 <= recent <= budget, (budget, recent)
+    assert new_block_table.dtype == torch.int32 and new_block_table.dim() == 2 and new_block_table.shape[0] == n_seq and new_block_table.stride(1) == 1
+    assert new_block_table.device == k_pages.device and new_block_table.data_ptr() != block_table.data_ptr()
+    most = min(budget, block_table.shape[1] * ps, weights.shape[2])
+    assert new_block_table.shape[1] * ps >= most, f'{most} tokens may stay: the new table holds {new_block_table.shape[1] * ps}'
+    new_w = torch.empty(weights.shape, dtype=torch.float32, device=weights.device)
+    new_lens = torch.empty(n_seq, dtype=torch.int32, device=weights.device)
+    kept = torch.empty(n_seq, hk, budget, dtype=torch.int32, device=weights.device)
+    hip.call('vm_kv_evict_paged_bf16', C.addressof(c), ptr(weights), weights.stride(0), _w_head(weights), weights.shape[2], ptr(kv_lens),
+             ptr(new_block_table), new_block_table.stride(0) if n_seq > 1 else new_block_table.shape[1], new_block_table.shape[1], budget, recent,
+             ptr(new_w), new_w.stride(0), _w_head(new_w), ptr(new_lens), ptr(kept), stream())
+    return new_w, new_lens, kept
+
+
 def gemv_supported(x: torch.Tensor, w: torch.Tensor, a2: torch.Tensor | None = None) -> bool:
     return (x.dtype == torch.bfloat16 and w.dtype == torch.bfloat16 and x.dim() == 2 and x.shape[0] <= 16 and x.shape[1] % 64 == 0
             and (a2 is None or a2.shape[1] % 64 == 0))

@@ -1,0 +1,125 @@
+"""Refusals of the paged-cache entry points: everything a host can see is checked before a launch (no GPU needed)."""
+import ctypes as C
+
+import pytest
+import torch
+
+from mmmm_amd import hip, kernels as K
+
+BAD, UNSUPPORTED, OK = -1, -2, 0
+P = 1 << 20                       # an aligned address that is never followed: every call below ends before a launch
+
+
+@pytest.fixture(scope='module')
+def lib():
+    from mmmm_amd import build
+    build.build(verbose=False)
+    return hip.lib()
+
+
+def cache(**kw):
+    c = hip.PagedKVArgs()
+    d = dict(k_pages=P, v_pages=P, ld_page=2 * 64 * 128, n_pages=4, page_size=64, block_table=P, ld_table=3, max_pages=3, n_seq=2, n_kv_heads=2, head_dim=128)
+    d.update(kw)
+    for k, v in d.items():
+        setattr(c, k, v)
+    return c
+
+
+CACHE_BAD = [(dict(k_pages=None), BAD), (dict(v_pages=None), BAD), (dict(block_table=None), BAD), (dict(n_pages=0), BAD), (dict(max_pages=0), BAD),
+             (dict(n_kv_heads=0), BAD), (dict(n_seq=-1), BAD), (dict(head_dim=96), UNSUPPORTED), (dict(head_dim=256), UNSUPPORTED),
+             (dict(page_size=8), UNSUPPORTED), (dict(page_size=48), UNSUPPORTED), (dict(page_size=2048, ld_page=1 << 20), UNSUPPORTED),
+             (dict(k_pages=P + 8), BAD), (dict(ld_page=2 * 64 * 128 - 8), BAD), (dict(ld_page=2 * 64 * 128 + 4), BAD), (dict(ld_table=2), BAD),
+             (dict(max_pages=1 << 26, ld_table=1 << 26), UNSUPPORTED)]
+
+
+def attn(c=None, **kw):
+    a = hip.AttnPagedArgs()
+    a.cache = c or cache()
+    d = dict(q=P, ldq=512, cu_q=P, kv_lens=P, row_of_pos=None, out=P, ldo=512, lse=P, ld_lse=10, n_rows=10, max_q=5, max_kv=100, n_heads=4, scale=0.1,
+             w_cols=0, weights=None, weights_out=None)
+    d.update(kw)
+    for k, v in d.items():
+        setattr(a, k, v)
+    return a
+
+
+@pytest.mark.parametrize('i', range(len(CACHE_BAD)))
+def test_cache_refused_everywhere(lib, i):
+    kw, rc = CACHE_BAD[i]
+    c = cache(**kw)
+    n = C.c_int64(0)
+    a = attn(c)
+    assert lib.vm_attn_paged_bf16(C.addressof(a), None) == rc
+    assert lib.vm_attn_paged_workspace(C.addressof(a), C.addressof(n)) == rc
+    assert lib.vm_kv_append_paged_bf16(C.addressof(c), P, 1024, P, P, P, P, P, 10, 4, 4, P, 512, None, None) == rc
+    assert lib.vm_kv_evict_paged_bf16(C.addressof(c), P, 200, 100, 100, P, 2 * P, 3, 3, 64, 8, 2 * P, 200, 100, 2 * P, P, None) == rc
+
+
+@pytest.mark.parametrize('kw,rc', [
+    (dict(n_heads=3), BAD), (dict(n_heads=0), BAD), (dict(ldq=504), BAD), (dict(ldq=516), BAD), (dict(ldo=508), BAD), (dict(q=P + 2), BAD), (dict(out=P + 8), BAD),
+    (dict(q=None), BAD), (dict(out=None), BAD), (dict(lse=None), BAD), (dict(ld_lse=9), BAD), (dict(cu_q=None), BAD), (dict(kv_lens=None), BAD),
+    (dict(scale=0.0), BAD), (dict(scale=-1.0), BAD), (dict(scale=float('nan')), BAD), (dict(scale=float('inf')), BAD), (dict(max_q=-1), BAD), (dict(max_kv=-1), BAD),
+    (dict(n_rows=-1), BAD), (dict(weights_out=P), BAD), (dict(weights=P, weights_out=P, w_cols=0), BAD),
+    (dict(weights=P, weights_out=P, w_cols=100, ldw_head=99, ldwo_head=100), BAD), (dict(weights=P, weights_out=P, w_cols=100, ldw_head=100, ldwo_head=99), BAD),
+])
+def test_attention_refused(lib, kw, rc):
+    a = attn(**kw)
+    assert lib.vm_attn_paged_bf16(C.addressof(a), None) == rc
+
+
+def test_attention_without_its_workspace_is_refused(lib):
+    a = attn(cache(max_pages=200, ld_table=200, n_pages=4), max_q=1, max_kv=12000)
+    n = C.c_int64(0)
+    assert lib.vm_attn_paged_workspace(C.addressof(a), C.addressof(n)) == OK
+    if n.value:
+        assert lib.vm_attn_paged_bf16(C.addressof(a), None) == BAD
+        a.workspace, a.workspace_bytes = P, n.value - 1
+        assert lib.vm_attn_paged_bf16(C.addressof(a), None) == BAD
+
+
+def test_append_refused(lib):
+    good = [P, 1024, P, P, P, P, P, 10, 4, 4, P, 512, None, None]      # qkv, ld, row_seq, row_index, row_pos, cos, sin, n_pos, rows, n_heads, q_out, ldq
+
+    def call(**kw):
+        names = ['qkv', 'ld', 'row_seq', 'row_index', 'row_pos', 'cos', 'sin', 'n_pos', 'rows', 'n_heads', 'q_out', 'ldq', 'nrows', 'stream']
+        args = [kw.get(n, g) for n, g in zip(names, good)]
+        c = cache()
+        return lib.vm_kv_append_paged_bf16(C.addressof(c), *args)
+    for kw in (dict(qkv=None), dict(qkv=P + 2), dict(ld=1016), dict(ld=1028), dict(row_seq=None), dict(row_index=None), dict(row_pos=None), dict(cos=None),
+               dict(sin=None), dict(sin=P + 4), dict(n_pos=0), dict(rows=-1), dict(n_heads=0), dict(q_out=None), dict(ldq=504)):
+        assert call(**kw) == BAD, kw
+    assert call(rows=0) == OK
+
+
+def test_evict_refused(lib):
+    names = ['weights', 'ldw_seq', 'ldw_head', 'w_cols', 'lens', 'new_table', 'ld_new', 'new_pages', 'budget', 'recent', 'new_w', 'ldn_seq', 'ldn_head', 'new_lens', 'kept']
+    good = [P, 200, 100, 100, P, 2 * P, 3, 3, 64, 8, 2 * P, 200, 100, 2 * P, P]
+    for kw in (dict(weights=None), dict(ldw_head=99), dict(w_cols=0), dict(lens=None), dict(new_table=None), dict(ld_new=2), dict(new_pages=0), dict(budget=0),
+               dict(recent=-1), dict(recent=65), dict(new_w=None), dict(ldn_head=99), dict(new_lens=None), dict(kept=None), dict(new_w=P), dict(new_lens=P), dict(new_table=P)):
+        c = cache()
+        assert lib.vm_kv_evict_paged_bf16(C.addressof(c), *[kw.get(n, g) for n, g in zip(names, good)], None) == BAD, kw
+
+
+def test_struct_layouts(lib):
+    assert C.sizeof(hip.PagedKVArgs) == 64 and hip.PagedKVArgs.block_table.offset == 32 and hip.PagedKVArgs.head_dim.offset == 60
+    assert C.sizeof(hip.AttnPagedArgs) == 224 and hip.AttnPagedArgs.n_rows.offset == 136 and hip.AttnPagedArgs.weights.offset == 160
+
+
+def test_wrappers_refuse_what_they_can_see():
+    k = torch.zeros(4, 2, 16, 64, dtype=torch.bfloat16)
+    t = torch.zeros(2, 3, dtype=torch.int32)
+    q = torch.zeros(3, 4 * 64, dtype=torch.bfloat16)
+    cu, lens = torch.zeros(3, dtype=torch.int32), torch.zeros(2, dtype=torch.int32)
+    ok = dict(q=q, k=k, v=k.clone(), t=t, cu=cu, lens=lens, scale=0.1)
+
+    def call(**kw):
+        d = {**ok, **kw}
+        return K.attn_paged(d['q'], d['k'], d['v'], d['t'], d['cu'], d['lens'], d['scale'], 3, 40)
+    for kw in (dict(q=q.float()), dict(q=q[:, :200]), dict(k=k.float(), v=k.float()), dict(v=k[:3]), dict(k=k.transpose(1, 2), v=k.transpose(1, 2)),
+               dict(t=t.long()), dict(scale=0.0), dict(scale=float('nan')), dict(k=k[..., :48].contiguous(), v=k[..., :48].contiguous()),
+               dict(k=k[:, :, :12].contiguous(), v=k[:, :, :12].contiguous())):
+        with pytest.raises(AssertionError):
+            call(**kw)
+    with pytest.raises(hip.HipError):                      # host tensors: there is no CPU path
+        call()

@@ -1,0 +1,263 @@
+"""Paged-cache operators on the MI355X against their 64-bit statements (tests/_paged.py), elementwise, with tolerances that count the
+roundings. Rows of the pools that hold no token are NaN throughout: nothing may read them as data."""
+import pytest
+import torch
+
+from tests import _paged as R
+
+pytestmark = pytest.mark.gpu
+NAN = float('nan')
+
+
+@pytest.fixture(scope='module')
+def K():
+    from mmmm_amd import kernels
+    return kernels
+
+
+def close(got, want, tol, what=''):
+    got = got.detach().double().cpu()
+    assert got.shape == want.shape, (what, got.shape, want.shape)
+    assert torch.equal(got.isfinite(), want.isfinite()), what
+    fin = want.isfinite()
+    assert torch.equal(got[~fin], want[~fin]), what
+    err = (got[fin] - want[fin]).abs() - tol[fin]
+    assert err.numel() == 0 or float(err.max()) <= 0, (what, float(err.max()), float((got[fin] - want[fin]).abs().max()))
+
+
+def i32(x, dev):
+    return torch.tensor(x, dtype=torch.int32, device=dev)
+
+
+def run_attention(K, dev, new, lens, H, hk, hd, page, packed=False, weights=False, seed=0, absent=(), scale=None, cols=None, qs=1.5):
+    g = torch.Generator().manual_seed(seed)
+    k, v, table = R.make_cache(lens, hk, hd, page, g, cols=cols)
+    for b, c, val in absent:
+        table[b, c] = val
+    T = sum(new)
+    rows = T + 5                                                          # rows of no position behind the last one
+    q = (torch.randn(rows, H * hd, generator=g) * qs).bfloat16()
+    rop = torch.randperm(rows, generator=g)[:rows].to(torch.int32) if packed else None
+    scale = hd ** -0.5 if scale is None else scale
+    w = torch.rand(len(lens), hk, max(1, max(lens)) + 3, generator=g) if weights else None
+    want = R.attention(q, k, v, table, new, lens, scale, rop, w)
+    big = torch.full((rows, H * hd + 24), 7.0, dtype=torch.bfloat16, device=dev)      # strided q and out
+    big[:, 8:8 + H * hd] = q.to(dev)
+    out = torch.full((rows, H * hd + 8), 3.0, dtype=torch.bfloat16, device=dev)
+    cu = [0]
+    for n in new:
+        cu.append(cu[-1] + n)
+    kw = {}
+    if weights:
+        wd = w.to(dev)
+        wo = torch.full_like(wd, -1.0)
+        kw = dict(weights=wd, weights_out=wo)
+    args = (big[:, 8:8 + H * hd], k.to(dev), v.to(dev), table.to(dev), i32(cu, dev), i32(lens, dev), scale, max(new), max(lens))
+    o, lse = K.attn_paged(*args, row_of_pos=rop.to(dev) if packed else None, out=out[:, :H * hd], **kw)
+    pos = torch.arange(T)
+    r = rop.long()[pos] if packed else pos
+    close(o.cpu()[r], want[0][r], want[1][r], 'out')
+    close(lse.cpu()[:, :T], want[2][:, :T], want[3][:, :T], 'lse')
+    rest = torch.ones(rows, dtype=torch.bool)
+    rest[r] = False
+    assert (o.cpu()[rest] == 3.0).all() and (out[:, H * hd:] == 3.0).all()            # left as they were
+    if weights:
+        for b, L in enumerate(lens):
+            close(wo[b, :, :L], want[4][b, :, :L], want[5][b, :, :L], 'weights')
+            assert (wo[b, :, L:] == -1.0).all()
+        assert torch.equal(wd.cpu(), w)
+    o2, lse2 = K.attn_paged(*args, row_of_pos=rop.to(dev) if packed else None, **kw)
+    assert torch.equal(o2.cpu()[r], o.cpu()[r]) and torch.equal(lse2[:, :T], lse[:, :T])      # same bits again
+    return o
+
+
+# (new tokens, cached tokens), query heads, kv heads, width, page
+ATTN = [
+    ([1], [1], 1, 1, 128, 16),
+    ([1, 1, 1], [1, 64, 65], 4, 4, 128, 64),
+    ([1, 1, 1, 1], [485, 31, 2, 257], 3, 3, 128, 32),
+    ([1, 1], [1000, 777], 8, 1, 64, 16),
+    ([1, 1], [300, 1], 12, 3, 32, 256),
+    ([2, 1, 5], [130, 7, 5], 6, 2, 128, 128),
+    ([7, 0, 3], [40, 0, 3], 2, 2, 64, 16),
+    ([16, 17], [16, 400], 4, 2, 128, 64),
+    ([33, 64], [97, 64], 2, 1, 32, 32),
+    ([37, 30, 1], [2086, 200, 90], 2, 2, 128, 64),
+    ([100, 65], [100, 321], 4, 1, 128, 16),
+    ([129, 257], [129, 300], 3, 3, 128, 64),
+    ([300], [300], 8, 2, 64, 128),
+    ([513], [1200], 2, 1, 128, 64),
+    ([200, 310], [456, 310], 2, 2, 32, 1024),
+]
+
+
+@pytest.mark.parametrize('case', ATTN, ids=[str(i) for i in range(len(ATTN))])
+@pytest.mark.parametrize('packed', [False, True])
+@pytest.mark.parametrize('weights', [False, True])
+def test_attention(dev, K, case, packed, weights):
+    run_attention(K, dev, *case, packed=packed, weights=weights, seed=len(case[0]))
+
+
+@pytest.mark.parametrize('new,lens', [([1], [5000]), ([3], [9001]), ([40], [3000]), ([70, 1], [4097, 1])])
+def test_attention_long_cache(dev, K, new, lens):
+    run_attention(K, dev, new, lens, 4, 2, 128, 64, packed=True, weights=True)
+
+
+@pytest.mark.parametrize('new,lens', [([5, 2], [3, 0]), ([40], [7]), ([300, 1], [270, 0])])
+@pytest.mark.parametrize('hd', [64, 128])
+def test_rows_that_see_nothing(dev, K, new, lens, hd):
+    """more new tokens than cached ones: the first of them see no token at all -> zeros, lse -inf"""
+    run_attention(K, dev, new, lens, 4, 2, hd, 16, weights=True)
+
+
+@pytest.mark.parametrize('new', [1, 9, 80, 300])
+@pytest.mark.parametrize('page', [16, 64, 256])
+def test_absent_pages_are_masked(dev, K, new, page):
+    """first, middle and last pages missing (-1, far out of range): never read through, their tokens are not there"""
+    absent = [(0, 0, -1), (0, 1, 2 ** 31 - 1), (1, 0, -2 ** 31), (0, 512 // page - 1, 10 ** 6)]
+    run_attention(K, dev, [new, min(new, 100)], [512, 300], 2, 1, 128, page, weights=True, absent=absent)
+    run_attention(K, dev, [new], [min(512, page)], 2, 2, 64, page, absent=[(0, 0, -7)]) if new <= page else None      # nothing left at all
+
+
+def test_large_scores(dev, K):
+    """scores of hundreds: the running maximum has to move, and nothing may overflow"""
+    for new in (1, 20, 200):
+        run_attention(K, dev, [new], [700], 2, 1, 128, 64, weights=True, qs=60.0)
+
+
+def test_other_scale(dev, K):
+    for new in (1, 70):
+        run_attention(K, dev, [new], [333], 2, 2, 128, 64, scale=0.7)
+
+
+def test_attention_of_nothing(dev, K):
+    g = torch.Generator().manual_seed(0)
+    k, v, table = (t.to(dev) for t in R.make_cache([40], 2, 64, 16, g))
+    q = torch.zeros(0, 2 * 64, dtype=torch.bfloat16, device=dev)
+    o, lse = K.attn_paged(q, k, v, table, i32([0, 0], dev), i32([40], dev), 0.1, 0, 40)
+    assert o.shape == (0, 128) and lse.shape == (2, 0)
+
+
+@pytest.mark.parametrize('hd', [32, 64, 128])
+@pytest.mark.parametrize('H,hk,page', [(1, 1, 16), (32, 32, 64), (6, 2, 256), (5, 5, 32)])
+def test_append(dev, K, hd, H, hk, page):
+    g = torch.Generator().manual_seed(hd + H)
+    lens = [page * 2 + 3, 1, 70]
+    k, v, table = R.make_cache(lens, hk, hd, page, g, poison=False)
+    table[2, 0] = -1                                                        # a page that is not there
+    rows = []
+    for b, L in enumerate(lens):
+        rows += [(b, j) for j in range(max(0, L - 40), L)]
+    rows += [(-1, 0), (3, 0), (0, -1), (0, table.shape[1] * page), (2 ** 31 - 1, 5)]      # not stored
+    rows = [rows[i] for i in torch.randperm(len(rows), generator=g).tolist()]
+    T = len(rows)
+    seq, idx = (torch.tensor(c, dtype=torch.int32) for c in zip(*rows))
+    pos = torch.randint(-2, 60, (T,), generator=g).to(torch.int32)           # clamped to the table
+    n_pos = 50
+    ang = torch.rand(n_pos, hd, generator=g) * 6
+    cos, sin = ang.cos(), ang.sin()
+    qkv = torch.randn(T + 2, (H + 2 * hk) * hd + 8, generator=g).bfloat16()
+    for nrows in (None, T - 7):
+        n = T if nrows is None else nrows
+        want = R.append(qkv[:n, :(H + 2 * hk) * hd].contiguous(), seq[:n], idx[:n], table, k, v, pos[:n], cos, sin, H)
+        kd, vd, x = k.to(dev), v.to(dev), qkv.to(dev)
+        q = torch.full((T + 1, H * hd), 5.0, dtype=torch.bfloat16, device=dev)
+        K.kv_append_paged(x[:T, :(H + 2 * hk) * hd], seq.to(dev), idx.to(dev), table.to(dev), kd, vd, pos.to(dev), cos.to(dev), sin.to(dev), H,
+                          nrows=None if nrows is None else i32([nrows], dev), q_out=q[:T])
+        close(q[:n], want[0], want[1], 'q')
+        close(kd, want[2], want[3], 'k')
+        assert torch.equal(vd.cpu().double(), want[4])
+        assert (q[n:] == 5.0).all() and torch.equal(x.cpu(), qkv)
+
+
+@pytest.mark.parametrize('lens,budget,recent', [([600], 512, 64), ([1, 0, 40], 8, 8), ([5000, 33, 512], 100, 0), ([64, 65, 66], 64, 1), ([300, 20], 1, 0),
+                                                ([2100], 2099, 700)])
+@pytest.mark.parametrize('hd,hk,page', [(128, 3, 64), (32, 1, 16)])
+@pytest.mark.parametrize('kind', ['random', 'ties', 'odd'])
+def test_evict(dev, K, lens, budget, recent, hd, hk, page, kind):
+    g = torch.Generator().manual_seed(sum(lens) + budget)
+    both = list(lens) + [min(n, budget) for n in lens]                       # old pages and new ones from one pool
+    k, v, tab = R.make_cache(both, hk, hd, page, g)
+    table, new_table = tab[:len(lens)], tab[len(lens):].clone()
+    cols = max(lens) + 2
+    w = torch.rand(len(lens), hk, cols, generator=g)
+    if kind == 'ties':
+        w = (w * 3).floor()
+    if kind == 'odd':
+        w = torch.where(w < 0.2, NAN, torch.where(w < 0.4, float('-inf'), torch.where(w < 0.5, -0.0, torch.where(w < 0.6, 0.0, torch.where(w > 0.97, float('inf'), -w)))))
+        if max(lens) > page:
+            table[0, 0] = -1
+            table[len(lens) - 1, 0] = 2 ** 30
+    kept, new = R.evict(w, table, k.shape[0], page, lens, budget, recent)
+    kd, vd = k.to(dev), v.to(dev)
+    got_w, got_l, got_k = K.kv_evict_paged(kd, vd, w.to(dev), table.to(dev), i32(lens, dev), new_table.to(dev), budget, recent)
+    assert got_l.cpu().tolist() == new
+    ke, ve = k.clone(), v.clone()
+    for b in range(len(lens)):
+        for h in range(hk):
+            idx = torch.tensor(kept[b][h], dtype=torch.long)
+            n = len(idx)
+            assert got_k[b, h].cpu().tolist() == idx.tolist() + [-1] * (budget - n)
+            a, c = got_w[b, h].cpu(), w[b, h][idx]
+            assert torch.equal(a[:n].view(torch.int32), c.view(torch.int32)) and (a[n:] == 0).all()
+            at = torch.arange(n)
+            src, dst = table[b].long()[idx // page], new_table[b].long()[at // page]
+            ke[dst, h, at % page], ve[dst, h, at % page] = k[src, h, idx % page], v[src, h, idx % page]
+    assert torch.equal(kd.cpu().view(torch.int16), ke.view(torch.int16)) and torch.equal(vd.cpu().view(torch.int16), ve.view(torch.int16))
+
+
+def test_append_attend_evict_together(dev, K):
+    """a conversation as the cache lives it: prompt, follow-up, single tokens, eviction, more tokens — against the same in 64 bits"""
+    g = torch.Generator().manual_seed(11)
+    H, hk, hd, page, B = 4, 2, 64, 16, 2
+    pages = 64
+    perm = torch.randperm(pages, generator=g).to(torch.int32)
+    table, free = torch.full((B, 12), -1, dtype=torch.int32), perm.tolist()
+    for b in range(B):
+        table[b, :12] = torch.tensor([free.pop() for _ in range(12)], dtype=torch.int32)
+    k = torch.full((pages, hk, page, hd), NAN).bfloat16()
+    v = k.clone()
+    kd, vd = k.to(dev), v.to(dev)
+    ang = torch.arange(256)[:, None] * torch.cat([1.0 / 10000 ** (torch.arange(0, hd, 2) / hd)] * 2)[None]
+    cos, sin = ang.cos(), ang.sin()
+    lens, w, wd = [0, 0], torch.zeros(B, hk, 192), torch.zeros(B, hk, 192, device=dev)
+    seen = [0, 0]
+    for step, new in enumerate([[100, 71], [9, 20], [1, 1], [1, 1], 'evict', [1, 1], [30, 2]]):
+        if new == 'evict':
+            nt = torch.full((B, 12), -1, dtype=torch.int32)
+            for b in range(B):
+                nt[b] = torch.tensor([free.pop() for _ in range(12)], dtype=torch.int32)
+            kept, new_lens = R.evict(wd.cpu(), table, pages, page, lens, 48, 8)           # the choice is exact given the weights
+            wd2, ld, got = K.kv_evict_paged(kd, vd, wd, table.to(dev), i32(lens, dev), nt.to(dev), 48, 8)
+            assert ld.cpu().tolist() == new_lens
+            k2, v2, w2 = k.clone(), v.clone(), torch.zeros_like(w)
+            for b in range(B):
+                for h in range(hk):
+                    idx = torch.tensor(kept[b][h])
+                    assert got[b, h].cpu().tolist() == kept[b][h]
+                    at = torch.arange(len(idx))
+                    k2[nt[b].long()[at // page], h, at % page] = k[table[b].long()[idx // page], h, idx % page]
+                    v2[nt[b].long()[at // page], h, at % page] = v[table[b].long()[idx // page], h, idx % page]
+                    w2[b, h, :len(idx)] = w[b, h][idx]
+            k, v, w, wd, table, lens = k2, v2, w2, wd2, nt, new_lens
+            continue
+        T = sum(new)
+        qkv = torch.randn(T, (H + 2 * hk) * hd, generator=g).bfloat16()
+        rows = [(b, lens[b] + i, seen[b] + i) for b in range(B) for i in range(new[b])]
+        seq, idx, pos = (torch.tensor(c, dtype=torch.int32) for c in zip(*rows))
+        lens = [a + n for a, n in zip(lens, new)]
+        seen = [a + n for a, n in zip(seen, new)]
+        q = K.kv_append_paged(qkv.to(dev), seq.to(dev), idx.to(dev), table.to(dev), kd, vd, pos.to(dev), cos.to(dev), sin.to(dev), H)
+        qw, qt, kw, kt, vw = R.append(qkv, seq, idx, table, k, v, pos, cos, sin, H)
+        close(q, qw, qt)
+        for b in range(B):
+            for h in range(hk):
+                close(R.tokens(kd.cpu(), table, b, lens[b], h)[0], R.tokens(kw, table, b, lens[b], h)[0], R.tokens(kt, table, b, lens[b], h)[0])
+        k, v = kd.cpu(), vd.cpu()                                                        # what was stored is the next stage's input
+        cu = [0, new[0], T]
+        want = R.attention(q.cpu(), k, v, table, new, lens, hd ** -0.5, None, wd.cpu())
+        o, lse = K.attn_paged(q, kd, vd, table.to(dev), i32(cu, dev), i32(lens, dev), hd ** -0.5, max(new), max(lens), weights=wd)
+        close(o, want[0], want[1], f'step {step}')
+        close(lse, want[2], want[3])
+        close(wd, want[4], want[5])
+        w = wd.cpu()
