@@ -4,6 +4,7 @@
 // Query rows of one kv head are taken together: row r of (sample b, kv head hk) is query i = r / G of head hk G + r % G (G heads share the
 // kv head), so grouped heads read K and V once. Query i sees the tokens j <= L - n + i.
 #include "paged.hpp"
+#include "vm_tile.hpp"
 
 namespace {
 
@@ -20,6 +21,11 @@ struct AttnPagedP {
   int max_q, max_kv;
   float scale;
   const float* w_in; float* w_out; int64_t ldw_seq, ldw_head, ldwo_seq, ldwo_head; int w_cols;
+  // split form: n_split key splits; workspace of s_rows query rows per (sample, kv head)
+  int n_split, s_rows, s_ld;
+  float* part;                // [.., s_rows, n_split, hd + 4]: max, sum, -, -, O
+  float* s_ws;                // [.., s_rows, s_ld] scores (log2 domain), if the received weights are asked for
+  float* l2_ws;               // [.., s_rows] log2 of the rows' sums
 };
 
 // what one sample brings, read from the device and held inside the buffers' bounds
@@ -37,6 +43,299 @@ __device__ __forceinline__ int phys_row(const AttnPagedP& p, int pos) {      // 
   return (unsigned)r < (unsigned)p.n_rows ? r : -1;
 }
 
+// ----------------------------------------------------------------------------- few query rows: keys split over waves and workgroups
+// HBM-bound: K and V of a sample are read once (4 hd bytes per token and kv head), the arithmetic is small beside it. A wave owns 16 query
+// rows and walks blocks of 32 keys:
+//   S^T[key][row] = K Q^T with v_mfma_f32_16x16x32_bf16: a lane loads its 16-byte pieces of K straight from the page as the A operand (K never
+//   touches LDS); the row sits on the lane (ln = lane & 15), so the running maximum and sum are per-lane scalars plus two lane swaps;
+//   O^T[d][row] += V^T P^T: V goes page -> registers -> the wave's own 8 KiB of LDS and comes back transposed (ds_read_b64_tr_b16); the two
+//   stacked score tiles ARE the B operand. P is taken as two bf16 terms (its rounding and what that left out: 16 significant bits), the
+//   second product costs matrix time that the loads leave idle, and the only rounding the result sees is its own.
+// The next block's K and V are in flight while one is computed; page numbers are fetched two blocks ahead through the scalar cache.
+// A workgroup has four waves: RT row tiles x 4 / RT key streams; its key streams are merged in LDS, and if the keys were split over
+// workgroups too the partial (max, sum, O) of each goes to the workspace and attn_paged_join_k joins them in a fixed order.
+constexpr int SP_WAVES = 4;
+
+__device__ __forceinline__ void swap16(float& a, float& b) { asm("s_nop 1\n\tv_permlane16_swap_b32 %0, %1" : "+v"(a), "+v"(b)); }
+__device__ __forceinline__ void swap32(float& a, float& b) { asm("s_nop 1\n\tv_permlane32_swap_b32 %0, %1" : "+v"(a), "+v"(b)); }
+__device__ __forceinline__ float max_over_g(float x) {        // maximum over the lanes that share lane & 15
+  float a = x, b = x;
+  swap16(a, b);
+  a = b = fmaxf(a, b);
+  asm volatile("" : "+v"(a), "+v"(b));
+  swap32(a, b);
+  return fmaxf(a, b);
+}
+__device__ __forceinline__ float sum_over_g(float x) {
+  float a = x, b = x;
+  swap16(a, b);
+  a = b = a + b;
+  asm volatile("" : "+v"(a), "+v"(b));
+  swap32(a, b);
+  return a + b;
+}
+__device__ __forceinline__ float fast_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
+
+template <int HD>
+struct KVBlock {                                    // 32 keys of one kv head on their way through a wave
+  static constexpr int KS = HD / 32, CPR = HD / 8, RPI = 64 / CPR, NV = 32 / RPI;
+  i32x4_t k[2][KS], v[NV];
+};
+
+// the two page numbers of a 32-key block (pages of 16 rows end inside it); -1 behind the last key
+struct PagePair { int a, b; };
+__device__ __forceinline__ PagePair block_pages(const AttnPagedP& p, const int32_t* table, int j0, int kv_end) {
+  PagePair r = {-1, -1};
+  if (j0 < kv_end) r.a = table[j0 >> p.c.shift];
+  if (j0 + 16 < kv_end) r.b = table[(j0 + 16) >> p.c.shift];
+  if (!page_ok(r.a, p.c.n_pages)) r.a = -1;
+  if (!page_ok(r.b, p.c.n_pages)) r.b = -1;
+  return r;
+}
+
+template <int HD>
+__device__ __forceinline__ void load_block(const AttnPagedP& p, KVBlock<HD>& x, PagePair pg, int hk, int j0, int kv_end, int lane) {
+  typedef KVBlock<HD> B;
+  const int ln = lane & 15, g = lane >> 4;
+  const i32x4_t zero = {0, 0, 0, 0};
+#pragma unroll
+  for (int jj = 0; jj < 2; ++jj) {
+    const int page = jj ? pg.b : pg.a, row = (j0 + 16 * jj) & p.c.mask;
+    const unsigned short* kb = p.c.k + page_row(page < 0 ? 0 : page, p.c.ld_page, hk, row, p.c.shift, HD) + ln * HD + 8 * g;
+#pragma unroll
+    for (int s = 0; s < B::KS; ++s) x.k[jj][s] = page < 0 ? zero : *reinterpret_cast<const i32x4_t*>(kb + 32 * s);
+  }
+#pragma unroll
+  for (int i = 0; i < B::NV; ++i) {
+    const int r = i * B::RPI + lane / B::CPR;        // row of the block
+    const int page = r < 16 ? pg.a : pg.b, row = (j0 + r) & p.c.mask;
+    x.v[i] = zero;                                   // rows behind the last token that is seen hold anything: they count as zeros
+    if (page >= 0 && j0 + r < kv_end)
+      x.v[i] = *reinterpret_cast<const i32x4_t*>(p.c.v + page_row(page, p.c.ld_page, hk, row, p.c.shift, HD) + (lane & (B::CPR - 1)) * 8);
+  }
+}
+
+template <int HD, int RT>
+__global__ __launch_bounds__(SP_WAVES * 64, 2) void attn_paged_split_k(const AttnPagedP p) {
+  typedef KVBlock<HD> B;
+  constexpr int KW = SP_WAVES / RT;                  // key streams of the workgroup
+  constexpr int ND = HD / 16;
+  __shared__ __attribute__((aligned(1024))) char smem[SP_WAVES][32 * ROWB];
+  __shared__ float red[SP_WAVES][2][16];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int ln = lane & 15, g = lane >> 4;
+  const int hk = blockIdx.y, b = blockIdx.z;
+  const int rt = wave % RT, kw = wave / RT;
+  const int tile = blockIdx.x / p.n_split, split = blockIdx.x % p.n_split;
+  const SeqInfo s = seq_info(p, b);
+  const int R = min(s.nq, p.max_q) * p.G, row0 = (tile * RT + rt) * 16, wg_row0 = tile * RT * 16;
+  if (wg_row0 >= R) return;
+  const int r = row0 + ln;
+  const bool live = r < R;
+  const int i = live ? r / p.G : 0, h = hk * p.G + (live ? r - i * p.G : 0);
+  const int prow = live ? phys_row(p, s.p0 + i) : -1;
+  const int lim = live ? s.len - s.nq + i : -1;      // last token this row sees
+  const int lim_min = s.len - s.nq + min(row0, R - 1) / p.G;
+  const int kv_end = max(0, s.len - s.nq + (min(wg_row0 + RT * 16, R) - 1) / p.G + 1);
+  // this workgroup's blocks
+  const int nblk = (kv_end + 31) / 32, per = (nblk + p.n_split - 1) / p.n_split;
+  const int blk0 = min(split * per, nblk), blk1 = row0 < R ? min(blk0 + per, nblk) : blk0;
+
+  bf16x8_t qf[B::KS];
+#pragma unroll
+  for (int t = 0; t < B::KS; ++t) {
+    i32x4_t v = {0, 0, 0, 0};
+    if (prow >= 0) v = *reinterpret_cast<const i32x4_t*>(p.q + prow * p.ldq + h * HD + 32 * t + 8 * g);
+    qf[t] = __builtin_bit_cast(bf16x8_t, v);
+  }
+  f32x4_t o[ND];
+#pragma unroll
+  for (int t = 0; t < ND; ++t) o[t] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
+  float m = -INFINITY, l = 0.f;
+  const float sc = p.scale * LOG2E;
+  const int32_t* table = p.c.table + b * p.c.ld_table;
+  char* tv = smem[wave];
+  float* srow = p.s_ws ? p.s_ws + (((int64_t)b * p.c.n_kv_heads + hk) * p.s_rows + r) * p.s_ld : nullptr;
+
+  KVBlock<HD> cur, nxt;
+  int blk = blk0 + kw;
+  PagePair pg = block_pages(p, table, blk * 32, kv_end);
+  if (blk < blk1) load_block<HD>(p, cur, pg, hk, blk * 32, kv_end, lane);
+  PagePair pg1 = block_pages(p, table, (blk + KW) * 32, kv_end);
+  for (; blk < blk1; blk += KW) {
+    const PagePair pg2 = block_pages(p, table, (blk + 2 * KW) * 32, kv_end);
+    if (blk + KW < blk1) load_block<HD>(p, nxt, pg1, hk, (blk + KW) * 32, kv_end, lane);
+    const int j0 = blk * 32;
+    f32x4_t sa[2];
+#pragma unroll
+    for (int jj = 0; jj < 2; ++jj) {
+      sa[jj] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int t = 0; t < B::KS; ++t) sa[jj] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, cur.k[jj][t]), qf[t], sa[jj], 0, 0, 0);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) sa[jj][e] *= sc;
+    }
+    if (j0 + 31 > lim_min || pg.a < 0 || pg.b < 0) {
+#pragma unroll
+      for (int jj = 0; jj < 2; ++jj)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if ((jj ? pg.b : pg.a) < 0 || j0 + 16 * jj + 4 * g + e > lim) sa[jj][e] = -INFINITY;
+    }
+    if (srow && live) {
+#pragma unroll
+      for (int jj = 0; jj < 2; ++jj)
+        if (j0 + 16 * jj + 4 * g < p.s_ld) *reinterpret_cast<f32x4_t*>(srow + j0 + 16 * jj + 4 * g) = sa[jj];
+    }
+    // V -> LDS while the scores settle
+#pragma unroll
+    for (int t = 0; t < B::NV; ++t)
+      *reinterpret_cast<i32x4_t*>(tv + tile_off16(t * B::RPI + lane / B::CPR, lane & (B::CPR - 1))) = cur.v[t];
+    float mx = fmaxf(fmaxf(fmaxf(sa[0][0], sa[0][1]), fmaxf(sa[0][2], sa[0][3])), fmaxf(fmaxf(sa[1][0], sa[1][1]), fmaxf(sa[1][2], sa[1][3])));
+    mx = max_over_g(mx);
+    if (__builtin_amdgcn_ballot_w64(mx > m) != 0) {
+      const float mn = fmaxf(m, mx), alpha = fast_exp2(m - (mn == -INFINITY ? 0.f : mn));
+      m = mn;
+      l *= alpha;
+#pragma unroll
+      for (int t = 0; t < ND; ++t)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[t][e] *= alpha;
+    }
+    const float base = m == -INFINITY ? 0.f : m;
+    u16x8_t hi, lo;
+#pragma unroll
+    for (int jj = 0; jj < 2; ++jj)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float x = fast_exp2(sa[jj][e] - base);
+        l += x;
+        hi[4 * jj + e] = f2bf(x);
+        lo[4 * jj + e] = f2bf(x - bf2f(hi[4 * jj + e]));
+      }
+    const bf16x8_t ph = __builtin_bit_cast(bf16x8_t, hi), pl = __builtin_bit_cast(bf16x8_t, lo);
+#pragma unroll
+    for (int t = 0; t < ND; ++t) {
+      const bf16x8_t vf = frag16_tr(tv, 0, t, lane);
+      o[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, ph, o[t], 0, 0, 0);
+      o[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pl, o[t], 0, 0, 0);
+    }
+    cur = nxt;
+    pg = pg1;
+    pg1 = pg2;
+  }
+  l = sum_over_g(l);
+  // ---- the key streams of a row tile meet in LDS: wave 0 of them adds up in order
+  if (KW > 1) {
+    if (g == 0) { red[wave][0][ln] = m; red[wave][1][ln] = l; }
+    __syncthreads();
+    float mm = m;
+#pragma unroll
+    for (int k = 0; k < KW; ++k) mm = fmaxf(mm, red[k * RT + rt][0][ln]);
+    const float base = mm == -INFINITY ? 0.f : mm, f = fast_exp2(m - base);
+    float ll = 0.f;
+#pragma unroll
+    for (int k = 0; k < KW; ++k) ll += red[k * RT + rt][1][ln] * fast_exp2(red[k * RT + rt][0][ln] - base);
+    m = mm;
+    l = ll;
+    float* slab = reinterpret_cast<float*>(smem[wave]);          // O^T of this wave, [d][row]
+#pragma unroll
+    for (int t = 0; t < ND; ++t)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) slab[(16 * t + 4 * g + e) * 16 + ln] = o[t][e] * f;
+    __syncthreads();
+    if (kw != 0) return;
+#pragma unroll
+    for (int t = 0; t < ND; ++t)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        float x = 0.f;
+#pragma unroll
+        for (int k = 0; k < KW; ++k) x += reinterpret_cast<const float*>(smem[k * RT + rt])[(16 * t + 4 * g + e) * 16 + ln];
+        o[t][e] = x;
+      }
+  }
+  if (!live) return;
+  if (p.n_split == 1) {
+    const bool some = !(l == 0.f);
+    const float inv = some ? 1.f / l : 0.f;
+    if (prow >= 0) {
+#pragma unroll
+      for (int t = 0; t < ND; ++t) {
+        const u16x4_t w = {f2bf(o[t][0] * inv), f2bf(o[t][1] * inv), f2bf(o[t][2] * inv), f2bf(o[t][3] * inv)};
+        *reinterpret_cast<u16x4_t*>(p.out + prow * p.ldo + h * HD + 16 * t + 4 * g) = some ? w : (u16x4_t){0, 0, 0, 0};
+      }
+    }
+    const float l2 = some ? m + log2f(l) : -INFINITY;
+    if (g == 0) {
+      p.lse[h * p.ld_lse + s.p0 + i] = l2 * LN2;
+      if (p.s_ws) p.l2_ws[((int64_t)b * p.c.n_kv_heads + hk) * p.s_rows + r] = l2;
+    }
+  } else {
+    float* part = p.part + ((((int64_t)b * p.c.n_kv_heads + hk) * p.s_rows + r) * p.n_split + split) * (HD + 4);
+    if (g == 0) { part[0] = m; part[1] = l; }
+#pragma unroll
+    for (int t = 0; t < ND; ++t) *reinterpret_cast<f32x4_t*>(part + 4 + 16 * t + 4 * g) = o[t];
+  }
+}
+
+// joins the key splits of a query row: one wave per row, HD / 64 (at least 1) elements per lane, the splits in their order
+template <int HD>
+__global__ __launch_bounds__(256) void attn_paged_join_k(const AttnPagedP p) {
+  constexpr int E = HD >= 128 ? 2 : 1;
+  const int lane = threadIdx.x & 63, hk = blockIdx.y, b = blockIdx.z;
+  const int r = blockIdx.x * 4 + (threadIdx.x >> 6);
+  const SeqInfo s = seq_info(p, b);
+  if (r >= min(s.nq, p.max_q) * p.G) return;
+  const int i = r / p.G, h = hk * p.G + r % p.G;
+  const int64_t slot = ((int64_t)b * p.c.n_kv_heads + hk) * p.s_rows + r;
+  const float* part = p.part + slot * p.n_split * (HD + 4);
+  float m = -INFINITY;
+  for (int k = lane; k < p.n_split; k += 64) m = fmaxf(m, part[k * (HD + 4)]);
+  m = wave_max(m);
+  const float base = m == -INFINITY ? 0.f : m;
+  float l = 0.f, o[E] = {0.f};
+  const int d = lane * E;
+  for (int k = 0; k < p.n_split; ++k) {
+    const float* q = part + k * (HD + 4);
+    const float f = fast_exp2(q[0] - base);
+    l += f * q[1];
+    if (d < HD) {
+#pragma unroll
+      for (int e = 0; e < E; ++e) o[e] = fmaf(f, q[4 + d + e], o[e]);
+    }
+  }
+  const bool some = !(l == 0.f);
+  const float inv = some ? 1.f / l : 0.f, l2 = some ? m + log2f(l) : -INFINITY;
+  const int prow = phys_row(p, s.p0 + i);
+  if (prow >= 0 && d < HD) {
+#pragma unroll
+    for (int e = 0; e < E; ++e) p.out[prow * p.ldo + h * HD + d + e] = some ? f2bf(o[e] * inv) : (unsigned short)0;
+  }
+  if (lane == 0) {
+    p.lse[h * p.ld_lse + s.p0 + i] = l2 * LN2;
+    if (p.s_ws) p.l2_ws[slot] = l2;
+  }
+}
+
+// received weights from the scores that the split form left behind: one thread per token, the query rows in their order
+__global__ __launch_bounds__(256) void attn_paged_count_k(const AttnPagedP p) {
+  const int j = blockIdx.x * 256 + threadIdx.x, hk = blockIdx.y, b = blockIdx.z;
+  const SeqInfo s = seq_info(p, b);
+  if (j >= min(s.len, min(p.w_cols, p.s_ld))) return;
+  const int64_t slot0 = ((int64_t)b * p.c.n_kv_heads + hk) * p.s_rows;
+  const int R = min(s.nq, p.max_q) * p.G;
+  float sum = 0.f;
+  // the first row of a query that sees the token: its scores, and those of all later rows, were stored by the wave that walked the block
+  for (int r = max(0, j - (s.len - s.nq)) * p.G; r < R; ++r) {
+    const float l2 = p.l2_ws[slot0 + r];
+    if (l2 == -INFINITY) continue;
+    sum += fast_exp2(p.s_ws[(slot0 + r) * p.s_ld + j] - l2);
+  }
+  p.w_out[b * p.ldwo_seq + hk * p.ldwo_head + j] = p.w_in[b * p.ldw_seq + hk * p.ldw_head + j] + sum;
+}
+
 // ----------------------------------------------------------------------------- one wave per query row (the plain form of the kernel)
 template <int HD>
 __global__ __launch_bounds__(256) void attn_paged_row_k(const AttnPagedP p) {
@@ -46,7 +345,7 @@ __global__ __launch_bounds__(256) void attn_paged_row_k(const AttnPagedP p) {
   const int r = blockIdx.x * 4 + wave, hk = blockIdx.y, b = blockIdx.z;
   const SeqInfo s = seq_info(p, b);
   const int i = r / p.G, h = hk * p.G + r % p.G;
-  if (i >= s.nq) return;
+  if (i >= min(s.nq, p.max_q)) return;
   const int row = phys_row(p, s.p0 + i);
   if (row < 0) return;
   const int lim = min(s.len - s.nq + i, s.len - 1);
@@ -100,7 +399,7 @@ __global__ __launch_bounds__(64) void attn_paged_weights_k(const AttnPagedP p) {
   const bool ok = page_ok(page, p.c.n_pages);
   const unsigned short* k = p.c.k + (ok ? page_row(page, p.c.ld_page, hk, j & p.c.mask, p.c.shift, HD) : 0);
   float sum = 0.f;
-  for (int i = 0; i < s.nq; ++i) {
+  for (int i = 0; i < min(s.nq, p.max_q); ++i) {
     const int row = phys_row(p, s.p0 + i);
     if (row < 0) continue;
     for (int g = 0; g < p.G; ++g) {
@@ -141,6 +440,40 @@ int fill(const vm_attn_paged_args* a, AttnPagedP& p) {
   return VM_OK;
 }
 
+// ----------------------------------------------------------------------------- which form, and its workspace
+constexpr int SP_MAX_ROWS = 64;                     // query rows per kv head up to which the split form is taken
+struct Plan { bool split; int rt, tiles; int64_t part, s_ws, l2_ws, bytes; };
+
+Plan plan(AttnPagedP& p, int hd) {
+  Plan a = {};
+  const int64_t rows = (int64_t)p.max_q * p.G, heads = (int64_t)p.n_seq * p.c.n_kv_heads;
+  a.split = rows <= SP_MAX_ROWS;
+  p.n_split = 1; p.s_rows = (int)rows; p.s_ld = (p.max_kv + 31) / 32 * 32;
+  p.part = p.s_ws = p.l2_ws = nullptr;
+  if (!a.split || rows == 0 || heads == 0) return a;
+  a.rt = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
+  a.tiles = (int)((rows + 16 * a.rt - 1) / (16 * a.rt));
+  const int64_t wgs = heads * a.tiles;
+  const int64_t want = (768 + wgs - 1) / wgs, most = (p.max_kv + 64 * (SP_WAVES / a.rt) - 1) / (64 * (SP_WAVES / a.rt));
+  p.n_split = (int)(want < most ? want : most);
+  if (p.n_split < 1) p.n_split = 1;
+  int64_t at = 0;
+  if (p.n_split > 1) { a.part = at; at += heads * rows * p.n_split * (hd + 4) * 4; }
+  if (p.w_out) { a.s_ws = at; at += heads * rows * p.s_ld * 4; a.l2_ws = at; at += (heads * rows * 4 + 15) / 16 * 16; }
+  a.bytes = at;
+  return a;
+}
+
+template <int HD>
+void launch_split(const AttnPagedP& p, const Plan& a, hipStream_t st) {
+  const dim3 grid(a.tiles * p.n_split, p.c.n_kv_heads, p.n_seq);
+  if (a.rt == 1) hipLaunchKernelGGL((attn_paged_split_k<HD, 1>), grid, dim3(SP_WAVES * 64), 0, st, p);
+  else if (a.rt == 2) hipLaunchKernelGGL((attn_paged_split_k<HD, 2>), grid, dim3(SP_WAVES * 64), 0, st, p);
+  else hipLaunchKernelGGL((attn_paged_split_k<HD, 4>), grid, dim3(SP_WAVES * 64), 0, st, p);
+  if (p.n_split > 1) hipLaunchKernelGGL(attn_paged_join_k<HD>, dim3((p.s_rows + 3) / 4, p.c.n_kv_heads, p.n_seq), dim3(256), 0, st, p);
+  if (p.w_out && p.max_kv > 0) hipLaunchKernelGGL(attn_paged_count_k, dim3((p.max_kv + 255) / 256, p.c.n_kv_heads, p.n_seq), dim3(256), 0, st, p);
+}
+
 }  // namespace
 
 extern "C" {
@@ -150,7 +483,7 @@ int vm_attn_paged_workspace(const vm_attn_paged_args* args_host, int64_t* bytes_
   if (!bytes_host) return VM_ERR_BAD_ARG;
   const int rc = fill(args_host, p);
   if (rc != VM_OK) return rc;
-  *bytes_host = 0;
+  *bytes_host = plan(p, args_host->cache.head_dim).bytes;
   return VM_OK;
 }
 
@@ -159,8 +492,20 @@ int vm_attn_paged_bf16(const vm_attn_paged_args* args_host, void* stream) {
   const int rc = fill(args_host, p);
   if (rc != VM_OK) return rc;
   hipStream_t st = (hipStream_t)stream;
-  if (p.n_seq == 0) return VM_OK;
   const int hd = args_host->cache.head_dim;
+  const Plan a = plan(p, hd);
+  if (a.bytes > 0 && (!args_host->workspace || args_host->workspace_bytes < a.bytes || misaligned16(args_host->workspace))) return VM_ERR_BAD_ARG;
+  if (p.n_seq == 0) return VM_OK;
+  char* ws = (char*)args_host->workspace;
+  if (a.split && p.max_q > 0) {
+    if (p.n_split > 1) p.part = (float*)(ws + a.part);
+    if (p.w_out) { p.s_ws = (float*)(ws + a.s_ws); p.l2_ws = (float*)(ws + a.l2_ws); }
+    if (hd == 128) launch_split<128>(p, a, st);
+    else if (hd == 64) launch_split<64>(p, a, st);
+    else launch_split<32>(p, a, st);
+    VM_LAUNCH_CHECK();
+    return VM_OK;
+  }
   if (p.max_q > 0) {
     const dim3 grid((p.max_q * p.G + 3) / 4, p.c.n_kv_heads, p.n_seq);
     if (hd == 128) hipLaunchKernelGGL(attn_paged_row_k<128>, grid, dim3(256), 0, st, p);

@@ -61,3 +61,31 @@ __device__ __forceinline__ void tr_asm_wait() {
   asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
   __builtin_amdgcn_sched_barrier(0);
 }
+
+// Chunk swizzle of the 256-byte-row tiles read by the 16-wide kernels: slot = chunk ^ ((row & 7) << 1).
+// Conflict-free for BOTH access patterns (bank rule: 16-byte slot s of a row occupies banks 4s..4s+3 of the 256-B bank row):
+//  * ds_read_b128 row fragments, lane (ln, g) -> (row 16j + ln, chunk 4s + g): inside each of the instruction's four
+//    16-lane groups the slots (4s + g) ^ 2(ln & 7) are 16 distinct values (the groups pair g = 0 with 1 and 2 with 3);
+//  * ds_read_b64_tr_b16, whose 32-lane half touches rows rbase + 0..7 (or 8..15), 32 contiguous bytes each at slot pair
+//    (2b ^ 2(row & 7)): eight distinct pairs.
+// (The 32-wide image swz() is 2-way conflicted under both of these patterns: measured SQ_LDS_BANK_CONFLICT 2.3x the
+// LDS instruction cycles.)
+__device__ __forceinline__ int swz16(int row) { return (row & 7) << 1; }
+__device__ __forceinline__ int tile_off16(int row, int chunk) { return row * ROWB + ((chunk ^ swz16(row)) << 4); }
+
+// A/B operand of a 16x16x32 MFMA read along rows: lane -> row r0 + (lane & 15), k = 32 s + 8 (lane >> 4) + 0..7
+__device__ __forceinline__ bf16x8_t frag16_row(const char* tile, int r0, int s, int lane) {
+  return *reinterpret_cast<const bf16x8_t*>(tile + tile_off16(r0 + (lane & 15), 4 * s + (lane >> 4)));
+}
+// transposed operand: lane (i = lane & 15, g = lane >> 4) gets tile[rbase + 4 g + 0..3][16 b + i] and
+// tile[rbase + 16 + 4 g + 0..3][16 b + i] — the k order in which two stacked 16x16 accumulator tiles
+// (registers 0..3 of rows 4g.. and of rows 16 + 4g..) appear as the other operand.
+__device__ __forceinline__ bf16x8_t frag16_tr(const char* tile, int rbase, int b, int lane) {
+  const int i = lane & 15, g = lane >> 4;
+  const int rowA = rbase + 4 * g + (i >> 2), rowB = rowA + 16;
+  const int chunk = 2 * b + ((i & 3) >> 1);
+  const int sub = (i & 1) << 3;
+  const s16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_ptr)(tile + tile_off16(rowA, chunk) + sub));
+  const s16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_ptr)(tile + tile_off16(rowB, chunk) + sub));
+  return __builtin_bit_cast(bf16x8_t, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+}
