@@ -3,6 +3,7 @@
 //
 // Query rows of one kv head are taken together: row r of (sample b, kv head hk) is query i = r / G of head hk G + r % G (G heads share the
 // kv head), so grouped heads read K and V once. Query i sees the tokens j <= L - n + i.
+#include <mutex>
 #include "paged.hpp"
 #include "vm_tile.hpp"
 
@@ -23,6 +24,7 @@ struct AttnPagedP {
   const float* w_in; float* w_out; int64_t ldw_seq, ldw_head, ldwo_seq, ldwo_head; int w_cols;
   // split form: n_split key splits; workspace of s_rows query rows per (sample, kv head)
   int n_split, s_rows, s_ld;
+  int n_tiles, n_wg;          // tile form: row tiles per (sample, kv head), workgroups
   float* part;                // [.., s_rows, n_split, hd + 4]: max, sum, -, -, O
   float* s_ws;                // [.., s_rows, s_ld] scores (log2 domain), if the received weights are asked for
   float* l2_ws;               // [.., s_rows] log2 of the rows' sums
@@ -84,7 +86,7 @@ struct KVBlock {                                    // 32 keys of one kv head on
 
 // the two page numbers of a 32-key block (pages of 16 rows end inside it); -1 behind the last key
 struct PagePair { int a, b; };
-__device__ __forceinline__ PagePair block_pages(const AttnPagedP& p, const int32_t* table, int j0, int kv_end) {
+__device__ __forceinline__ PagePair block_pages(const AttnPagedP& p, table_ptr table, int j0, int kv_end) {
   PagePair r = {-1, -1};
   if (j0 < kv_end) r.a = table[j0 >> p.c.shift];
   if (j0 + 16 < kv_end) r.b = table[(j0 + 16) >> p.c.shift];
@@ -154,7 +156,7 @@ __global__ __launch_bounds__(SP_WAVES * 64, 2) void attn_paged_split_k(const Att
   for (int t = 0; t < ND; ++t) o[t] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
   float m = -INFINITY, l = 0.f;
   const float sc = p.scale * LOG2E;
-  const int32_t* table = p.c.table + b * p.c.ld_table;
+  const table_ptr table = table_of(p.c, b);
   char* tv = smem[wave];
   float* srow = p.s_ws ? p.s_ws + (((int64_t)b * p.c.n_kv_heads + hk) * p.s_rows + r) * p.s_ld : nullptr;
 
@@ -336,83 +338,9 @@ __global__ __launch_bounds__(256) void attn_paged_count_k(const AttnPagedP p) {
   p.w_out[b * p.ldwo_seq + hk * p.ldwo_head + j] = p.w_in[b * p.ldw_seq + hk * p.ldw_head + j] + sum;
 }
 
-// ----------------------------------------------------------------------------- one wave per query row (the plain form of the kernel)
-template <int HD>
-__global__ __launch_bounds__(256) void attn_paged_row_k(const AttnPagedP p) {
-  __shared__ float sp[4][64];
-  __shared__ float sq[4][HD];
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  const int r = blockIdx.x * 4 + wave, hk = blockIdx.y, b = blockIdx.z;
-  const SeqInfo s = seq_info(p, b);
-  const int i = r / p.G, h = hk * p.G + r % p.G;
-  if (i >= min(s.nq, p.max_q)) return;
-  const int row = phys_row(p, s.p0 + i);
-  if (row < 0) return;
-  const int lim = min(s.len - s.nq + i, s.len - 1);
-  for (int d = lane; d < HD; d += 64) sq[wave][d] = bf2f(p.q[row * p.ldq + h * HD + d]);
-  __builtin_amdgcn_wave_barrier();
-  const float sc = p.scale * LOG2E;
-  float m = -INFINITY, l = 0.f, o[(HD + 63) / 64] = {0.f};
-  for (int j0 = 0; j0 <= lim; j0 += 64) {
-    const int j = j0 + lane;
-    float sco = -INFINITY;
-    if (j <= lim) {
-      const int page = p.c.table[b * p.c.ld_table + (j >> p.c.shift)];
-      if (page_ok(page, p.c.n_pages)) {
-        const unsigned short* k = p.c.k + page_row(page, p.c.ld_page, hk, j & p.c.mask, p.c.shift, HD);
-        float a = 0.f;
-        for (int d = 0; d < HD; ++d) a = fmaf(sq[wave][d], bf2f(k[d]), a);
-        sco = a * sc;
-      }
-    }
-    const float mn = fmaxf(m, wave_max(sco)), base = mn == -INFINITY ? 0.f : mn;
-    const float corr = exp2f(m - base), e = exp2f(sco - base);
-    m = mn;
-    l = l * corr + wave_sum(e);
-    sp[wave][lane] = e;
-    __builtin_amdgcn_wave_barrier();
-    for (int t = 0; t < (HD + 63) / 64; ++t) o[t] *= corr;
-    for (int jj = 0; jj < 64 && j0 + jj <= lim; ++jj) {
-      const int page = p.c.table[b * p.c.ld_table + ((j0 + jj) >> p.c.shift)];
-      if (!page_ok(page, p.c.n_pages)) continue;
-      const unsigned short* v = p.c.v + page_row(page, p.c.ld_page, hk, (j0 + jj) & p.c.mask, p.c.shift, HD);
-      const float e2 = sp[wave][jj];
-      for (int t = 0; t < (HD + 63) / 64; ++t)
-        if (lane + 64 * t < HD) o[t] = fmaf(e2, bf2f(v[lane + 64 * t]), o[t]);
-    }
-    __builtin_amdgcn_wave_barrier();
-  }
-  for (int t = 0; t < (HD + 63) / 64; ++t)
-    if (lane + 64 * t < HD) p.out[row * p.ldo + h * HD + lane + 64 * t] = f2bf(l > 0.f || l != l ? o[t] / l : 0.f);
-  if (lane == 0) p.lse[h * p.ld_lse + s.p0 + i] = l > 0.f || l != l ? (m + log2f(l)) * LN2 : -INFINITY;
-}
-
-// one wave per 64 tokens of (sample, kv head): the lane's token against every query row
-template <int HD>
-__global__ __launch_bounds__(64) void attn_paged_weights_k(const AttnPagedP p) {
-  const int lane = threadIdx.x, j = blockIdx.x * 64 + lane, hk = blockIdx.y, b = blockIdx.z;
-  const SeqInfo s = seq_info(p, b);
-  if (blockIdx.x * 64 >= min(s.len, p.w_cols)) return;
-  const float sc = p.scale * LOG2E;
-  int page = -1;
-  if (j < s.len) page = p.c.table[b * p.c.ld_table + (j >> p.c.shift)];
-  const bool ok = page_ok(page, p.c.n_pages);
-  const unsigned short* k = p.c.k + (ok ? page_row(page, p.c.ld_page, hk, j & p.c.mask, p.c.shift, HD) : 0);
-  float sum = 0.f;
-  for (int i = 0; i < min(s.nq, p.max_q); ++i) {
-    const int row = phys_row(p, s.p0 + i);
-    if (row < 0) continue;
-    for (int g = 0; g < p.G; ++g) {
-      const int h = hk * p.G + g;
-      const float l2 = p.lse[h * p.ld_lse + s.p0 + i] * LOG2E;
-      if (!ok || j > s.len - s.nq + i) continue;
-      float a = 0.f;
-      for (int d = 0; d < HD; ++d) a = fmaf(bf2f(p.q[row * p.ldq + h * HD + d]), bf2f(k[d]), a);
-      sum += exp2f(a * sc - l2);
-    }
-  }
-  if (j < min(s.len, p.w_cols)) p.w_out[b * p.ldwo_seq + hk * p.ldwo_head + j] = p.w_in[b * p.ldw_seq + hk * p.ldw_head + j] + sum;
-}
+}  // namespace
+#include "attn_paged_tile.hpp"
+namespace {
 
 int fill(const vm_attn_paged_args* a, AttnPagedP& p) {
   if (!a) return VM_ERR_BAD_ARG;
@@ -450,7 +378,17 @@ Plan plan(AttnPagedP& p, int hd) {
   a.split = rows <= SP_MAX_ROWS;
   p.n_split = 1; p.s_rows = (int)rows; p.s_ld = (p.max_kv + 31) / 32 * 32;
   p.part = p.s_ws = p.l2_ws = nullptr;
-  if (!a.split || rows == 0 || heads == 0) return a;
+  p.n_tiles = p.n_wg = 0;
+  if (rows == 0 || heads == 0) return a;
+  if (!a.split) {
+    p.n_tiles = (int)((rows + apt::QB - 1) / apt::QB);
+    const int64_t wgs = heads * p.n_tiles, want = (256 + wgs - 1) / wgs, most = (p.max_kv + 511) / 512;
+    p.n_split = (int)(want < most ? want : most);
+    if (p.n_split < 1) p.n_split = 1;
+    if (p.n_split > 1) a.bytes = heads * rows * p.n_split * (hd + 4) * 4;
+    p.n_wg = wgs * p.n_split > 0x7FFFFF00 ? -1 : (int)(wgs * p.n_split);
+    return a;
+  }
   a.rt = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
   a.tiles = (int)((rows + 16 * a.rt - 1) / (16 * a.rt));
   const int64_t wgs = heads * a.tiles;
@@ -472,6 +410,19 @@ void launch_split(const AttnPagedP& p, const Plan& a, hipStream_t st) {
   else hipLaunchKernelGGL((attn_paged_split_k<HD, 4>), grid, dim3(SP_WAVES * 64), 0, st, p);
   if (p.n_split > 1) hipLaunchKernelGGL(attn_paged_join_k<HD>, dim3((p.s_rows + 3) / 4, p.c.n_kv_heads, p.n_seq), dim3(256), 0, st, p);
   if (p.w_out && p.max_kv > 0) hipLaunchKernelGGL(attn_paged_count_k, dim3((p.max_kv + 255) / 256, p.c.n_kv_heads, p.n_seq), dim3(256), 0, st, p);
+}
+
+template <int HD>
+int launch_tile(const AttnPagedP& p, hipStream_t st) {
+  static std::once_flag once;
+  static bool ok = false;
+  std::call_once(once, [] { ok = hipFuncSetAttribute((const void*)apt::tile_k<HD>, hipFuncAttributeMaxDynamicSharedMemorySize, apt::RING_LDS) == hipSuccess; });
+  if (!ok) return VM_ERR_LAUNCH;
+  hipLaunchKernelGGL(apt::tile_k<HD>, dim3((p.n_wg + 7) / 8 * 8), dim3(apt::NW * 64), apt::RING_LDS, st, p);
+  if (p.n_split > 1) hipLaunchKernelGGL(attn_paged_join_k<HD>, dim3((p.s_rows + 3) / 4, p.c.n_kv_heads, p.n_seq), dim3(256), 0, st, p);
+  if (p.w_out && p.max_kv > 0) hipLaunchKernelGGL(apt::weigh_k<HD>, dim3((p.max_kv + 127) / 128, p.c.n_kv_heads, p.n_seq), dim3(256), 0, st, p);
+  VM_LAUNCH_CHECK();
+  return VM_OK;
 }
 
 }  // namespace
@@ -507,17 +458,14 @@ int vm_attn_paged_bf16(const vm_attn_paged_args* args_host, void* stream) {
     return VM_OK;
   }
   if (p.max_q > 0) {
-    const dim3 grid((p.max_q * p.G + 3) / 4, p.c.n_kv_heads, p.n_seq);
-    if (hd == 128) hipLaunchKernelGGL(attn_paged_row_k<128>, grid, dim3(256), 0, st, p);
-    else if (hd == 64) hipLaunchKernelGGL(attn_paged_row_k<64>, grid, dim3(256), 0, st, p);
-    else hipLaunchKernelGGL(attn_paged_row_k<32>, grid, dim3(256), 0, st, p);
-    VM_LAUNCH_CHECK();
+    if (p.n_wg < 0) return VM_ERR_UNSUPPORTED;
+    if (p.n_split > 1) p.part = (float*)(ws + a.part);
+    if (hd == 128) return launch_tile<128>(p, st);
+    if (hd == 64) return launch_tile<64>(p, st);
+    return launch_tile<32>(p, st);
   }
-  if (p.w_out && p.max_kv > 0) {
-    const dim3 grid((p.max_kv + 63) / 64, p.c.n_kv_heads, p.n_seq);
-    if (hd == 128) hipLaunchKernelGGL(attn_paged_weights_k<128>, grid, dim3(64), 0, st, p);
-    else if (hd == 64) hipLaunchKernelGGL(attn_paged_weights_k<64>, grid, dim3(64), 0, st, p);
-    else hipLaunchKernelGGL(attn_paged_weights_k<32>, grid, dim3(64), 0, st, p);
+  if (p.w_out && p.max_kv > 0) {                     // no new token anywhere: the weights stay what they are
+    hipLaunchKernelGGL(apt::weigh_k<32>, dim3((p.max_kv + 127) / 128, p.c.n_kv_heads, p.n_seq), dim3(256), 0, st, p);
     VM_LAUNCH_CHECK();
   }
   return VM_OK;

@@ -1,0 +1,451 @@
+// attn_paged.hip, the form for many query rows: 32 query rows per wave on v_mfma_f32_32x32x16_bf16, 8 waves = 256 rows per workgroup.
+//
+// The pipeline is the one of attn32_fwd.hpp (scores transposed so that a query sits on the MFMA column and its softmax is in-lane; four
+// clusters per 64-key tile between raw barriers, the two waves of a SIMD one cluster apart; K and V by LDS-DMA into three-slot rings retired
+// by counted vmcnt). What the cache changes:
+//  * a 64-key tile may lie in up to four pages. The unit of the DMA is the 8-row group a wave stages: it never crosses a page (page size
+//    >= 16), its page number is one scalar load, fetched a tile ahead, and the buffer descriptor is made for exactly that group — base in 64
+//    bits, extent = the rows that exist — so rows behind the last token and pages that are not there arrive as zeros without a compare;
+//  * rows are (query, head of the group) pairs: grouped heads fill the tile together and read K and V once;
+//  * the causal limit of a row is any token, not its own position: the last two tiles of a wave may need the mask, and a row may see nothing
+//    (scores at -inf, a base of 0 while the maximum is -inf);
+//  * with fewer than one workgroup per CU the keys are split over workgroups too (partial results joined by attn_paged_join_k);
+//  * V^T fragments are read in two assembly statements of 16 ds_read_b64_tr_b16 that end in their own wait.
+#pragma once
+#include "attn32_tile.hpp"
+
+namespace apt {
+
+using a32::TILE;
+using a32::NW;
+using a32::NS;
+using a32::SLAB;
+using a32::SLAB_PITCH;
+using a32::RING_LDS;
+constexpr int QB = NW * 32;                     // query rows per workgroup
+
+typedef __attribute__((address_space(3))) void* lds_vptr_t;
+
+// eight transposed fragments, complete on return (offsets: 4096 per 16 rows, 512 per 32 columns)
+template <int O0, int O1, int O2, int O3, int O4, int O5, int O6, int O7>
+__device__ __forceinline__ void ld_tr8(unsigned a, unsigned b, bf16x8_t* f) {
+  s16x4_t l0, l1, l2, l3, l4, l5, l6, l7, h0, h1, h2, h3, h4, h5, h6, h7;
+  asm volatile(
+      "ds_read_b64_tr_b16 %0, %16 offset:%18\n\tds_read_b64_tr_b16 %8, %17 offset:%18\n\t"
+      "ds_read_b64_tr_b16 %1, %16 offset:%19\n\tds_read_b64_tr_b16 %9, %17 offset:%19\n\t"
+      "ds_read_b64_tr_b16 %2, %16 offset:%20\n\tds_read_b64_tr_b16 %10, %17 offset:%20\n\t"
+      "ds_read_b64_tr_b16 %3, %16 offset:%21\n\tds_read_b64_tr_b16 %11, %17 offset:%21\n\t"
+      "ds_read_b64_tr_b16 %4, %16 offset:%22\n\tds_read_b64_tr_b16 %12, %17 offset:%22\n\t"
+      "ds_read_b64_tr_b16 %5, %16 offset:%23\n\tds_read_b64_tr_b16 %13, %17 offset:%23\n\t"
+      "ds_read_b64_tr_b16 %6, %16 offset:%24\n\tds_read_b64_tr_b16 %14, %17 offset:%24\n\t"
+      "ds_read_b64_tr_b16 %7, %16 offset:%25\n\tds_read_b64_tr_b16 %15, %17 offset:%25\n\t"
+      "s_waitcnt lgkmcnt(0)"
+      : "=&v"(l0), "=&v"(l1), "=&v"(l2), "=&v"(l3), "=&v"(l4), "=&v"(l5), "=&v"(l6), "=&v"(l7), "=&v"(h0), "=&v"(h1), "=&v"(h2), "=&v"(h3), "=&v"(h4),
+        "=&v"(h5), "=&v"(h6), "=&v"(h7)
+      : "v"(a), "v"(b), "n"(O0), "n"(O1), "n"(O2), "n"(O3), "n"(O4), "n"(O5), "n"(O6), "n"(O7)
+      : "memory");
+  const s16x4_t lo[8] = {l0, l1, l2, l3, l4, l5, l6, l7}, hi[8] = {h0, h1, h2, h3, h4, h5, h6, h7};
+#pragma unroll
+  for (int i = 0; i < 8; ++i) f[i] = __builtin_bit_cast(bf16x8_t, __builtin_shufflevector(lo[i], hi[i], 0, 1, 2, 3, 4, 5, 6, 7));
+}
+template <int O0, int O1, int O2, int O3>
+__device__ __forceinline__ void ld_tr4(unsigned a, unsigned b, bf16x8_t* f) {
+  s16x4_t l0, l1, l2, l3, h0, h1, h2, h3;
+  asm volatile(
+      "ds_read_b64_tr_b16 %0, %8 offset:%10\n\tds_read_b64_tr_b16 %4, %9 offset:%10\n\t"
+      "ds_read_b64_tr_b16 %1, %8 offset:%11\n\tds_read_b64_tr_b16 %5, %9 offset:%11\n\t"
+      "ds_read_b64_tr_b16 %2, %8 offset:%12\n\tds_read_b64_tr_b16 %6, %9 offset:%12\n\t"
+      "ds_read_b64_tr_b16 %3, %8 offset:%13\n\tds_read_b64_tr_b16 %7, %9 offset:%13\n\t"
+      "s_waitcnt lgkmcnt(0)"
+      : "=&v"(l0), "=&v"(l1), "=&v"(l2), "=&v"(l3), "=&v"(h0), "=&v"(h1), "=&v"(h2), "=&v"(h3)
+      : "v"(a), "v"(b), "n"(O0), "n"(O1), "n"(O2), "n"(O3)
+      : "memory");
+  const s16x4_t lo[4] = {l0, l1, l2, l3}, hi[4] = {h0, h1, h2, h3};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) f[i] = __builtin_bit_cast(bf16x8_t, __builtin_shufflevector(lo[i], hi[i], 0, 1, 2, 3, 4, 5, 6, 7));
+}
+// the V^T fragments of a tile: f[m * ND + b] = rows 16 m .. + 15, columns 32 b .. + 31
+template <int ND>
+__device__ __forceinline__ void ld_v(unsigned a, unsigned b, bf16x8_t* f) {
+  if constexpr (ND == 4) {
+    ld_tr8<0, 512, 1024, 1536, 4096, 4608, 5120, 5632>(a, b, f);
+    ld_tr8<8192, 8704, 9216, 9728, 12288, 12800, 13312, 13824>(a, b, f + 8);
+  } else if constexpr (ND == 2) {
+    ld_tr8<0, 512, 4096, 4608, 8192, 8704, 12288, 12800>(a, b, f);
+  } else {
+    ld_tr4<0, 4096, 8192, 12288>(a, b, f);
+  }
+}
+
+// maximum of a lane's 32 scores. Assembly: fmaxf() of MFMA results costs a canonicalising instruction per operand. The statement waits out
+// the matrix pipe itself (v_mfma_f32_32x32x16: 16 passes) and its operands are read only behind the wait.
+__device__ __forceinline__ float max32(const f32x16_t (&S)[2]) {
+  float m0, m1, m2, m3;
+  asm("s_nop 15\n\ts_nop 3\n\t"
+      "v_max3_f32 %0, %4, %5, %6\n\tv_max3_f32 %1, %8, %9, %10\n\tv_max3_f32 %2, %12, %13, %14\n\tv_max3_f32 %3, %16, %17, %18\n\t"
+      "v_max_f32 %0, %0, %7\n\tv_max_f32 %1, %1, %11\n\tv_max_f32 %2, %2, %15\n\tv_max_f32 %3, %3, %19"
+      : "=&v"(m0), "=&v"(m1), "=&v"(m2), "=&v"(m3)
+      : "v"(S[0][0]), "v"(S[0][1]), "v"(S[0][2]), "v"(S[0][3]), "v"(S[0][4]), "v"(S[0][5]), "v"(S[0][6]), "v"(S[0][7]), "v"(S[0][8]), "v"(S[0][9]),
+        "v"(S[0][10]), "v"(S[0][11]), "v"(S[0][12]), "v"(S[0][13]), "v"(S[0][14]), "v"(S[0][15]));
+  asm("v_max3_f32 %0, %0, %4, %5\n\tv_max3_f32 %1, %1, %8, %9\n\tv_max3_f32 %2, %2, %12, %13\n\tv_max3_f32 %3, %3, %16, %17\n\t"
+      "v_max3_f32 %0, %0, %6, %7\n\tv_max3_f32 %1, %1, %10, %11\n\tv_max3_f32 %2, %2, %14, %15\n\tv_max3_f32 %3, %3, %18, %19\n\t"
+      "v_max3_f32 %0, %0, %1, %2\n\tv_max_f32 %0, %0, %3"
+      : "+v"(m0), "+v"(m1), "+v"(m2), "+v"(m3)
+      : "v"(S[1][0]), "v"(S[1][1]), "v"(S[1][2]), "v"(S[1][3]), "v"(S[1][4]), "v"(S[1][5]), "v"(S[1][6]), "v"(S[1][7]), "v"(S[1][8]), "v"(S[1][9]),
+        "v"(S[1][10]), "v"(S[1][11]), "v"(S[1][12]), "v"(S[1][13]), "v"(S[1][14]), "v"(S[1][15]));
+  return m0;
+}
+
+// end of a cluster (attn32_tile.hpp) with any count
+template <int VM>
+__device__ __forceinline__ void cluster_end() {
+  if constexpr (VM >= 0) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(VM) : "memory");
+  else asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  __builtin_amdgcn_sched_barrier(0);
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_sched_barrier(0);
+}
+
+__device__ __forceinline__ int acc_row(int r, int h) { return (r & 3) + 8 * (r >> 2) + 4 * h; }
+
+// what a wave needs to stage its 8-row group of a tile
+template <int HD>
+struct Stager {
+  static constexpr int PW = HD > 64 ? 2 : 1;     // DMA instructions per group: 64 columns each
+  int voff[PW];                                  // byte offset inside the group, or out of every descriptor's reach
+  int64_t head;                                  // element offset of (kv head, row 0) inside a page
+  __device__ __forceinline__ void init(int hk, int shift, int wave, int lane) {
+    const int row = 8 * wave + ((lane >> 2) & 7);
+    head = ((int64_t)hk << shift) * HD;
+#pragma unroll
+    for (int i = 0; i < PW; ++i) {
+      const int chunk = 4 * (2 * i + (lane >> 5)) + ((lane & 3) ^ ((row >> 2) & 3));      // the image's XOR goes onto the source chunk
+      voff[i] = chunk * 8 < HD ? ((lane >> 2) & 7) * HD * 2 + chunk * 16 : 0x7FFFFFF0;
+    }
+  }
+  __device__ __forceinline__ void stage(const unsigned short* pool, const PagedKV& c, int page, int t, int kv_end, char* tile, int wave) const {
+    const int tok = 64 * t + 8 * wave;
+    const int rows = page < 0 ? 0 : max(0, min(8, kv_end - tok));
+    const uint64_t at = (uint64_t)(pool + (page < 0 ? 0 : (int64_t)page * c.ld_page) + head + (int64_t)(tok & c.mask) * HD);
+    const unsigned lo = __builtin_amdgcn_readfirstlane((unsigned)at), hi = __builtin_amdgcn_readfirstlane((unsigned)(at >> 32));
+    const __amdgpu_buffer_rsrc_t rs =
+        __builtin_amdgcn_make_buffer_rsrc((void*)(((uint64_t)hi << 32) | lo), 0, __builtin_amdgcn_readfirstlane(rows * HD * 2), 0x00020000);
+#pragma unroll
+    for (int i = 0; i < PW; ++i)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_vptr_t)(tile + (2 * wave + i) * 1024), 16, voff[i], 0, 0, 0);
+  }
+};
+
+template <int HD>
+__global__ __launch_bounds__(NW * 64, 2) void tile_k(const AttnPagedP p) {
+  typedef Stager<HD> St;
+  constexpr int KS = HD / 16;                 // k-steps of the score product
+  constexpr int ND = HD / 32;                 // 32-row d-tiles of O^T
+  constexpr int PW = St::PW;
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int hf = lane >> 5;
+  // ---- which tile. Workgroups id and id + 8 share an XCD (one L2 each): every XCD takes a contiguous piece of the list (kv head, sample,
+  // row tile, split) so that the tiles of one cache meet in one L2; the longest row tiles come first. Few caches: spread them instead.
+  int lin;
+  {
+    const int id = blockIdx.x, xcd = id & 7, slot = id >> 3, per = (p.n_wg + 7) >> 3;
+    lin = p.n_seq * p.c.n_kv_heads >= 16 ? xcd * per + slot : id;
+    if (slot >= per || lin >= p.n_wg) return;
+  }
+  const int split = lin % p.n_split, rest = lin / p.n_split;
+  const int tile = p.n_tiles - 1 - rest % p.n_tiles, hs = rest / p.n_tiles;
+  const int b = hs % p.n_seq, hk = hs / p.n_seq;
+  const SeqInfo s = seq_info(p, b);
+  const int R = min(s.nq, p.max_q) * p.G, row0 = tile * QB;
+  if (row0 >= R) return;
+  const int past = s.len - s.nq;
+  const int qw = row0 + wave * 32;                                 // this wave's first row
+  const bool wave_live = qw < R;
+  const int r = qw + (lane & 31);
+  const bool live = r < R;
+  const int qi = live ? r / p.G : 0, h = hk * p.G + (live ? r - qi * p.G : 0);
+  const int prow = live ? phys_row(p, s.p0 + qi) : -1;
+  const int lim = live ? past + qi : -1;                           // last token the row sees (may be negative: none)
+  const int lim_lo = past + min(qw, R - 1) / p.G, lim_hi = past + min(qw + 31, R - 1) / p.G;
+  const int kv_end = max(0, past + (min(row0 + QB, R) - 1) / p.G + 1);
+  const int nt_all = (kv_end + 63) / 64, per = (nt_all + p.n_split - 1) / p.n_split;
+  const int t0 = min(split * per, nt_all), t1 = min(t0 + per, nt_all), nt = t1 - t0;
+  const int t_w = wave_live && lim_hi >= 0 ? min(t1, lim_hi / 64 + 1) : t0;      // tiles [t0, t_w) are this wave's
+  const bool late = wave >= NW / 2;
+
+  bf16x8_t qf[KS];
+#pragma unroll
+  for (int k = 0; k < KS; ++k) {
+    i32x4_t v = {0, 0, 0, 0};
+    if (prow >= 0) v = *reinterpret_cast<const i32x4_t*>(p.q + prow * p.ldq + h * HD + 16 * k + 8 * hf);
+    qf[k] = __builtin_bit_cast(bf16x8_t, v);
+  }
+  f32x16_t o[ND];
+#pragma unroll
+  for (int b2 = 0; b2 < ND; ++b2)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) o[b2][e] = 0.f;
+  const float sc = p.scale * LOG2E;
+  float msc = -INFINITY, base = 0.f, l_run = 0.f;                  // running maximum (log2 domain), what is subtracted, this half's sum
+
+  if (nt > 0) {
+    const table_ptr table = table_of(p.c, b);
+    // pages that are not there: looked for once, the tile loop asks the table again only if there are any
+    int gone = 0;
+    for (int i = (64 * t0 >> p.c.shift) + tid; i <= (min(64 * t1, kv_end) - 1) >> p.c.shift; i += NW * 64) gone |= !page_ok(table[i], p.c.n_pages);
+    const bool any_gone = __syncthreads_or(gone) != 0;
+    auto page_of = [&](int t) -> int {                             // page of this wave's group of tile t; -1: none
+      const int tok = 64 * t + 8 * wave;
+      if (t >= t1 || tok >= kv_end) return -1;
+      const int pg = table[__builtin_amdgcn_readfirstlane(tok >> p.c.shift)];
+      return page_ok(pg, p.c.n_pages) ? pg : -1;
+    };
+    char* const kring = smem;
+    char* const vring = smem + NS * TILE;
+    St st;
+    st.init(hk, p.c.shift, wave, lane);
+    // DMA order per wave (PW instructions a group): K(0) V(0) V(1) K(1); c0(u) issues V(u+2), c1(u) issues K(u+2). At the end of c0(u) V(u)
+    // must have landed (V(u+1) K(u+1) V(u+2) may fly: vmcnt(3 PW)), at the end of c2(u) K(u+1) (V(u+2) K(u+2): vmcnt(2 PW)).
+    int pga = page_of(t0), pgb = page_of(t0 + 1), pgc = page_of(t0 + 2);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");               // nothing older in the queue
+    st.stage(p.c.k, p.c, pga, t0, kv_end, kring, wave);
+    st.stage(p.c.v, p.c, pga, t0, kv_end, vring, wave);
+    if (nt > 1) {
+      st.stage(p.c.v, p.c, pgb, t0 + 1, kv_end, vring + TILE, wave);
+      st.stage(p.c.k, p.c, pgb, t0 + 1, kv_end, kring + TILE, wave);
+      cluster_end<3 * PW>();
+    } else {
+      cluster_end<0>();
+    }
+    if (late) cluster_end<-1>();
+    const char* const kb0 = kring + a32::row_base(lane, 0);
+    const char* const kb1 = kring + a32::row_base(lane, 1);
+    const unsigned vbA = (unsigned)(size_t)(vring + a32::tr_base(lane, 0)), vbB = (unsigned)(size_t)(vring + a32::tr_base(lane, 1));
+    f32x16_t S[2];
+    bf16x8_t kv[(4 * ND > 2 * KS) ? 4 * ND : 2 * KS];              // the K fragments of a tile, then its V fragments
+    int s0 = 0, s1 = TILE, s2 = 2 * TILE;
+    for (int u = 0; u < nt; ++u) {
+      const int t = t0 + u;
+      const bool on = t < t_w;
+      const bool more1 = u + 1 < nt, more2 = u + 2 < nt;
+      const int pgd = page_of(t + 3);
+      // ---- c0: K fragments -> registers; DMA of V(u+2)
+      if (on) {
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+          for (int ks = 0; ks < KS; ++ks) kv[kt * KS + ks] = a32::ld_row(((ks & 1) ? kb1 : kb0) + s0, 8192 * kt + 512 * (ks >> 1));
+      }
+      if (more2) st.stage(p.c.v, p.c, pgc, t + 2, kv_end, vring + s2, wave);
+      if (more2) cluster_end<3 * PW>(); else if (more1) cluster_end<2 * PW>(); else cluster_end<0>();
+      // ---- c1: S^T = K Q^T; DMA of K(u+2)
+      if (on) {
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt) {
+          f32x16_t acc = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int ks = 0; ks < KS; ++ks) acc = a32::mfma32(kv[kt * KS + ks], qf[ks], acc);
+          S[kt] = acc;
+        }
+      }
+      if (more2) st.stage(p.c.k, p.c, pgc, t + 2, kv_end, kring + s2, wave);
+      cluster_end<-1>();
+      // ---- c2: V fragments -> registers, mask, maximum, rescale
+      if (on) {
+        ld_v<ND>(vbA + s0, vbB + s0, kv);
+        const int kv0 = 64 * t;
+        if (kv0 + 63 > lim_lo || any_gone) {
+#pragma unroll
+          for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+            for (int e2 = 0; e2 < 2; ++e2) {                       // 16 keys of one page
+              const int k0 = kv0 + 32 * kt + 16 * e2;
+              const bool ok = !any_gone || (k0 < kv_end && page_ok(table[__builtin_amdgcn_readfirstlane(min(k0, kv_end - 1) >> p.c.shift)], p.c.n_pages));
+#pragma unroll
+              for (int e = 8 * e2; e < 8 * e2 + 8; ++e) S[kt][e] = ok && kv0 + 32 * kt + acc_row(e, hf) <= lim ? S[kt][e] : -INFINITY;
+            }
+        }
+        float ma = max32(S), mb = ma;
+        a32::swap_halves(ma, mb);
+        const float mxs = fmaxf(ma, mb) * sc;
+        if (__builtin_amdgcn_ballot_w64(mxs > msc) != 0) {
+          const float mn = fmaxf(msc, mxs);
+          base = mn == -INFINITY ? 0.f : mn;
+          const float alpha = fast_exp2(msc - base);               // 0 while nothing was seen
+          msc = mn;
+          l_run *= alpha;
+#pragma unroll
+          for (int b2 = 0; b2 < ND; ++b2)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) o[b2][e] *= alpha;
+        }
+      }
+      if (more2) cluster_end<2 * PW>(); else cluster_end<0>();
+      // ---- c3: O^T += V^T P^T, the next 16 keys' exponentials beside it
+      if (on) {
+        float rs0 = 0.f, rs1 = 0.f;
+#pragma unroll
+        for (int m = 0; m < 4; ++m) {
+          u16x8_t w;
+#pragma unroll
+          for (int j = 0; j < 8; j += 2) {
+            const int e = 8 * (m & 1) + j;
+            const float e0 = fast_exp2(fmaf(S[m >> 1][e], sc, -base)), e1 = fast_exp2(fmaf(S[m >> 1][e + 1], sc, -base));
+            w[j] = f2bf(e0);
+            w[j + 1] = f2bf(e1);
+            rs0 += e0;
+            rs1 += e1;
+          }
+          const bf16x8_t pf = __builtin_bit_cast(bf16x8_t, w);
+#pragma unroll
+          for (int b2 = 0; b2 < ND; ++b2) o[b2] = a32::mfma32(kv[m * ND + b2], pf, o[b2]);
+        }
+        l_run += rs0 + rs1;
+      }
+      cluster_end<-1>();
+      { const int x = s0; s0 = s1; s1 = s2; s2 = x; }
+      pgc = pgd;
+    }
+    if (!late) cluster_end<-1>();                // every LDS read is over: the slabs may overlay the rings
+  }
+
+  if (!wave_live) return;
+  {
+    float a = l_run, c = l_run;
+    a32::swap_halves(a, c);
+    l_run = a + c;
+  }
+  if (p.n_split > 1) {
+    if (!live) return;
+    float* part = p.part + ((((int64_t)b * p.c.n_kv_heads + hk) * p.s_rows + r) * p.n_split + split) * (HD + 4);
+    if (hf == 0) { part[0] = msc; part[1] = l_run; }
+#pragma unroll
+    for (int b2 = 0; b2 < ND; ++b2)
+#pragma unroll
+      for (int g4 = 0; g4 < 4; ++g4)
+        *reinterpret_cast<f32x4_t*>(part + 4 + 32 * b2 + 8 * g4 + 4 * hf) = (f32x4_t){o[b2][4 * g4], o[b2][4 * g4 + 1], o[b2][4 * g4 + 2], o[b2][4 * g4 + 3]};
+    return;
+  }
+  const bool some = !(l_run == 0.f);
+  const float inv = some ? 1.f / l_run : 0.f;
+  if (live && hf == 0) p.lse[h * p.ld_lse + s.p0 + qi] = some ? (msc + log2f(l_run)) * LN2 : -INFINITY;
+  // O^T registers -> this wave's slab [32 rows][HD], then whole rows out
+  char* slab = smem + wave * SLAB;
+#pragma unroll
+  for (int b2 = 0; b2 < ND; ++b2)
+#pragma unroll
+    for (int g4 = 0; g4 < 4; ++g4) {
+      const u16x4_t w = {f2bf(o[b2][4 * g4] * inv), f2bf(o[b2][4 * g4 + 1] * inv), f2bf(o[b2][4 * g4 + 2] * inv), f2bf(o[b2][4 * g4 + 3] * inv)};
+      *reinterpret_cast<u16x4_t*>(slab + (lane & 31) * SLAB_PITCH + (32 * b2 + 8 * g4 + 4 * hf) * 2) = w;
+    }
+  __builtin_amdgcn_wave_barrier();
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  constexpr int CPR = HD / 8;                    // 16-byte chunks per row
+#pragma unroll
+  for (int i = lane; i < 32 * CPR; i += 64) {
+    const int rr = i / CPR, ch = i - rr * CPR;
+    if (qw + rr < R) {
+      const int i2 = (qw + rr) / p.G, h2 = hk * p.G + (qw + rr) - i2 * p.G;
+      const int64_t row = phys_row(p, s.p0 + i2);
+      if (row >= 0) *reinterpret_cast<i32x4_t*>(p.out + row * p.ldo + h2 * HD + ch * 8) = *reinterpret_cast<const i32x4_t*>(slab + rr * SLAB_PITCH + ch * 16);
+    }
+  }
+}
+
+// ----------------------------------------------------------------------------- received weights of a chunk
+// w[j] += sum over the query rows of exp2(s q_r . k_j - l2_r): the scores once more (2 hd of the 4 hd operations of the attention itself;
+// keeping them would be 4 bytes per row and token), key-stationary. A wave holds 32 tokens as A operands (HD / 16 fragments, straight from
+// the page) and walks the rows that see them, 32 at a time as B operands; the tokens' sums stay in its registers, each row tile adds in its
+// turn, and the 32 columns are added up in a fixed tree at the end. Bound by the exponentials (16 per lane and 32 x 32 tile: 256 cycles
+// beside 256 of the matrix pipe).
+template <int HD>
+__global__ __launch_bounds__(256, 2) void weigh_k(const AttnPagedP p) {
+  constexpr int KS = HD / 16;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), hf = lane >> 5;
+  const int hk = blockIdx.y, b = blockIdx.z;
+  const SeqInfo s = seq_info(p, b);
+  const int n = min(s.len, p.w_cols), j0 = (blockIdx.x * 4 + wave) * 32;
+  if (j0 >= n) return;
+  const int R = min(s.nq, p.max_q) * p.G, past = s.len - s.nq;
+  const table_ptr table = table_of(p.c, b);
+  bf16x8_t kf[KS];
+  {
+    const int j = j0 + (lane & 31);
+    int page = -1;
+    if (j < n) page = table[j >> p.c.shift];
+#pragma unroll
+    for (int k = 0; k < KS; ++k) {
+      i32x4_t v = {0, 0, 0, 0};
+      if (j < n && page_ok(page, p.c.n_pages))
+        v = *reinterpret_cast<const i32x4_t*>(p.c.k + page_row(page, p.c.ld_page, hk, j & p.c.mask, p.c.shift, HD) + 16 * k + 8 * hf);
+      kf[k] = __builtin_bit_cast(bf16x8_t, v);
+    }
+  }
+  const float sc = p.scale * LOG2E;
+  float sum[16];
+#pragma unroll
+  for (int e = 0; e < 16; ++e) sum[e] = 0.f;
+  struct Row { int prow, h, lim; float l2; };
+  auto row_of = [&](int r) -> Row {
+    Row x = {-1, 0, -1, 0.f};
+    if (r < R) {
+      const int i = r / p.G;
+      x.h = hk * p.G + r - i * p.G;
+      x.prow = phys_row(p, s.p0 + i);
+      x.lim = past + i;
+      x.l2 = p.lse[x.h * p.ld_lse + s.p0 + i] * LOG2E;
+      if (x.prow < 0 || x.l2 == -INFINITY) x.lim = -1;
+    }
+    return x;
+  };
+  auto load_q = [&](const Row& x, bf16x8_t* q) {
+#pragma unroll
+    for (int k = 0; k < KS; ++k) {
+      i32x4_t v = {0, 0, 0, 0};
+      if (x.prow >= 0) v = *reinterpret_cast<const i32x4_t*>(p.q + x.prow * p.ldq + x.h * HD + 16 * k + 8 * hf);
+      q[k] = __builtin_bit_cast(bf16x8_t, v);
+    }
+  };
+  const int r0 = max(0, j0 - past) * p.G / 32 * 32;                // the first row that sees one of these tokens
+  Row cur = row_of(r0 + (lane & 31)), nxt = row_of(r0 + 32 + (lane & 31));
+  bf16x8_t q[KS], qn[KS];
+  load_q(cur, q);
+  for (int r = r0; r < R; r += 32) {
+    load_q(nxt, qn);
+    const Row nn = row_of(r + 64 + (lane & 31));
+    f32x16_t acc = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int k = 0; k < KS; ++k) acc = a32::mfma32(kf[k], q[k], acc);
+    const int seen = cur.lim - j0;                                 // tokens 0 .. seen of the 32 are seen by this lane's row
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      const float w = fast_exp2(fmaf(acc[e], sc, -cur.l2));
+      sum[e] += acc_row(e, hf) <= seen ? w : 0.f;
+    }
+    cur = nxt;
+    nxt = nn;
+#pragma unroll
+    for (int k = 0; k < KS; ++k) q[k] = qn[k];
+  }
+  // the 32 rows of the columns
+#pragma unroll
+  for (int e = 0; e < 16; ++e) {
+    float x = sum[e];
+#pragma unroll
+    for (int o2 = 1; o2 < 32; o2 <<= 1) x += __shfl_xor(x, o2, 64);
+    sum[e] = x;
+  }
+#pragma unroll
+  for (int e = 0; e < 16; ++e) {
+    const int j = j0 + acc_row(e, hf);
+    if ((lane & 31) == e && j < n) {
+      const bool there = page_ok(p.c.table[b * p.c.ld_table + (j >> p.c.shift)], p.c.n_pages);
+      p.w_out[b * p.ldwo_seq + hk * p.ldwo_head + j] = p.w_in[b * p.ldw_seq + hk * p.ldw_head + j] + (there ? sum[e] : 0.f);
+    }
+  }
+}
+
+}  // namespace apt

@@ -25,6 +25,10 @@ __device__ __forceinline__ int64_t page_row(int page, int64_t ld_page, int hk, i
   return (int64_t)page * ld_page + (((int64_t)hk << shift) + row) * head_dim;
 }
 
+// the page numbers of a sample, through the scalar cache (the table does not change while a kernel runs)
+typedef const __attribute__((address_space(4))) int32_t* table_ptr;
+__device__ __forceinline__ table_ptr table_of(const PagedKV& c, int seq) { return (table_ptr)(uintptr_t)(c.table + (int64_t)seq * c.ld_table); }
+
 inline int paged_shift(int page_size) {          // log2 of a legal page size, -1 otherwise
   for (int s = 4; s <= 10; ++s)
     if (page_size == 1 << s) return s;

@@ -136,6 +136,10 @@ def test_attention_of_nothing(dev, K):
     q = torch.zeros(0, 2 * 64, dtype=torch.bfloat16, device=dev)
     o, lse = K.attn_paged(q, k, v, table, i32([0, 0], dev), i32([40], dev), 0.1, 0, 40)
     assert o.shape == (0, 128) and lse.shape == (2, 0)
+    w = torch.rand(1, 2, 48, generator=g).to(dev)
+    wo = torch.full_like(w, -1.0)
+    K.attn_paged(q, k, v, table, i32([0, 0], dev), i32([40], dev), 0.1, 0, 40, weights=w, weights_out=wo)
+    assert torch.equal(wo[..., :40], w[..., :40]) and (wo[..., 40:] == -1.0).all()
 
 
 @pytest.mark.parametrize('hd', [32, 64, 128])
