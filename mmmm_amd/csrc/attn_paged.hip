@@ -54,9 +54,11 @@ __device__ __forceinline__ int phys_row(const AttnPagedP& p, int pos) {      // 
 //   stacked score tiles ARE the B operand. P is taken as two bf16 terms (its rounding and what that left out: 16 significant bits), the
 //   second product costs matrix time that the loads leave idle, and the only rounding the result sees is its own.
 // The next block's K and V are in flight while one is computed; page numbers are fetched two blocks ahead through the scalar cache.
-// A workgroup has four waves: RT row tiles x 4 / RT key streams; its key streams are merged in LDS, and if the keys were split over
-// workgroups too the partial (max, sum, O) of each goes to the workspace and attn_paged_join_k joins them in a fixed order.
-constexpr int SP_WAVES = 4;
+// A workgroup has eight waves, each a key stream of its own (one workgroup per CU: 8 x 16 KiB in flight); they meet in LDS, and if the keys
+// were split over workgroups too the partial (max, sum, O) of each goes to the workspace and attn_paged_join_k joins them in a fixed order.
+// Measured beside four waves a workgroup and two of them per CU: 32 x 16384 grouped 281 us (5.8 TB/s) / 285 us, 8 x 4609 92 / 91 us.
+constexpr int SP_WAVES = 8;
+constexpr int SP_ROWS = 16;                        // query rows (queries x heads of the group) of the form
 
 __device__ __forceinline__ void swap16(float& a, float& b) { asm("s_nop 1\n\tv_permlane16_swap_b32 %0, %1" : "+v"(a), "+v"(b)); }
 __device__ __forceinline__ void swap32(float& a, float& b) { asm("s_nop 1\n\tv_permlane32_swap_b32 %0, %1" : "+v"(a), "+v"(b)); }
@@ -117,10 +119,10 @@ __device__ __forceinline__ void load_block(const AttnPagedP& p, KVBlock<HD>& x, 
   }
 }
 
-template <int HD, int RT>
+template <int HD>
 __global__ __launch_bounds__(SP_WAVES * 64, 2) void attn_paged_split_k(const AttnPagedP p) {
   typedef KVBlock<HD> B;
-  constexpr int KW = SP_WAVES / RT;                  // key streams of the workgroup
+  constexpr int KW = SP_WAVES;
   constexpr int ND = HD / 16;
   __shared__ __attribute__((aligned(1024))) char smem[SP_WAVES][32 * ROWB];
   __shared__ float red[SP_WAVES][2][16];
@@ -128,21 +130,20 @@ __global__ __launch_bounds__(SP_WAVES * 64, 2) void attn_paged_split_k(const Att
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int ln = lane & 15, g = lane >> 4;
   const int hk = blockIdx.y, b = blockIdx.z;
-  const int rt = wave % RT, kw = wave / RT;
-  const int tile = blockIdx.x / p.n_split, split = blockIdx.x % p.n_split;
+  const int split = blockIdx.x;
   const SeqInfo s = seq_info(p, b);
-  const int R = min(s.nq, p.max_q) * p.G, row0 = (tile * RT + rt) * 16, wg_row0 = tile * RT * 16;
-  if (wg_row0 >= R) return;
-  const int r = row0 + ln;
+  const int R = min(min(s.nq, p.max_q) * p.G, SP_ROWS);
+  if (R <= 0) return;
+  const int r = ln;
   const bool live = r < R;
   const int i = live ? r / p.G : 0, h = hk * p.G + (live ? r - i * p.G : 0);
   const int prow = live ? phys_row(p, s.p0 + i) : -1;
   const int lim = live ? s.len - s.nq + i : -1;      // last token this row sees
-  const int lim_min = s.len - s.nq + min(row0, R - 1) / p.G;
-  const int kv_end = max(0, s.len - s.nq + (min(wg_row0 + RT * 16, R) - 1) / p.G + 1);
+  const int lim_min = s.len - s.nq;
+  const int kv_end = max(0, s.len - s.nq + (R - 1) / p.G + 1);
   // this workgroup's blocks
   const int nblk = (kv_end + 31) / 32, per = (nblk + p.n_split - 1) / p.n_split;
-  const int blk0 = min(split * per, nblk), blk1 = row0 < R ? min(blk0 + per, nblk) : blk0;
+  const int blk0 = min(split * per, nblk), blk1 = min(blk0 + per, nblk);
 
   bf16x8_t qf[B::KS];
 #pragma unroll
@@ -161,7 +162,7 @@ __global__ __launch_bounds__(SP_WAVES * 64, 2) void attn_paged_split_k(const Att
   float* srow = p.s_ws ? p.s_ws + (((int64_t)b * p.c.n_kv_heads + hk) * p.s_rows + r) * p.s_ld : nullptr;
 
   KVBlock<HD> cur, nxt;
-  int blk = blk0 + kw;
+  int blk = blk0 + wave;
   PagePair pg = block_pages(p, table, blk * 32, kv_end);
   if (blk < blk1) load_block<HD>(p, cur, pg, hk, blk * 32, kv_end, lane);
   PagePair pg1 = block_pages(p, table, (blk + KW) * 32, kv_end);
@@ -228,57 +229,49 @@ __global__ __launch_bounds__(SP_WAVES * 64, 2) void attn_paged_split_k(const Att
     pg1 = pg2;
   }
   l = sum_over_g(l);
-  // ---- the key streams of a row tile meet in LDS: wave 0 of them adds up in order
-  if (KW > 1) {
-    if (g == 0) { red[wave][0][ln] = m; red[wave][1][ln] = l; }
-    __syncthreads();
+  // ---- the key streams meet in LDS: each wave adds up its share of O^T, in the order of the streams
+  if (g == 0) { red[wave][0][ln] = m; red[wave][1][ln] = l; }
+  __syncthreads();
+  {
     float mm = m;
 #pragma unroll
-    for (int k = 0; k < KW; ++k) mm = fmaxf(mm, red[k * RT + rt][0][ln]);
+    for (int k = 0; k < KW; ++k) mm = fmaxf(mm, red[k][0][ln]);
     const float base = mm == -INFINITY ? 0.f : mm, f = fast_exp2(m - base);
-    float ll = 0.f;
+    l = 0.f;
 #pragma unroll
-    for (int k = 0; k < KW; ++k) ll += red[k * RT + rt][1][ln] * fast_exp2(red[k * RT + rt][0][ln] - base);
+    for (int k = 0; k < KW; ++k) l += red[k][1][ln] * fast_exp2(red[k][0][ln] - base);
     m = mm;
-    l = ll;
     float* slab = reinterpret_cast<float*>(smem[wave]);          // O^T of this wave, [d][row]
 #pragma unroll
     for (int t = 0; t < ND; ++t)
 #pragma unroll
       for (int e = 0; e < 4; ++e) slab[(16 * t + 4 * g + e) * 16 + ln] = o[t][e] * f;
-    __syncthreads();
-    if (kw != 0) return;
-#pragma unroll
-    for (int t = 0; t < ND; ++t)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        float x = 0.f;
-#pragma unroll
-        for (int k = 0; k < KW; ++k) x += reinterpret_cast<const float*>(smem[k * RT + rt])[(16 * t + 4 * g + e) * 16 + ln];
-        o[t][e] = x;
-      }
   }
-  if (!live) return;
+  __syncthreads();
+  if (!live || wave >= ND) return;
+  f32x4_t x = {0.f, 0.f, 0.f, 0.f};                // the wave's 16 columns
+#pragma unroll
+  for (int k = 0; k < KW; ++k)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[e] += reinterpret_cast<const float*>(smem[k])[(16 * wave + 4 * g + e) * 16 + ln];
+  const bool writes_row = wave == 0 && g == 0;
+  const int64_t slot = ((int64_t)b * p.c.n_kv_heads + hk) * p.s_rows + r;
   if (p.n_split == 1) {
     const bool some = !(l == 0.f);
     const float inv = some ? 1.f / l : 0.f;
     if (prow >= 0) {
-#pragma unroll
-      for (int t = 0; t < ND; ++t) {
-        const u16x4_t w = {f2bf(o[t][0] * inv), f2bf(o[t][1] * inv), f2bf(o[t][2] * inv), f2bf(o[t][3] * inv)};
-        *reinterpret_cast<u16x4_t*>(p.out + prow * p.ldo + h * HD + 16 * t + 4 * g) = some ? w : (u16x4_t){0, 0, 0, 0};
-      }
+      const u16x4_t w = {f2bf(x[0] * inv), f2bf(x[1] * inv), f2bf(x[2] * inv), f2bf(x[3] * inv)};
+      *reinterpret_cast<u16x4_t*>(p.out + prow * p.ldo + h * HD + 16 * wave + 4 * g) = some ? w : (u16x4_t){0, 0, 0, 0};
     }
-    const float l2 = some ? m + log2f(l) : -INFINITY;
-    if (g == 0) {
+    if (writes_row) {
+      const float l2 = some ? m + log2f(l) : -INFINITY;
       p.lse[h * p.ld_lse + s.p0 + i] = l2 * LN2;
-      if (p.s_ws) p.l2_ws[((int64_t)b * p.c.n_kv_heads + hk) * p.s_rows + r] = l2;
+      if (p.s_ws) p.l2_ws[slot] = l2;
     }
   } else {
-    float* part = p.part + ((((int64_t)b * p.c.n_kv_heads + hk) * p.s_rows + r) * p.n_split + split) * (HD + 4);
-    if (g == 0) { part[0] = m; part[1] = l; }
-#pragma unroll
-    for (int t = 0; t < ND; ++t) *reinterpret_cast<f32x4_t*>(part + 4 + 16 * t + 4 * g) = o[t];
+    float* part = p.part + (slot * p.n_split + split) * (HD + 4);
+    if (writes_row) { part[0] = m; part[1] = l; }
+    *reinterpret_cast<f32x4_t*>(part + 4 + 16 * wave + 4 * g) = x;
   }
 }
 
@@ -369,13 +362,14 @@ int fill(const vm_attn_paged_args* a, AttnPagedP& p) {
 }
 
 // ----------------------------------------------------------------------------- which form, and its workspace
-constexpr int SP_MAX_ROWS = 64;                     // query rows per kv head up to which the split form is taken
-struct Plan { bool split; int rt, tiles; int64_t part, s_ws, l2_ws, bytes; };
+struct Plan { bool split; int64_t part, s_ws, l2_ws, bytes; };
 
 Plan plan(AttnPagedP& p, int hd) {
   Plan a = {};
   const int64_t rows = (int64_t)p.max_q * p.G, heads = (int64_t)p.n_seq * p.c.n_kv_heads;
-  a.split = rows <= SP_MAX_ROWS;
+  // 16 rows are what the split form's matrix tile holds. Beyond it the tile form wins although most of its 256 rows are empty: 4 x 17 queries
+  // over 2086 tokens 34 us beside 37 us (two row tiles a workgroup), 17 x 4 heads over 8704 28 beside 45, 64 queries 38 beside 53.
+  a.split = rows <= SP_ROWS;
   p.n_split = 1; p.s_rows = (int)rows; p.s_ld = (p.max_kv + 31) / 32 * 32;
   p.part = p.s_ws = p.l2_ws = nullptr;
   p.n_tiles = p.n_wg = 0;
@@ -389,10 +383,8 @@ Plan plan(AttnPagedP& p, int hd) {
     p.n_wg = wgs * p.n_split > 0x7FFFFF00 ? -1 : (int)(wgs * p.n_split);
     return a;
   }
-  a.rt = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
-  a.tiles = (int)((rows + 16 * a.rt - 1) / (16 * a.rt));
-  const int64_t wgs = heads * a.tiles;
-  const int64_t want = (768 + wgs - 1) / wgs, most = (p.max_kv + 64 * (SP_WAVES / a.rt) - 1) / (64 * (SP_WAVES / a.rt));
+  // one workgroup per CU, two rounds (ragged lengths): 512, and 64 keys for a wave at least
+  const int64_t want = (512 + heads - 1) / heads, most = (p.max_kv + 64 * SP_WAVES - 1) / (64 * SP_WAVES);
   p.n_split = (int)(want < most ? want : most);
   if (p.n_split < 1) p.n_split = 1;
   int64_t at = 0;
@@ -403,11 +395,8 @@ Plan plan(AttnPagedP& p, int hd) {
 }
 
 template <int HD>
-void launch_split(const AttnPagedP& p, const Plan& a, hipStream_t st) {
-  const dim3 grid(a.tiles * p.n_split, p.c.n_kv_heads, p.n_seq);
-  if (a.rt == 1) hipLaunchKernelGGL((attn_paged_split_k<HD, 1>), grid, dim3(SP_WAVES * 64), 0, st, p);
-  else if (a.rt == 2) hipLaunchKernelGGL((attn_paged_split_k<HD, 2>), grid, dim3(SP_WAVES * 64), 0, st, p);
-  else hipLaunchKernelGGL((attn_paged_split_k<HD, 4>), grid, dim3(SP_WAVES * 64), 0, st, p);
+void launch_split(const AttnPagedP& p, hipStream_t st) {
+  hipLaunchKernelGGL(attn_paged_split_k<HD>, dim3(p.n_split, p.c.n_kv_heads, p.n_seq), dim3(SP_WAVES * 64), 0, st, p);
   if (p.n_split > 1) hipLaunchKernelGGL(attn_paged_join_k<HD>, dim3((p.s_rows + 3) / 4, p.c.n_kv_heads, p.n_seq), dim3(256), 0, st, p);
   if (p.w_out && p.max_kv > 0) hipLaunchKernelGGL(attn_paged_count_k, dim3((p.max_kv + 255) / 256, p.c.n_kv_heads, p.n_seq), dim3(256), 0, st, p);
 }
@@ -451,9 +440,9 @@ int vm_attn_paged_bf16(const vm_attn_paged_args* args_host, void* stream) {
   if (a.split && p.max_q > 0) {
     if (p.n_split > 1) p.part = (float*)(ws + a.part);
     if (p.w_out) { p.s_ws = (float*)(ws + a.s_ws); p.l2_ws = (float*)(ws + a.l2_ws); }
-    if (hd == 128) launch_split<128>(p, a, st);
-    else if (hd == 64) launch_split<64>(p, a, st);
-    else launch_split<32>(p, a, st);
+    if (hd == 128) launch_split<128>(p, st);
+    else if (hd == 64) launch_split<64>(p, st);
+    else launch_split<32>(p, st);
     VM_LAUNCH_CHECK();
     return VM_OK;
   }

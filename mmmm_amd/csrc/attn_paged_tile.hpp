@@ -357,95 +357,121 @@ __global__ __launch_bounds__(NW * 64, 2) void tile_k(const AttnPagedP p) {
 
 // ----------------------------------------------------------------------------- received weights of a chunk
 // w[j] += sum over the query rows of exp2(s q_r . k_j - l2_r): the scores once more (2 hd of the 4 hd operations of the attention itself;
-// keeping them would be 4 bytes per row and token), key-stationary. A wave holds 32 tokens as A operands (HD / 16 fragments, straight from
-// the page) and walks the rows that see them, 32 at a time as B operands; the tokens' sums stay in its registers, each row tile adds in its
-// turn, and the 32 columns are added up in a fixed tree at the end. Bound by the exponentials (16 per lane and 32 x 32 tile: 256 cycles
-// beside 256 of the matrix pipe).
+// keeping them would be 4 bytes per row and token). A wave keeps 32 tokens as B operands in registers (straight from the page) and the
+// workgroup's four waves walk the rows that see them, 64 at a time through LDS as A operands: a token sits on the lane, so its sum over the
+// rows is in-lane — per tile first, then onto the running sum, halves last: a fixed order. Row numbers and lse are fetched two tiles ahead, the
+// rows one tile ahead through registers. Bound by the exponentials: 32 x (16 + 8) cycles per 64 x 32 tile beside 512 of the matrix pipe.
+// (The first form had the rows straight from memory as B operands of each wave: 60 us on 8 x 456, bound by the L1's line rate.)
 template <int HD>
-__global__ __launch_bounds__(256, 2) void weigh_k(const AttnPagedP p) {
-  constexpr int KS = HD / 16;
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), hf = lane >> 5;
+__global__ __launch_bounds__(256, 3) void weigh_k(const AttnPagedP p) {
+  constexpr int KS = HD / 16, CPR = HD / 8, NQ = CPR / 4;          // 16-byte chunks per row, chunks per thread and tile
+  __shared__ __attribute__((aligned(16))) char qbuf[2][TILE];
+  __shared__ __attribute__((aligned(16))) float s_l2[3][64];
+  __shared__ __attribute__((aligned(16))) int s_lim[3][64];
+  __shared__ int64_t s_off[3][64];                                 // element offset of the row's query, -1: no such row
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), hf = lane >> 5;
   const int hk = blockIdx.y, b = blockIdx.z;
   const SeqInfo s = seq_info(p, b);
-  const int n = min(s.len, p.w_cols), j0 = (blockIdx.x * 4 + wave) * 32;
-  if (j0 >= n) return;
+  const int n = min(s.len, p.w_cols), jw = blockIdx.x * 128, j0 = jw + wave * 32, j = j0 + (lane & 31);
+  if (jw >= n) return;
   const int R = min(s.nq, p.max_q) * p.G, past = s.len - s.nq;
-  const table_ptr table = table_of(p.c, b);
+  bool there = false;
   bf16x8_t kf[KS];
   {
-    const int j = j0 + (lane & 31);
     int page = -1;
-    if (j < n) page = table[j >> p.c.shift];
+    if (j < n) page = p.c.table[b * p.c.ld_table + (j >> p.c.shift)];
+    there = page_ok(page, p.c.n_pages);
+    const unsigned short* kr = p.c.k + (there ? page_row(page, p.c.ld_page, hk, j & p.c.mask, p.c.shift, HD) + 8 * hf : 0);
 #pragma unroll
     for (int k = 0; k < KS; ++k) {
       i32x4_t v = {0, 0, 0, 0};
-      if (j < n && page_ok(page, p.c.n_pages))
-        v = *reinterpret_cast<const i32x4_t*>(p.c.k + page_row(page, p.c.ld_page, hk, j & p.c.mask, p.c.shift, HD) + 16 * k + 8 * hf);
+      if (there) v = *reinterpret_cast<const i32x4_t*>(kr + 16 * k);
       kf[k] = __builtin_bit_cast(bf16x8_t, v);
     }
   }
   const float sc = p.scale * LOG2E;
-  float sum[16];
-#pragma unroll
-  for (int e = 0; e < 16; ++e) sum[e] = 0.f;
-  struct Row { int prow, h, lim; float l2; };
-  auto row_of = [&](int r) -> Row {
-    Row x = {-1, 0, -1, 0.f};
+  float sum = 0.f;
+  const int rs = max(0, jw - past) * p.G / 64 * 64;                // the first tile with a row that sees one of these tokens
+  const int tiles = R > rs ? (R - rs + 63) / 64 : 0;
+  struct Info { int64_t off; float l2; int lim; };
+  auto info = [&](int r) -> Info {
+    Info x = {-1, INFINITY, -1};                                   // no such row: exp2(. - inf) = 0
     if (r < R) {
-      const int i = r / p.G;
-      x.h = hk * p.G + r - i * p.G;
-      x.prow = phys_row(p, s.p0 + i);
-      x.lim = past + i;
-      x.l2 = p.lse[x.h * p.ld_lse + s.p0 + i] * LOG2E;
-      if (x.prow < 0 || x.l2 == -INFINITY) x.lim = -1;
+      const int i = r / p.G, h = hk * p.G + r - i * p.G, prow = phys_row(p, s.p0 + i);
+      const float l2 = p.lse[h * p.ld_lse + s.p0 + i] * LOG2E;
+      if (prow >= 0 && l2 != -INFINITY) x = {prow * p.ldq + h * HD, l2, past + i};
     }
     return x;
   };
-  auto load_q = [&](const Row& x, bf16x8_t* q) {
+  auto put = [&](int slot, const Info& x) { s_off[slot][tid] = x.off; s_l2[slot][tid] = x.l2; s_lim[slot][tid] = x.lim; };
+  i32x4_t qv[NQ];
+  auto load_q = [&](int slot) {
 #pragma unroll
-    for (int k = 0; k < KS; ++k) {
-      i32x4_t v = {0, 0, 0, 0};
-      if (x.prow >= 0) v = *reinterpret_cast<const i32x4_t*>(p.q + x.prow * p.ldq + x.h * HD + 16 * k + 8 * hf);
-      q[k] = __builtin_bit_cast(bf16x8_t, v);
+    for (int i = 0; i < NQ; ++i) {
+      const int c = tid + 256 * i;
+      const int64_t off = s_off[slot][c / CPR];
+      qv[i] = (i32x4_t){0, 0, 0, 0};
+      if (off >= 0) qv[i] = *reinterpret_cast<const i32x4_t*>(p.q + off + (c % CPR) * 8);
     }
   };
-  const int r0 = max(0, j0 - past) * p.G / 32 * 32;                // the first row that sees one of these tokens
-  Row cur = row_of(r0 + (lane & 31)), nxt = row_of(r0 + 32 + (lane & 31));
-  bf16x8_t q[KS], qn[KS];
-  load_q(cur, q);
-  for (int r = r0; r < R; r += 32) {
-    load_q(nxt, qn);
-    const Row nn = row_of(r + 64 + (lane & 31));
-    f32x16_t acc = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  auto store_q = [&](char* tile) {
 #pragma unroll
-    for (int k = 0; k < KS; ++k) acc = a32::mfma32(kf[k], q[k], acc);
-    const int seen = cur.lim - j0;                                 // tokens 0 .. seen of the 32 are seen by this lane's row
-#pragma unroll
-    for (int e = 0; e < 16; ++e) {
-      const float w = fast_exp2(fmaf(acc[e], sc, -cur.l2));
-      sum[e] += acc_row(e, hf) <= seen ? w : 0.f;
+    for (int i = 0; i < NQ; ++i) {
+      const int c = tid + 256 * i, row = c / CPR, ch = c % CPR;
+      *reinterpret_cast<i32x4_t*>(tile + 2048 * (row >> 3) + 512 * (ch >> 2) + 64 * (row & 7) + 16 * ((ch & 3) ^ ((row >> 2) & 3))) = qv[i];
     }
-    cur = nxt;
-    nxt = nn;
-#pragma unroll
-    for (int k = 0; k < KS; ++k) q[k] = qn[k];
-  }
-  // the 32 rows of the columns
-#pragma unroll
-  for (int e = 0; e < 16; ++e) {
-    float x = sum[e];
-#pragma unroll
-    for (int o2 = 1; o2 < 32; o2 <<= 1) x += __shfl_xor(x, o2, 64);
-    sum[e] = x;
-  }
-#pragma unroll
-  for (int e = 0; e < 16; ++e) {
-    const int j = j0 + acc_row(e, hf);
-    if ((lane & 31) == e && j < n) {
-      const bool there = page_ok(p.c.table[b * p.c.ld_table + (j >> p.c.shift)], p.c.n_pages);
-      p.w_out[b * p.ldwo_seq + hk * p.ldwo_head + j] = p.w_in[b * p.ldw_seq + hk * p.ldw_head + j] + (there ? sum[e] : 0.f);
+  };
+  if (tiles > 0) {
+    if (tid < 64) {
+      const Info a = info(rs + tid), c = info(rs + 64 + tid);
+      put(0, a);
+      put(1, c);
     }
+    __syncthreads();
+    load_q(0);
+    store_q(qbuf[0]);
+    __syncthreads();
   }
+  const int rb0 = a32::row_base(lane, 0), rb1 = a32::row_base(lane, 1);
+  int slot = 0;
+  for (int u = 0; u < tiles; ++u) {
+    const int next = slot == 2 ? 0 : slot + 1, third = next == 2 ? 0 : next + 1;
+    Info ahead;
+    if (tid < 64) ahead = info(rs + 64 * (u + 2) + tid);
+    if (u + 1 < tiles) load_q(next);
+    const char* qt = qbuf[u & 1];
+    const int r_last = min(rs + 64 * u + 63, R - 1);
+    if (past + r_last / p.G >= j0) {
+      const bool edge = past + (rs + 64 * u) / p.G < j0 + 31;
+      float part[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int rt = 0; rt < 2; ++rt) {
+        f32x16_t acc = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int k = 0; k < KS; ++k) acc = a32::mfma32(a32::ld_row(qt + ((k & 1) ? rb1 : rb0), 8192 * rt + 512 * (k >> 1)), kf[k], acc);
+#pragma unroll
+        for (int g4 = 0; g4 < 4; ++g4) {
+          const int row = 32 * rt + 8 * g4 + 4 * hf;
+          const f32x4_t l2 = *reinterpret_cast<const f32x4_t*>(&s_l2[slot][row]);
+          i32x4_t lim = {0x7FFFFFFF, 0x7FFFFFFF, 0x7FFFFFFF, 0x7FFFFFFF};
+          if (edge) lim = *reinterpret_cast<const i32x4_t*>(&s_lim[slot][row]);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float x = fast_exp2(fmaf(acc[4 * g4 + e], sc, -l2[e]));
+            part[e] += !edge || j <= lim[e] ? x : 0.f;
+          }
+        }
+      }
+      sum += (part[0] + part[1]) + (part[2] + part[3]);
+    }
+    if (u + 1 < tiles) store_q(qbuf[(u + 1) & 1]);
+    if (tid < 64) put(third, ahead);
+    __syncthreads();
+    slot = next;
+  }
+  float a = sum, c = sum;
+  a32::swap_halves(a, c);
+  if (hf == 0 && j < n) p.w_out[b * p.ldwo_seq + hk * p.ldwo_head + j] = p.w_in[b * p.ldw_seq + hk * p.ldw_head + j] + (there ? a + c : 0.f);
 }
 
 }  // namespace apt

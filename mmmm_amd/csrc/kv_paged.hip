@@ -1,5 +1,6 @@
 // Paged KV cache of the generation path: storing new tokens (with the rotary positions of q and k) and eviction by received attention
 // weight. Replaces, for a paged cache, the rotary call and the torch.cat of /root/reference/mmmm/models/cogvlm/modeling_cogvlm.py:246-262.
+#include <mutex>
 #include "paged.hpp"
 
 namespace {
@@ -78,8 +79,10 @@ __global__ __launch_bounds__(256) void kv_append_k(const AppendP p) {
 // ----------------------------------------------------------------------------- eviction
 // One workgroup per (sample, kv head) picks the tokens that stay: the `budget` best by (key descending, index ascending), where the key
 // is 2^32 - 1 for the `recent` newest tokens, an order-preserving image of the weight for the others (NaN lowest, -0 = +0) and 0 for
-// tokens of absent pages, which never stay. The threshold key is found digit by digit (8 bits a pass, histogram in LDS) — exact, whatever
-// the distribution — and a last pass in index order emits the survivors, the first few of those AT the threshold included.
+// tokens of absent pages, which never stay. The threshold key is found digit by digit (11 + 11 + 10 bits, histogram in LDS) — exact,
+// whatever the distribution; then every thread takes a run of consecutive tokens, one scan of the (above, at the threshold) counts gives
+// each its place, and the first of those AT the threshold stay. The keys are read and made once and held in LDS (up to EV_LDS_KEYS; beyond
+// that they are made again in each pass). Latency-bound: three histogram rounds and four scans of a few hundred cycles.
 constexpr int EV_THREADS = 1024, EV_WAVES = EV_THREADS / 64;
 
 __device__ __forceinline__ unsigned weight_key(float w) {
@@ -93,7 +96,7 @@ struct EvictP {
   const float* w; float* w_new; int64_t ldw_seq, ldw_head, ldn_seq, ldn_head; int w_cols;
   const int32_t* lens; int32_t* new_lens;
   const int32_t* new_table; int64_t ld_new; int new_pages;
-  int32_t* kept; int budget, recent;
+  int32_t* kept; int budget, recent, lds_keys;
   PagedKV c;
 };
 
@@ -102,11 +105,38 @@ __device__ __forceinline__ unsigned evict_key(const EvictP& p, const float* w, c
   return j >= newest ? 0xFFFFFFFFu : weight_key(w[j]);
 }
 
+constexpr int EV_LDS_KEYS = 32768;
+
+// exclusive scan of a pair of counts over the workgroup; `total`: the sums. Two barriers.
+__device__ __forceinline__ uint2 block_scan2(uint2 v, uint2 (*ws)[EV_WAVES], uint2& total) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  uint2 x = v;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const unsigned a = __shfl_up(x.x, o, 64), b = __shfl_up(x.y, o, 64);
+    if (lane >= o) { x.x += a; x.y += b; }
+  }
+  if (lane == 63) (*ws)[wave] = x;
+  __syncthreads();
+  uint2 before = {0, 0};
+  total = {0, 0};
+#pragma unroll
+  for (int i = 0; i < EV_WAVES; ++i) {
+    const uint2 w = (*ws)[i];
+    if (i < wave) { before.x += w.x; before.y += w.y; }
+    total.x += w.x;
+    total.y += w.y;
+  }
+  __syncthreads();
+  return {before.x + x.x - v.x, before.y + x.y - v.y};
+}
+
 __global__ __launch_bounds__(EV_THREADS) void kv_evict_select_k(const EvictP p) {
-  __shared__ unsigned hist[256];
-  __shared__ unsigned sh[4];
-  __shared__ unsigned wsum[2][EV_WAVES];
-  const int hk = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  extern __shared__ unsigned keys[];              // min(n, EV_LDS_KEYS) of them
+  __shared__ unsigned hist[2048];
+  __shared__ unsigned found[2];
+  __shared__ uint2 ws[EV_WAVES];
+  const int hk = blockIdx.x, b = blockIdx.y, tid = threadIdx.x;
   const int cap = (int)min((int64_t)p.c.max_pages << p.c.shift, (int64_t)p.w_cols);
   const int n = max(0, min(p.lens[b], cap));
   const int newest = n - min(p.recent, n);
@@ -114,71 +144,65 @@ __global__ __launch_bounds__(EV_THREADS) void kv_evict_select_k(const EvictP p) 
   float* wn = p.w_new + b * p.ldn_seq + hk * p.ldn_head;
   const int32_t* table = p.c.table + b * p.c.ld_table;
   int32_t* kept = p.kept + ((int64_t)b * p.c.n_kv_heads + hk) * p.budget;
+  const bool in_lds = n <= p.lds_keys;
+  auto key_of = [&](int j) -> unsigned { return in_lds ? keys[j] : evict_key(p, w, table, j, newest); };
   // ---- threshold
   unsigned prefix = 0, pmask = 0;
   int want = 0, keep = 0;                         // how many of the keys that share the prefix stay
-  for (int pass = 0; pass < 4; ++pass) {
-    const int sh_bits = 24 - 8 * pass;
-    for (int i = tid; i < 256; i += EV_THREADS) hist[i] = 0;
-    if (tid == 0) sh[2] = 0;
+  for (int pass = 0; pass < 3; ++pass) {
+    const int bits = pass < 2 ? 11 : 10, shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
+    hist[tid] = hist[tid + EV_THREADS] = 0;
     __syncthreads();
-    unsigned present = 0;
     for (int j = tid; j < n; j += EV_THREADS) {
-      const unsigned key = evict_key(p, w, table, j, newest);
-      if (key != 0) {
-        ++present;
-        if ((key & pmask) == prefix) atomicAdd(&hist[(key >> sh_bits) & 255], 1u);
+      unsigned key;
+      if (pass == 0) {
+        key = evict_key(p, w, table, j, newest);
+        if (in_lds) keys[j] = key;
+      } else {
+        key = key_of(j);
       }
-    }
-    if (pass == 0 && present) atomicAdd(&sh[2], present);
-    __syncthreads();
-    if (pass == 0) keep = want = min((int)sh[2], p.budget);
-    if (tid == 0) {                               // the digit whose bin holds the want-th largest key
-      unsigned above = 0;
-      int d = 255;
-      for (; d > 0; --d) {
-        if (above + hist[d] >= (unsigned)want) break;
-        above += hist[d];
-      }
-      sh[0] = (unsigned)d;
-      sh[1] = above;
+      if (key != 0 && (key & pmask) == prefix) atomicAdd(&hist[(key >> shift) & ((1 << bits) - 1)], 1u);
     }
     __syncthreads();
-    prefix |= sh[0] << sh_bits;
-    pmask |= 0xFFu << sh_bits;
-    want -= (int)sh[1];
+    // bins in descending order, two per thread: the one that holds the want-th largest key
+    const unsigned h0 = hist[2047 - 2 * tid], h1 = hist[2046 - 2 * tid];
+    uint2 all;
+    const unsigned above = block_scan2({h0 + h1, 0}, &ws, all).x;
+    if (pass == 0) keep = want = min((int)all.x, p.budget);
+    if (above < (unsigned)want && (unsigned)want <= above + h0 + h1) {
+      const bool second = (unsigned)want > above + h0;
+      found[0] = 2047 - 2 * tid - (second ? 1 : 0);
+      found[1] = above + (second ? h0 : 0);
+    }
     __syncthreads();
+    if (want > 0) {
+      prefix |= found[0] << shift;
+      want -= (int)found[1];
+    }
+    pmask |= ((1u << bits) - 1) << shift;
   }
   // ---- survivors in index order
-  int out0 = 0, eq0 = 0;
-  for (int j0 = 0; j0 < n && out0 < keep; j0 += EV_THREADS) {
-    const int j = j0 + tid;
-    const unsigned key = j < n ? evict_key(p, w, table, j, newest) : 0u;
-    const bool eq = key != 0 && key == prefix, gt = key > prefix;
-    const uint64_t beq = __ballot(eq);
-    if (lane == 0) wsum[0][wave] = __popcll(beq);
-    __syncthreads();
-    int eq_before = eq0 + __popcll(beq & ((1ull << lane) - 1)), eq_all = 0;
-    for (int i = 0; i < EV_WAVES; ++i) {
-      if (i < wave) eq_before += wsum[0][i];
-      eq_all += wsum[0][i];
+  if (keep > 0) {
+    const int run = ((n + EV_THREADS - 1) / EV_THREADS) | 1;        // odd: no LDS bank conflicts between the threads' runs
+    const int j0 = min(tid * run, n), j1 = min(j0 + run, n);
+    uint2 c = {0, 0}, all;
+    for (int j = j0; j < j1; ++j) {
+      const unsigned key = key_of(j);
+      c.x += key > prefix;
+      c.y += key == prefix;
     }
-    const bool stay = gt || (eq && eq_before < want);
-    const uint64_t bst = __ballot(stay);
-    if (lane == 0) wsum[1][wave] = __popcll(bst);
-    __syncthreads();
-    int at = out0 + __popcll(bst & ((1ull << lane) - 1)), all = 0;
-    for (int i = 0; i < EV_WAVES; ++i) {
-      if (i < wave) at += wsum[1][i];
-      all += wsum[1][i];
+    const uint2 before = block_scan2(c, &ws, all);
+    unsigned eq = before.y, at = before.x + min(eq, (unsigned)want);
+    for (int j = j0; j < j1; ++j) {
+      const unsigned key = key_of(j);
+      const bool tie = key == prefix;
+      if (key > prefix || (tie && eq < (unsigned)want)) {
+        kept[at] = j;
+        wn[at] = w[j];
+        ++at;
+      }
+      eq += tie;
     }
-    if (stay && at < keep) {
-      kept[at] = j;
-      if (at < p.w_cols) wn[at] = w[j];
-    }
-    out0 += all;
-    eq0 += eq_all;
-    __syncthreads();
   }
   for (int j = keep + tid; j < p.budget; j += EV_THREADS) kept[j] = -1;
   for (int j = keep + tid; j < p.w_cols; j += EV_THREADS) wn[j] = 0.f;      // the next tokens of this sample start at zero
@@ -249,7 +273,14 @@ int vm_kv_evict_paged_bf16(const vm_paged_kv* cache_host, const float* weights, 
   p.lens = kv_lens; p.new_lens = new_lens; p.new_table = new_table; p.ld_new = ld_new_table; p.new_pages = new_pages;
   p.kept = kept; p.budget = budget; p.recent = recent;
   hipStream_t st = (hipStream_t)stream;
-  hipLaunchKernelGGL(kv_evict_select_k, dim3(p.c.n_kv_heads, cache_host->n_seq), dim3(EV_THREADS), 0, st, p);
+  static std::once_flag once;
+  static bool ok = false;
+  std::call_once(once, [] { ok = hipFuncSetAttribute((const void*)kv_evict_select_k, hipFuncAttributeMaxDynamicSharedMemorySize, EV_LDS_KEYS * 4) == hipSuccess; });
+  if (!ok) return VM_ERR_LAUNCH;
+  const int64_t most = (int64_t)p.c.max_pages << p.c.shift;
+  const int cols = (int)(most < w_cols ? most : w_cols);
+  p.lds_keys = cols < EV_LDS_KEYS ? cols : EV_LDS_KEYS;
+  hipLaunchKernelGGL(kv_evict_select_k, dim3(p.c.n_kv_heads, cache_host->n_seq), dim3(EV_THREADS), p.lds_keys * 4, st, p);
   VM_LAUNCH_CHECK();
   const int hd = cache_host->head_dim, rpb = 256 / (hd / 8);
   const dim3 grid((budget + rpb - 1) / rpb, p.c.n_kv_heads, cache_host->n_seq);
