@@ -401,13 +401,19 @@ void launch_split(const AttnPagedP& p, hipStream_t st) {
   if (p.w_out && p.max_kv > 0) hipLaunchKernelGGL(attn_paged_count_k, dim3((p.max_kv + 255) / 256, p.c.n_kv_heads, p.n_seq), dim3(256), 0, st, p);
 }
 
+// workgroups of the tile form: eight XCDs, each as many as the longest piece of the list (tile_k: whole caches where the list is short)
+int64_t tile_grid(const AttnPagedP& p) {
+  const int64_t caches = (int64_t)p.n_seq * p.c.n_kv_heads, even = ((int64_t)p.n_wg + 7) / 8, whole = (caches + 7) / 8 * p.n_tiles * p.n_split;
+  return 8 * (whole > even ? whole : even);
+}
+
 template <int HD>
 int launch_tile(const AttnPagedP& p, hipStream_t st) {
   static std::once_flag once;
   static bool ok = false;
   std::call_once(once, [] { ok = hipFuncSetAttribute((const void*)apt::tile_k<HD>, hipFuncAttributeMaxDynamicSharedMemorySize, apt::RING_LDS) == hipSuccess; });
   if (!ok) return VM_ERR_LAUNCH;
-  hipLaunchKernelGGL(apt::tile_k<HD>, dim3((p.n_wg + 7) / 8 * 8), dim3(apt::NW * 64), apt::RING_LDS, st, p);
+  hipLaunchKernelGGL(apt::tile_k<HD>, dim3((unsigned)tile_grid(p)), dim3(apt::NW * 64), apt::RING_LDS, st, p);
   if (p.n_split > 1) hipLaunchKernelGGL(attn_paged_join_k<HD>, dim3((p.s_rows + 3) / 4, p.c.n_kv_heads, p.n_seq), dim3(256), 0, st, p);
   if (p.w_out && p.max_kv > 0) hipLaunchKernelGGL(apt::weigh_k<HD>, dim3((p.max_kv + 127) / 128, p.c.n_kv_heads, p.n_seq), dim3(256), 0, st, p);
   VM_LAUNCH_CHECK();
