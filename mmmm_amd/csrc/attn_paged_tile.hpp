@@ -12,6 +12,7 @@
 //  * with fewer than one workgroup per CU the keys are split over workgroups too (partial results joined by attn_paged_join_k);
 //  * V^T fragments are read in two assembly statements of 16 ds_read_b64_tr_b16 that end in their own wait.
 #pragma once
+#include <type_traits>
 #include "attn32_tile.hpp"
 
 namespace apt {
@@ -378,7 +379,7 @@ __global__ __launch_bounds__(NW * 64, 2) void tile_k(const AttnPagedP p) {
 // rows one tile ahead through registers. Bound by the exponentials: 32 x (16 + 8) cycles per 64 x 32 tile beside 512 of the matrix pipe.
 // (The first form had the rows straight from memory as B operands of each wave: 60 us on 8 x 456, bound by the L1's line rate.)
 template <int HD>
-__global__ __launch_bounds__(256, 3) void weigh_k(const AttnPagedP p) {
+__global__ __launch_bounds__(256, 2) void weigh_k(const AttnPagedP p) {
   constexpr int KS = HD / 16, CPR = HD / 8, NQ = CPR / 4;          // 16-byte chunks per row, chunks per thread and tile
   __shared__ __attribute__((aligned(16))) char qbuf[2][TILE];
   __shared__ __attribute__((aligned(16))) float s_l2[3][64];
@@ -396,37 +397,44 @@ __global__ __launch_bounds__(256, 3) void weigh_k(const AttnPagedP p) {
     int page = -1;
     if (j < n) page = p.c.table[b * p.c.ld_table + (j >> p.c.shift)];
     there = page_ok(page, p.c.n_pages);
-    const unsigned short* kr = p.c.k + (there ? page_row(page, p.c.ld_page, hk, j & p.c.mask, p.c.shift, HD) + 8 * hf : 0);
+    // (a token that is not there reads row 0 of the pool and counts as zeros: no branch per load)
+    const unsigned short* kr = p.c.k + (there ? page_row(page, p.c.ld_page, hk, j & p.c.mask, p.c.shift, HD) : 0) + 8 * hf;
 #pragma unroll
     for (int k = 0; k < KS; ++k) {
-      i32x4_t v = {0, 0, 0, 0};
-      if (there) v = *reinterpret_cast<const i32x4_t*>(kr + 16 * k);
-      kf[k] = __builtin_bit_cast(bf16x8_t, v);
+      const i32x4_t v = *reinterpret_cast<const i32x4_t*>(kr + 16 * k);
+      kf[k] = __builtin_bit_cast(bf16x8_t, there ? v : (i32x4_t){0, 0, 0, 0});
     }
   }
   const float sc = p.scale * LOG2E;
   float sum = 0.f;
   const int rs = max(0, jw - past) * p.G / 64 * 64;                // the first tile with a row that sees one of these tokens
   const int tiles = R > rs ? (R - rs + 63) / 64 : 0;
-  struct Info { int64_t off; float l2; int lim; };
+  struct Info { int r, i, h, row; float lse; };                    // as loaded: looked at when it is put into LDS, a tile later
   auto info = [&](int r) -> Info {
-    Info x = {-1, INFINITY, -1};                                   // no such row: exp2(. - inf) = 0
-    if (r < R) {
-      const int i = r / p.G, h = hk * p.G + r - i * p.G, prow = phys_row(p, s.p0 + i);
-      const float l2 = p.lse[h * p.ld_lse + s.p0 + i] * LOG2E;
-      if (prow >= 0 && l2 != -INFINITY) x = {prow * p.ldq + h * HD, l2, past + i};
-    }
+    Info x;
+    x.r = r;
+    const int rr = min(r, R - 1);
+    x.i = p.G == 1 ? rr : rr / p.G;
+    x.h = hk * p.G + rr - x.i * p.G;
+    x.row = s.p0 + x.i;
+    if (p.row_of_pos) x.row = p.row_of_pos[s.p0 + x.i];
+    x.lse = p.lse[x.h * p.ld_lse + s.p0 + x.i];
     return x;
   };
-  auto put = [&](int slot, const Info& x) { s_off[slot][tid] = x.off; s_l2[slot][tid] = x.l2; s_lim[slot][tid] = x.lim; };
+  auto put = [&](int slot, const Info& x) {
+    const bool ok = x.r < R && (unsigned)x.row < (unsigned)p.n_rows && x.lse != -INFINITY;
+    s_off[slot][tid] = ok ? x.row * p.ldq + x.h * HD : -1;
+    s_l2[slot][tid] = ok ? x.lse * LOG2E : INFINITY;               // no such row: exp2(. - inf) = 0
+    s_lim[slot][tid] = ok ? past + x.i : -1;
+  };
   i32x4_t qv[NQ];
   auto load_q = [&](int slot) {
 #pragma unroll
     for (int i = 0; i < NQ; ++i) {
       const int c = tid + 256 * i;
       const int64_t off = s_off[slot][c / CPR];
-      qv[i] = (i32x4_t){0, 0, 0, 0};
-      if (off >= 0) qv[i] = *reinterpret_cast<const i32x4_t*>(p.q + off + (c % CPR) * 8);
+      const i32x4_t v = *reinterpret_cast<const i32x4_t*>(p.q + (off < 0 ? 0 : off) + (c % CPR) * 8);
+      qv[i] = off < 0 ? (i32x4_t){0, 0, 0, 0} : v;
     }
   };
   auto store_q = [&](char* tile) {
@@ -448,6 +456,31 @@ __global__ __launch_bounds__(256, 3) void weigh_k(const AttnPagedP p) {
     __syncthreads();
   }
   const int rb0 = a32::row_base(lane, 0), rb1 = a32::row_base(lane, 1);
+  // 64 rows against the wave's 32 tokens; edge: some rows do not see some of the tokens
+  auto add = [&](const char* qt, int slot, auto edge) {
+    f32x16_t acc[2];
+#pragma unroll
+    for (int rt = 0; rt < 2; ++rt) {
+      acc[rt] = (f32x16_t){0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int k = 0; k < KS; ++k) acc[rt] = a32::mfma32(a32::ld_row(qt + ((k & 1) ? rb1 : rb0), 8192 * rt + 512 * (k >> 1)), kf[k], acc[rt]);
+    }
+    float part[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int g4 = 0; g4 < 8; ++g4) {
+      const int row = 8 * g4 + 4 * hf;
+      const f32x4_t l2 = *reinterpret_cast<const f32x4_t*>(&s_l2[slot][row]);
+      i32x4_t lim;
+      if constexpr (decltype(edge)::value) lim = *reinterpret_cast<const i32x4_t*>(&s_lim[slot][row]);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float x = fast_exp2(fmaf(acc[g4 >> 2][4 * (g4 & 3) + e], sc, -l2[e]));
+        if constexpr (decltype(edge)::value) part[e] += j <= lim[e] ? x : 0.f;
+        else part[e] += x;
+      }
+    }
+    sum += (part[0] + part[1]) + (part[2] + part[3]);
+  };
   int slot = 0;
   for (int u = 0; u < tiles; ++u) {
     const int next = slot == 2 ? 0 : slot + 1, third = next == 2 ? 0 : next + 1;
@@ -457,27 +490,8 @@ __global__ __launch_bounds__(256, 3) void weigh_k(const AttnPagedP p) {
     const char* qt = qbuf[u & 1];
     const int r_last = min(rs + 64 * u + 63, R - 1);
     if (past + r_last / p.G >= j0) {
-      const bool edge = past + (rs + 64 * u) / p.G < j0 + 31;
-      float part[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int rt = 0; rt < 2; ++rt) {
-        f32x16_t acc = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int k = 0; k < KS; ++k) acc = a32::mfma32(a32::ld_row(qt + ((k & 1) ? rb1 : rb0), 8192 * rt + 512 * (k >> 1)), kf[k], acc);
-#pragma unroll
-        for (int g4 = 0; g4 < 4; ++g4) {
-          const int row = 32 * rt + 8 * g4 + 4 * hf;
-          const f32x4_t l2 = *reinterpret_cast<const f32x4_t*>(&s_l2[slot][row]);
-          i32x4_t lim = {0x7FFFFFFF, 0x7FFFFFFF, 0x7FFFFFFF, 0x7FFFFFFF};
-          if (edge) lim = *reinterpret_cast<const i32x4_t*>(&s_lim[slot][row]);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float x = fast_exp2(fmaf(acc[4 * g4 + e], sc, -l2[e]));
-            part[e] += !edge || j <= lim[e] ? x : 0.f;
-          }
-        }
-      }
-      sum += (part[0] + part[1]) + (part[2] + part[3]);
+      if (past + (rs + 64 * u) / p.G < j0 + 31) add(qt, slot, std::true_type{});
+      else add(qt, slot, std::false_type{});
     }
     if (u + 1 < tiles) store_q(qbuf[(u + 1) & 1]);
     if (tid < 64) put(third, ahead);
