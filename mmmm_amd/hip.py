@@ -10,6 +10,7 @@ import ctypes as C
 import os
 from pathlib import Path
 import re
+import struct
 
 import torch
 
@@ -112,6 +113,16 @@ class AttnPagedArgs(C.Structure):
         ('workspace', C.c_void_p), ('workspace_bytes', C.c_int64),
     ]
 
+
+def _packer(cls) -> struct.Struct:
+    """the same bytes as the C struct from one pack(*fields) call: a decode step fills such a struct per layer, and a ctypes attribute at a
+    time costs 0.15 us each"""
+    codes = {C.c_void_p: 'Q', C.c_int64: 'q', C.c_uint64: 'Q', C.c_int32: 'i', C.c_float: 'f'}
+    fmt = lambda c: ''.join(fmt(t) if issubclass(t, C.Structure) else codes[t] for _, t in c._fields_)      # noqa: E731
+    return struct.Struct('=' + fmt(cls))
+
+
+PAGED_KV, ATTN_PAGED = _packer(PagedKVArgs), _packer(AttnPagedArgs)      # (no padding inside either: tests/test_paged_cpu.py)
 
 TN_GROUP_MAX = 32
 

@@ -819,29 +819,47 @@ def attn_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k
     return out
 
 
-def _paged_cache(k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: torch.Tensor) -> hip.PagedKVArgs:
-    """checked vm_paged_kv of a paged cache: k_pages / v_pages bf16 [pages, kv heads, page size, head dim] (page stride free),
-    block_table int32 [samples, pages per sample]"""
-    assert k_pages.dim() == 4 and k_pages.shape == v_pages.shape and k_pages.stride() == v_pages.stride(), (k_pages.shape, v_pages.shape)
-    assert k_pages.dtype == torch.bfloat16 and v_pages.dtype == torch.bfloat16, 'the paged cache is bf16'
-    n, hk, ps, hd = k_pages.shape
-    assert k_pages.stride()[1:] == (ps * hd, hd, 1), 'a page is contiguous: [kv heads, page size, head dim]'
+@functools.lru_cache(maxsize=256)
+def _paged_geometry(shape, stride, v_shape, v_stride, dtype, v_dtype):
+    """(pages, kv heads, page size, head dim, page stride) of a checked pair of page pools"""
+    assert len(shape) == 4 and shape == v_shape and stride == v_stride, (shape, v_shape, stride, v_stride)
+    assert dtype == torch.bfloat16 and v_dtype == torch.bfloat16, 'the paged cache is bf16'
+    n, hk, ps, hd = shape
+    assert stride[1:] == (ps * hd, hd, 1), 'a page is contiguous: [kv heads, page size, head dim]'
     assert hd in (32, 64, 128), f'head_dim {hd}: 32, 64 or 128'
     assert 16 <= ps <= 1024 and ps & (ps - 1) == 0, f'page size {ps}: a power of two in 16 .. 1024'
-    assert block_table.dtype == torch.int32 and block_table.dim() == 2 and block_table.stride(1) == 1 and block_table.shape[1] > 0
-    assert k_pages.device == v_pages.device == block_table.device
-    c = hip.PagedKVArgs()
-    c.k_pages, c.v_pages, c.ld_page = ptr(k_pages), ptr(v_pages), k_pages.stride(0) if n > 1 else hk * ps * hd
-    c.n_pages, c.page_size, c.n_kv_heads, c.head_dim = n, ps, hk, hd
-    c.block_table, c.max_pages, c.n_seq = ptr(block_table), block_table.shape[1], block_table.shape[0]
-    c.ld_table = block_table.stride(0) if block_table.shape[0] > 1 else block_table.shape[1]
-    assert k_pages.device.index == torch.cuda.current_device(), 'the cache lies on another device than the current one'
-    return c
+    return n, hk, ps, hd, stride[0] if n > 1 else hk * ps * hd
 
 
-def _i32(t: torch.Tensor, n: int, like: torch.Tensor) -> torch.Tensor:
-    assert t.dtype == torch.int32 and t.is_contiguous() and t.numel() >= n and t.device == like.device, (t.dtype, t.shape, n)
-    return t
+def _paged(k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: torch.Tensor):
+    """checked fields of vm_paged_kv: k_pages / v_pages bf16 [pages, kv heads, page size, head dim] (page stride free), block_table int32
+    [samples, pages per sample]"""
+    n, hk, ps, hd, ld = _paged_geometry(k_pages.shape, k_pages.stride(), v_pages.shape, v_pages.stride(), k_pages.dtype, v_pages.dtype)
+    assert block_table.dtype == torch.int32 and block_table.dim() == 2 and block_table.shape[1] > 0
+    n_seq, cols = block_table.shape
+    row, one = block_table.stride()
+    assert one == 1 or cols == 1
+    dev = k_pages.get_device()
+    assert v_pages.get_device() == dev and block_table.get_device() == dev
+    return (k_pages.data_ptr(), v_pages.data_ptr(), ld, n, ps, block_table.data_ptr(), row if n_seq > 1 else cols, cols, n_seq, hk, hd), dev
+
+
+def _here(t: torch.Tensor, dev: int):
+    """the launch goes to the current device's stream: what it works on has to lie there"""
+    if dev < 0:
+        ptr(t)                                          # raises: there is no CPU path
+    assert dev == torch.cuda.current_device(), f'the cache lies on device {dev}, the current one is {torch.cuda.current_device()}'
+
+
+def _i32(t: torch.Tensor, n: int, dev: int) -> int:
+    assert t.dtype == torch.int32 and t.is_contiguous() and t.numel() >= n and t.get_device() == dev, (t.dtype, t.shape, n)
+    return t.data_ptr()
+
+
+def _rows(t: torch.Tensor, shape, dev: int) -> tuple[int, int]:
+    """pointer and row stride of a bf16 [rows, cols] view with unit inner stride"""
+    assert t.dtype == torch.bfloat16 and t.shape == shape and t.get_device() == dev, (t.dtype, t.shape, shape)
+    return t.data_ptr(), _ld(t)
 
 
 def kv_append_paged(qkv: torch.Tensor, row_seq: torch.Tensor, row_index: torch.Tensor, block_table: torch.Tensor, k_pages: torch.Tensor,
@@ -850,28 +868,48 @@ def kv_append_paged(qkv: torch.Tensor, row_seq: torch.Tensor, row_index: torch.T
     """new tokens into a paged cache, rotary positions included (vm_kv_append_paged_bf16). qkv [T, (n_heads + 2 kv heads) hd] bf16, not
     changed; row r is token row_index[r] of sample row_seq[r] (out of range, e.g. -1: not stored) at position row_pos[r]; all int32.
     -> rotated q [T, n_heads hd]"""
+    c, dev = _paged(k_pages, v_pages, block_table)
+    hk, hd = c[9], c[10]
     T = qkv.shape[0]
-    _, hk, _, hd = k_pages.shape
-    assert qkv.dim() == 2 and qkv.dtype == torch.bfloat16 and qkv.stride(1) == 1 and qkv.shape[1] == (n_heads + 2 * hk) * hd, (qkv.shape, n_heads, hk, hd)
-    assert qkv.device == k_pages.device and n_heads > 0
-    assert cos.dtype == torch.float32 and sin.dtype == torch.float32 and cos.is_contiguous() and sin.is_contiguous()
-    assert cos.shape == sin.shape and cos.dim() == 2 and cos.shape[1] == hd and cos.device == sin.device == qkv.device
+    x, ldx = _rows(qkv, (T, (n_heads + 2 * hk) * hd), dev)
+    assert n_heads > 0 and cos.dtype == torch.float32 and sin.dtype == torch.float32 and cos.is_contiguous() and sin.is_contiguous()
+    assert cos.shape == sin.shape and cos.dim() == 2 and cos.shape[1] == hd and cos.get_device() == dev and sin.get_device() == dev
+    seq, idx, pos = _i32(row_seq, T, dev), _i32(row_index, T, dev), _i32(row_pos, T, dev)
+    _here(k_pages, dev)
     if q_out is None:
-        q_out = torch.empty(T, n_heads * hd, dtype=qkv.dtype, device=qkv.device)
-    assert q_out.shape == (T, n_heads * hd) and q_out.dtype == qkv.dtype and q_out.stride(1) == 1 and q_out.device == qkv.device
-    for t in (row_seq, row_index, row_pos):
-        _i32(t, T, qkv)
-    c = _paged_cache(k_pages, v_pages, block_table)
+        q_out = qkv.new_empty((T, n_heads * hd))
+    o, ldo = _rows(q_out, (T, n_heads * hd), dev)
     if T:
-        hip.call('vm_kv_append_paged_bf16', C.addressof(c), ptr(qkv), _ld(qkv), ptr(row_seq), ptr(row_index), ptr(row_pos), ptr(cos), ptr(sin),
-                 cos.shape[0], T, n_heads, ptr(q_out), _ld(q_out), ptr(_i32(nrows, 1, qkv)) if nrows is not None else None, stream())
+        hip.call('vm_kv_append_paged_bf16', hip.PAGED_KV.pack(*c), x, ldx, seq, idx, pos,
+                 cos.data_ptr(), sin.data_ptr(), cos.shape[0], T, n_heads, o, ldo, None if nrows is None else _i32(nrows, 1, dev), stream())
     return q_out
 
 
-def _weights_view(w: torch.Tensor, n_seq: int, n_kv_heads: int, like: torch.Tensor) -> torch.Tensor:
-    assert w.dtype == torch.float32 and w.dim() == 3 and w.shape[:2] == (n_seq, n_kv_heads) and w.stride(2) == 1 and w.device == like.device, w.shape
-    assert w.shape[2] > 0 and (n_kv_heads == 1 or w.stride(1) >= w.shape[2])
-    return w
+def _weights_of(w: torch.Tensor, n_seq: int, n_kv_heads: int, dev: int) -> tuple[int, int, int, int]:
+    """pointer, sample stride, head stride and columns of fp32 [samples, kv heads, tokens]"""
+    assert w.dtype == torch.float32 and w.dim() == 3 and w.get_device() == dev, (w.dtype, w.shape)
+    s, h, cols = w.shape
+    ls, lh, one = w.stride()
+    assert (s, h) == (n_seq, n_kv_heads) and cols > 0 and one == 1 and (h == 1 or lh >= cols), (w.shape, w.stride())
+    return w.data_ptr(), ls, lh if h > 1 else max(lh, cols), cols
+
+
+@functools.lru_cache(maxsize=512)
+def _attn_paged_ws_bytes(n_seq: int, hk: int, hd: int, page_size: int, max_pages: int, rows: int, max_q: int, max_kv: int, n_heads: int, w_cols: int) -> int:
+    """(the library looks at sizes only: the pointers stand for any aligned ones)"""
+    a, n, any_ = hip.AttnPagedArgs(), C.c_int64(0), 1 << 20
+    c = a.cache
+    c.k_pages = c.v_pages = c.block_table = any_
+    c.ld_page, c.n_pages, c.page_size, c.ld_table, c.max_pages, c.n_seq, c.n_kv_heads, c.head_dim = hk * page_size * hd, 1, page_size, max_pages, max_pages, n_seq, hk, hd
+    a.q = a.out = a.lse = a.cu_q = a.kv_lens = any_
+    a.ldq = a.ldo = n_heads * hd
+    a.ld_lse = a.n_rows = rows
+    a.max_q, a.max_kv, a.n_heads, a.scale = max_q, max_kv, n_heads, 1.0
+    if w_cols:
+        a.weights = a.weights_out = any_
+        a.w_cols = a.ldw_head = a.ldwo_head = w_cols
+    hip.call('vm_attn_paged_workspace', C.addressof(a), C.addressof(n))
+    return n.value
 
 
 def attn_paged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: torch.Tensor, cu_q: torch.Tensor,
@@ -882,68 +920,57 @@ def attn_paged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, bl
     row_of_pos: packed row of a position. max_q / max_kv: host upper bounds of the new and of the cached tokens of a sample.
     weights [samples, kv heads, >= max_kv] fp32: the attention weight every token has received so far; with this call's added it goes to
     weights_out (default: in place). -> (out [rows, heads hd], lse fp32 [heads, rows] by position)"""
-    rows = q.shape[0]
-    n_seq = block_table.shape[0]
-    _, hk, _, hd = k_pages.shape
-    assert q.dim() == 2 and q.dtype == torch.bfloat16 and q.stride(1) == 1 and q.shape[1] % hd == 0 and q.device == k_pages.device
-    n_heads = q.shape[1] // hd
-    assert n_heads > 0 and n_heads % hk == 0, f'{n_heads} query heads over {hk} kv heads'
+    c, dev = _paged(k_pages, v_pages, block_table)
+    ps, cols, n_seq, hk, hd = c[4], c[7], c[8], c[9], c[10]
+    assert q.dim() == 2
+    rows, width = q.shape
+    n_heads = width // hd
+    assert width == n_heads * hd and n_heads > 0 and n_heads % hk == 0, f'q {tuple(q.shape)}: heads of {hd}, a multiple of {hk} of them'
     assert math.isfinite(scale) and scale > 0 and max_q >= 0 and max_kv >= 0
-    a = hip.AttnPagedArgs()
-    a.cache = _paged_cache(k_pages, v_pages, block_table)
-    if out is None:
-        out = torch.empty(rows, n_heads * hd, dtype=q.dtype, device=q.device)
-    assert out.shape == q.shape and out.dtype == q.dtype and out.stride(1) == 1 and out.device == q.device
-    lse = torch.empty(n_heads, rows, dtype=torch.float32, device=q.device)
-    a.q, a.ldq, a.out, a.ldo = ptr(q), _ld(q), ptr(out), _ld(out)
-    a.cu_q, a.kv_lens = ptr(_i32(cu_q, n_seq + 1, q)), ptr(_i32(kv_lens, n_seq, q))
-    if row_of_pos is not None:
-        a.row_of_pos = ptr(_i32(row_of_pos, rows, q))
-    a.lse, a.ld_lse = ptr(lse), rows
-    a.n_rows, a.max_q, a.max_kv, a.n_heads, a.scale = rows, max_q, max_kv, n_heads, scale
+    qp, ldq = _rows(q, q.shape, dev)
+    cu, lens, order = _i32(cu_q, n_seq + 1, dev), _i32(kv_lens, n_seq, dev), 0 if row_of_pos is None else _i32(row_of_pos, rows, dev)
+    w = wo = ws_ = wh = wos = woh = w_cols = 0
     if weights is not None:
-        w_out = weights if weights_out is None else weights_out
-        _weights_view(weights, n_seq, hk, q), _weights_view(w_out, n_seq, hk, q)
-        assert w_out.shape == weights.shape and weights.shape[2] >= min(max_kv, block_table.shape[1] * k_pages.shape[2])
-        a.weights, a.weights_out, a.w_cols = ptr(weights), ptr(w_out), weights.shape[2]
-        a.ldw_seq, a.ldw_head, a.ldwo_seq, a.ldwo_head = weights.stride(0), _w_head(weights), w_out.stride(0), _w_head(w_out)
+        w, ws_, wh, w_cols = _weights_of(weights, n_seq, hk, dev)
+        wo, wos, woh, wo_cols = _weights_of(weights if weights_out is None else weights_out, n_seq, hk, dev)
+        assert wo_cols == w_cols and w_cols >= min(max_kv, cols * ps), f'{w_cols} columns of weights'
     else:
         assert weights_out is None
-    need = C.c_int64(0)
-    hip.call('vm_attn_paged_workspace', C.addressof(a), C.addressof(need))
-    if need.value:
-        ws = torch.empty(need.value, dtype=torch.uint8, device=q.device)
-        a.workspace, a.workspace_bytes = ptr(ws), need.value
-    hip.call('vm_attn_paged_bf16', C.addressof(a), stream())
+    _here(k_pages, dev)
+    if out is None:
+        out = q.new_empty((rows, width))
+    op, ldo = _rows(out, q.shape, dev)
+    lse = torch.empty(n_heads, rows, dtype=torch.float32, device=q.device)
+    need = _attn_paged_ws_bytes(n_seq, hk, hd, ps, cols, rows, max_q, max_kv, n_heads, w_cols)
+    ws = torch.empty(need, dtype=torch.uint8, device=q.device).data_ptr() if need else 0
+    hip.call('vm_attn_paged_bf16', hip.ATTN_PAGED.pack(
+        *c, qp, ldq, cu, lens, order, op, ldo, lse.data_ptr(), rows, rows, max_q, max_kv, n_heads, scale, w_cols, w, wo, ws_, wh, wos, woh, ws, need), stream())
     return out, lse
-
-
-def _w_head(w: torch.Tensor) -> int:
-    return w.stride(1) if w.shape[1] > 1 else max(w.stride(1), w.shape[2])
 
 
 def kv_evict_paged(k_pages: torch.Tensor, v_pages: torch.Tensor, weights: torch.Tensor, block_table: torch.Tensor, kv_lens: torch.Tensor,
                    new_block_table: torch.Tensor, budget: int, recent: int):
     """of every sample and kv head the `budget` tokens stay that are among the `recent` newest or have received the most attention weight
-    (weights fp32 [samples, kv heads, cols]; ties: the older token), in their order, in the pages of new_block_table — pages that nothing
-    else uses; the old ones are not changed (vm_kv_evict_paged_bf16). -> (new weights, new lens int32 [samples], kept int32 [samples,
-    kv heads, budget]: old indices, -1 behind the last)"""
-    n_seq = block_table.shape[0]
-    _, hk, ps, _ = k_pages.shape
-    c = _paged_cache(k_pages, v_pages, block_table)
-    _weights_view(weights, n_seq, hk, k_pages)
-    _i32(kv_lens, n_seq, k_pages)
+    (weights fp32 [samples, kv heads, cols], a column for every cached token; ties: the older token), in their order, in the pages of
+    new_block_table — pages that nothing else uses; the old ones are not changed (vm_kv_evict_paged_bf16). -> (new weights, new lens int32
+    [samples], kept int32 [samples, kv heads, budget]: old indices, -1 behind the last)"""
+    c, dev = _paged(k_pages, v_pages, block_table)
+    ps, cols, n_seq, hk = c[4], c[7], c[8], c[9]
+    w, ws_, wh, w_cols = _weights_of(weights, n_seq, hk, dev)
     assert 0 < budget and 0 <= recent <= budget, (budget, recent)
-    assert new_block_table.dtype == torch.int32 and new_block_table.dim() == 2 and new_block_table.shape[0] == n_seq and new_block_table.stride(1) == 1
-    assert new_block_table.device == k_pages.device and new_block_table.data_ptr() != block_table.data_ptr()
-    most = min(budget, block_table.shape[1] * ps, weights.shape[2])
-    assert new_block_table.shape[1] * ps >= most, f'{most} tokens may stay: the new table holds {new_block_table.shape[1] * ps}'
-    new_w = torch.empty(weights.shape, dtype=torch.float32, device=weights.device)
+    assert new_block_table.dtype == torch.int32 and new_block_table.dim() == 2 and new_block_table.shape[0] == n_seq
+    new_cols = new_block_table.shape[1]
+    row, one = new_block_table.stride()
+    assert (one == 1 or new_cols == 1) and new_block_table.get_device() == dev and new_block_table.data_ptr() != block_table.data_ptr()
+    most = min(budget, cols * ps, w_cols)
+    assert new_cols * ps >= most, f'{most} tokens may stay: the new table holds {new_cols * ps}'
+    lens = _i32(kv_lens, n_seq, dev)
+    _here(k_pages, dev)
+    new_w = torch.empty(n_seq, hk, w_cols, dtype=torch.float32, device=weights.device)
     new_lens = torch.empty(n_seq, dtype=torch.int32, device=weights.device)
     kept = torch.empty(n_seq, hk, budget, dtype=torch.int32, device=weights.device)
-    hip.call('vm_kv_evict_paged_bf16', C.addressof(c), ptr(weights), weights.stride(0), _w_head(weights), weights.shape[2], ptr(kv_lens),
-             ptr(new_block_table), new_block_table.stride(0) if n_seq > 1 else new_block_table.shape[1], new_block_table.shape[1], budget, recent,
-             ptr(new_w), new_w.stride(0), _w_head(new_w), ptr(new_lens), ptr(kept), stream())
+    hip.call('vm_kv_evict_paged_bf16', hip.PAGED_KV.pack(*c), w, ws_, wh, w_cols, lens, new_block_table.data_ptr(),
+             row if n_seq > 1 else new_cols, new_cols, budget, recent, new_w.data_ptr(), hk * w_cols, w_cols, new_lens.data_ptr(), kept.data_ptr(), stream())
     return new_w, new_lens, kept
 
 

@@ -26,7 +26,7 @@ from torch.utils.checkpoint import checkpoint
 from ... import functional as Fh
 from ... import kernels as K
 from ...param import NoWeightDecayParameter
-from .kv_cache import KVCache
+from .kv_cache import KVCache, PagedKVCache
 from ..lora import ActivationBudget, Linear, gated_linear, linear_decode
 from .configuration_cogvlm import CogVLMConfig
 from .visual import EVA2CLIPModel
@@ -113,7 +113,7 @@ class Routing:
     B: int
     L: int
     n_pos: int                  # rope table length (upper bound, host)
-    kv: object = None           # KVCache being filled by this forward (generation path), else None
+    kv: object = None           # KVCache / PagedKVCache being filled by this forward (generation path), else None
     kv_lens: torch.Tensor | None = None     # decode step: cached tokens per sample including the new one
 
 
@@ -144,6 +144,12 @@ class VisionExpertAttention(nn.Module):
         else:
             qkv = gated_linear(x, self.vision_expert_query_key_value, self.language_expert_query_key_value, rt.counts)
         cos, sin = self.rotary_emb.tables(rt.n_pos, x.device)
+        if isinstance(rt.kv, PagedKVCache):     # prompt, follow-up chunk or single token: rotary + store, then attention over the cache
+            q = rt.kv.append(self.layer_idx, qkv, rt.row_pos, cos, sin, rt.n_rows)
+            ctx = rt.kv.attend(self.layer_idx, q, rt.cu_seqlens, rt.row_of_pos, rt.L, self.head_dim ** -0.5)
+            if decode:
+                return linear_decode(ctx, self.language_expert_dense, residual)
+            return gated_linear(ctx, self.vision_expert_dense, self.language_expert_dense, rt.counts, residual=residual)
         fuse_rope = rt.kv is None and rt.kv_lens is None      # training / plain forward: rotation inside the attention node
         if not fuse_rope:
             qkv = Fh.rope_(qkv, rt.row_pos, cos, sin, self.num_heads, self.head_dim, rt.n_rows)
@@ -230,8 +236,9 @@ class CogVLMModel(nn.Module):
                        B=B, L=L, n_pos=n_pos)
 
     def forward(self, input_ids, *, image=None, patch_size=None, pool_size=None, token_type_ids=None, attention_mask=None,
-                position_ids=None, output_hidden_states: bool = False, kv_cache: KVCache | None = None):
-        """kv_cache: an EMPTY cache to fill (prefill of the generation path, `use_cache=True` with no past)"""
+                position_ids=None, output_hidden_states: bool = False, kv_cache: KVCache | PagedKVCache | None = None):
+        """kv_cache: an EMPTY cache to fill (prefill of the generation path, `use_cache=True` with no past), or a PagedKVCache that already
+        holds a conversation: the tokens of this call follow it"""
         B, L = input_ids.shape
         dev = input_ids.device
         if token_type_ids is None:
@@ -243,6 +250,7 @@ class CogVLMModel(nn.Module):
         rt = self.build_routing(token_type_ids, attention_mask, position_ids)
         if kv_cache is not None:
             assert not torch.is_grad_enabled() or not self.training, 'the KV cache is an inference-only structure'
+            assert B == kv_cache.batch, f'batch size mismatch: {B} samples, a cache of {kv_cache.batch}'
             # packed rows are expert-sorted, not sequence-ordered: a row's cache slot is (its sample, its rank among the
             # sample's valid tokens)
             tok = rt.tok_of_row.clamp_min(0).long()
@@ -286,14 +294,19 @@ class CogVLMModel(nn.Module):
         return x, rt, (PackedHidden(hs, rt) if hs is not None else None)
 
     @torch.no_grad()
-    def decode_step(self, input_ids: torch.Tensor, position_ids: torch.Tensor, kv_cache: KVCache) -> torch.Tensor:
-        """one new token per sample against the cache: input_ids, position_ids [B] (device). A single-token call never
+    def decode_step(self, input_ids: torch.Tensor, position_ids: torch.Tensor, kv_cache: KVCache | PagedKVCache,
+                    live: torch.Tensor | None = None) -> torch.Tensor:
+        """one new token per sample against the cache: input_ids, position_ids [B] (device); live bool [B] (paged cache): the samples that
+        still go on, the others store nothing and their rows mean nothing. A single-token call never
         touches the vision expert (get_expert_mask with L == 1, reference :58-70) and skips the padding-masked norms
         (:306-309), so every row is a language row. No host synchronisation. -> final hidden [B, h]"""
         B = input_ids.shape[0]
         c = kv_cache
         assert B == c.batch
-        c.begin(c.rows, c.zeros, c.ones, 1)
+        if live is None:
+            c.begin(c.rows, c.zeros, c.ones, 1)
+        else:
+            c.begin(torch.where(live, c.rows, c.zeros - 1), c.zeros, live.to(torch.int32), 1)
         rt = Routing(counts=c.decode_counts, row_of_tok=c.rows, tok_of_row=c.rows, cu_seqlens=c.cu_rows, row_of_pos=c.rows,
                      expert_mask=None, row_pos=position_ids.to(torch.int32).contiguous(), n_rows=c.decode_counts[1:2],
                      B=B, L=1, n_pos=int(self.config.max_position_embeddings), kv=c, kv_lens=c.lens_after())
@@ -405,8 +418,15 @@ class CogVLMForCausalLM(nn.Module):
 
     default_max_new_tokens = 256
 
-    def new_kv_cache(self, batch: int, max_len: int, device) -> KVCache:
+    def new_kv_cache(self, batch: int, max_len: int, device, *, page_size: int | None = None, n_pages: int | None = None,
+                     track_weights: bool = False) -> KVCache | PagedKVCache:
+        """page_size: a PagedKVCache (follow-up chunks, eviction with track_weights) instead of one slab per sample"""
         cfg = self.config
+        if page_size is not None:
+            return PagedKVCache(cfg.num_hidden_layers, batch, max_len, cfg.num_attention_heads, cfg.hidden_size // cfg.num_attention_heads, device,
+                                page_size=page_size, n_pages=n_pages, track_weights=track_weights, dtype=self.lm_head.weight.dtype)
+        if n_pages is not None or track_weights:
+            raise ValueError('n_pages / track_weights belong to a paged cache: give page_size')
         return KVCache(cfg.num_hidden_layers, batch, max_len, cfg.hidden_size, device, dtype=self.lm_head.weight.dtype)
 
     def gradient_checkpointing_enable(self, kwargs: dict | None = None):
@@ -419,14 +439,14 @@ class CogVLMForCausalLM(nn.Module):
                 materialize_logits: bool | None = None) -> CausalLMOutputWithPast:
         if inputs_embeds is not None:
             raise NotImplementedError('inputs_embeds is not part of the reference\'s own call sites of this path')
-        if past_key_values is not None and len(past_key_values) > 0:
+        if past_key_values is not None and len(past_key_values) > 0 and not (isinstance(past_key_values, PagedKVCache) and input_ids.shape[1] > 1):
             # decode step of the generation path (reference :441-442, 253-262): the last column is the new token
             assert labels is None and input_ids.shape[1] >= 1
             x = self.model.decode_step(input_ids[:, -1], position_ids[:, -1], past_key_values)
             logits = linear_decode(x, self.lm_head).float()
             return CausalLMOutputWithPast(logits=logits[:, None], past_key_values=past_key_values, last_hidden_packed=x)
         cache = None
-        if use_cache:
+        if use_cache or past_key_values is not None and len(past_key_values) > 0:
             cache = past_key_values if past_key_values is not None else self.new_kv_cache(
                 input_ids.shape[0], input_ids.shape[1] + self.default_max_new_tokens, input_ids.device)
         x, rt, hs = self.model(input_ids, image=image, patch_size=patch_size, pool_size=pool_size, token_type_ids=token_type_ids,

@@ -21,6 +21,7 @@ from .. import functional as Fh
 from .. import kernels as K
 from ..utils import apply_prefix, get_lora_modules_default, get_lora_modules_finetune_all
 from .cogvlm.configuration_cogvlm import CogVLMConfig
+from .cogvlm.kv_cache import PagedKVCache
 from .cogvlm.modeling_cogvlm import CausalLMOutputWithPast, CogVLMForCausalLM
 from .lora import ActivationBudget, Linear, LoraTransposes, StepState, linear_decode
 from .loss import DiceFocalLoss
@@ -386,7 +387,9 @@ class MMMMForCausalLM(CogVLMForCausalLM):
     @torch.no_grad()
     def generate(self, input_ids, *, token_type_ids, position_ids, image, patch_size, pool_size, attention_mask=None,
                  max_new_tokens: int = 32, eos_token_id: int | None = None, forced_tokens: torch.Tensor | None = None,
-                 eos_check_every: int = 16, return_logits: bool = False, use_graph: bool = False) -> GenerateOutput:
+                 eos_check_every: int = 16, return_logits: bool = False, use_graph: bool = False,
+                 past_key_values: PagedKVCache | None = None, kv_page_size: int | None = None, kv_budget: int | None = None,
+                 kv_recent: int = 64) -> GenerateOutput:
         """Greedy decoding (`num_beams=1`, what scripts/demo.py and `evaluate`, mmmm.py:426-452, use): one prefill that fills
         the KV cache, then one token per sample and step. Unlike the reference (whose image scatter assumes column 1 and
         whose HF loop wants left padding, so images force batch size 1) a RIGHT-padded prompt batch is decoded together:
@@ -394,7 +397,19 @@ class MMMMForCausalLM(CogVLMForCausalLM):
         loop synchronises with the host only every `eos_check_every` steps to test for early termination.
         `forced_tokens` [B, steps] replaces the arg-max choice (teacher forcing for parity tests). `use_graph` captures one
         decode step (32 layers of ~25 launches + token choice) into a hipGraph and replays it: a step is launch-bound
-        otherwise (16.5 ms eager vs ~3 ms of HBM time at batch 1)."""
+        otherwise (16.5 ms eager vs ~3 ms of HBM time at batch 1).
+        `kv_page_size` keeps the cache in pages, for this call; a conversation gives a paged cache of its own as `past_key_values` to every turn
+        (`new_kv_cache(batch, max_len, device, page_size=...)`, empty at first): the `input_ids` of a turn follow what is cached (image None or a
+        further one). A sample's last new token — its eos, where it has ended — is not cached: the next
+        `input_ids` begin with it. `kv_budget` bounds the cached tokens per sample: after the prompt, and whenever one page more has gathered,
+        the tokens that have received the least attention leave (per layer and head; the `kv_recent` newest always stay)."""
+        if past_key_values is not None and not isinstance(past_key_values, PagedKVCache):
+            raise ValueError('only a paged cache can be continued: kv_page_size')
+        if kv_budget is not None:
+            if past_key_values is None and kv_page_size is None or past_key_values is not None and past_key_values.weights is None:
+                raise ValueError('kv_budget needs a paged cache that tracks the received weights (kv_page_size)')
+            if kv_budget <= 0 or not 0 <= kv_recent <= kv_budget:
+                raise ValueError(f'kv_budget {kv_budget}, kv_recent {kv_recent}: 0 <= recent <= budget, budget > 0')
         was_training = self.training
         self.eval()
         try:
@@ -403,7 +418,18 @@ class MMMMForCausalLM(CogVLMForCausalLM):
             if attention_mask is None:
                 attention_mask = torch.ones_like(input_ids)
             steps = max_new_tokens if forced_tokens is None else forced_tokens.shape[1]
-            cache = self.new_kv_cache(B, L + steps, dev)
+            if past_key_values is not None:
+                cache = past_key_values
+                cache.tighten()
+            elif kv_page_size is not None:
+                cache = self._new_paged_cache(B, L, steps, dev, kv_page_size, kv_budget)
+            else:
+                cache = self.new_kv_cache(B, L + steps, dev)
+            paged = isinstance(cache, PagedKVCache)
+
+            def trim():      # after the prompt, and when a page more than the budget has gathered
+                if kv_budget is not None and cache.len_bound >= kv_budget + cache.page_size:
+                    cache.evict(kv_budget, kv_recent)
             out = self(input_ids, image=image, patch_size=patch_size, pool_size=pool_size, token_type_ids=token_type_ids,
                        attention_mask=attention_mask, position_ids=position_ids, past_key_values=cache, use_cache=True,
                        materialize_logits=False)
@@ -412,8 +438,12 @@ class MMMMForCausalLM(CogVLMForCausalLM):
             n_valid = am.sum(1)
             last_col = (torch.arange(L, device=dev)[None] * am).argmax(1)
             rt = out.routing
-            last_row = rt.row_of_tok.long()[torch.arange(B, device=dev) * L + last_col]
-            logits = linear_decode(out.last_hidden_packed[last_row].contiguous(), self.lm_head).float()
+            if rt is None:                     # a single further token: the call was a decode step
+                logits = out.logits[:, 0]
+            else:
+                last_row = rt.row_of_tok.long()[torch.arange(B, device=dev) * L + last_col]
+                logits = linear_decode(out.last_hidden_packed[last_row].contiguous(), self.lm_head).float()
+            trim()
             prev_tok = input_ids[torch.arange(B, device=dev), last_col]
             pos = position_ids[torch.arange(B, device=dev), last_col]
             bop, eop = self.tokenizer.bop_token_id, self.tokenizer.eop_token_id
@@ -430,7 +460,7 @@ class MMMMForCausalLM(CogVLMForCausalLM):
 
             if use_graph and forced_tokens is None and not return_logits and steps > 2:
                 new_tokens, new_pos = self._generate_graphed(cache, head, logits, prev_tok, pos, done, steps, eos_token_id, bop, eop,
-                                                             eos_check_every)
+                                                             eos_check_every, trim)
                 return GenerateOutput(new_tokens=new_tokens, new_position_ids=new_pos, prompt_lengths=n_valid, past_key_values=cache)
             new_tokens, new_pos, all_logits = [], [], ([logits] if return_logits else None)
             for t in range(steps):
@@ -441,7 +471,9 @@ class MMMMForCausalLM(CogVLMForCausalLM):
                     break
                 if forced_tokens is None and eos_token_id is not None and (t + 1) % eos_check_every == 0 and bool(done.all()):
                     break
-                logits = linear_decode(self.model.decode_step(tok, pos, cache), self.lm_head).float()
+                live = ~done if paged and eos_token_id is not None else None
+                logits = linear_decode(self.model.decode_step(tok, pos, cache, live), self.lm_head).float()
+                trim()
                 if return_logits:
                     all_logits.append(logits)
                 prev_tok = tok
@@ -451,7 +483,15 @@ class MMMMForCausalLM(CogVLMForCausalLM):
             self.train(was_training)
 
 
-    def _generate_graphed(self, cache, head, logits, prev_tok, pos, done, steps, eos_token_id, bop, eop, eos_check_every):
+    def _new_paged_cache(self, B: int, L: int, steps: int, dev, page_size: int, budget: int | None) -> PagedKVCache:
+        """room for the prompt and the steps, or — with a budget — for the prompt and for the budget, a page more, and the copy eviction makes"""
+        if budget is None:
+            return self.new_kv_cache(B, L + steps, dev, page_size=page_size)
+        up = lambda n: -(-n // page_size)      # noqa: E731
+        most = max(L, min(L + steps, budget + page_size + 1))
+        return self.new_kv_cache(B, most, dev, page_size=page_size, n_pages=B * (up(most) + up(budget)), track_weights=True)
+
+    def _generate_graphed(self, cache, head, logits, prev_tok, pos, done, steps, eos_token_id, bop, eop, eos_check_every, trim):
         """greedy loop with the decode step captured in a hipGraph. State lives in static device buffers that the graph
         updates in place: (tok, pos, done) of the newest token, a step counter, and the [B, steps] outputs it scatters into.
         One eager step first: it sets the lazily-initialised kernel attributes and warms the allocator outside the capture."""
@@ -467,20 +507,29 @@ class MMMMForCausalLM(CogVLMForCausalLM):
                 done = done | (tok == eos_token_id)
             return tok, pos + 1 - ((prev_tok == bop) | (tok == eop)).long(), done
 
+        paged = isinstance(cache, PagedKVCache)
+
+        def decode(tok, pos, done):
+            live = ~done if paged and eos_token_id is not None else None
+            return linear_decode(self.model.decode_step(tok, pos, cache, live), self.lm_head).float()
+
         tok, pos, done = choose(logits, prev_tok, pos, done)
         out_tok[:, 0], out_pos[:, 0] = tok, pos
-        logits = linear_decode(self.model.decode_step(tok, pos, cache), self.lm_head).float()          # eager step 1
+        logits = decode(tok, pos, done)                  # eager step 1
         s_prev, s_pos, s_done = tok.clone(), pos.clone(), done.clone()
         s_logits = logits.clone()
         s_col = torch.ones(B, 1, dtype=torch.long, device=dev)
         cache.launch_bound = cache.max_len
+        if paged:                                 # no page may be handed out inside the captured step
+            trim()
+            cache.reserve(min(cache.max_len, cache.len_bound + 1))
 
         def step():
             tok, pos, done = choose(s_logits, s_prev, s_pos, s_done)
             out_tok.scatter_(1, s_col, tok[:, None])
             out_pos.scatter_(1, s_col, pos[:, None])
             s_col.add_(1)
-            s_logits.copy_(linear_decode(self.model.decode_step(tok, pos, cache), self.lm_head).float())
+            s_logits.copy_(decode(tok, pos, done))
             s_prev.copy_(tok); s_pos.copy_(pos); s_done.copy_(done)
 
         torch.cuda.synchronize()
@@ -491,6 +540,9 @@ class MMMMForCausalLM(CogVLMForCausalLM):
         cache.len_bound = bound0                  # the capture ran the host bookkeeping once without executing anything
         t = 1
         while t < steps - 1:
+            if paged:
+                trim()
+                cache.reserve(cache.len_bound + 1)
             graph.replay()
             cache.len_bound += 1
             t += 1

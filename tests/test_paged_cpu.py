@@ -104,6 +104,10 @@ def test_evict_refused(lib):
 def test_struct_layouts(lib):
     assert C.sizeof(hip.PagedKVArgs) == 64 and hip.PagedKVArgs.block_table.offset == 32 and hip.PagedKVArgs.head_dim.offset == 60
     assert C.sizeof(hip.AttnPagedArgs) == 224 and hip.AttnPagedArgs.n_rows.offset == 136 and hip.AttnPagedArgs.weights.offset == 160
+    assert hip.PAGED_KV.size == 64 and hip.ATTN_PAGED.size == 224
+    a = attn(weights=3, weights_out=4, w_cols=5, ldw_seq=6, workspace=7, workspace_bytes=8, row_of_pos=9)
+    flat = [getattr(a.cache, n) for n, _ in hip.PagedKVArgs._fields_] + [getattr(a, n) for n, _ in hip.AttnPagedArgs._fields_[1:]]
+    assert hip.ATTN_PAGED.pack(*[0 if v is None else v for v in flat]) == bytes(a)
 
 
 def test_wrappers_refuse_what_they_can_see():

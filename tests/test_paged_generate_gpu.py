@@ -1,0 +1,135 @@
+"""The generation path over a paged cache: the same tokens and logits as over the contiguous one, conversations that go on, finished samples,
+captured steps, eviction by received weight. bf16 bounds as in test_generate_gpu.py (two bf16 evaluations of the same logits)."""
+import pytest
+import torch
+
+from tests._gpu_common import rel
+from tests.test_generate_gpu import _forced, _sample
+from tests.test_model_gpu import lm, make_inputs  # noqa: F401  (module fixture)
+
+pytestmark = pytest.mark.gpu
+
+
+def _batch(batch):
+    vi = batch['vlm_inputs']
+    return vi['input_ids'], dict(token_type_ids=vi['token_type_ids'], position_ids=vi['position_ids'], attention_mask=vi['attention_mask'],
+                                 image=batch['image'], patch_size=batch['patch_size'], pool_size=batch['pool_size'])
+
+
+@pytest.mark.parametrize('page', [16, 64])
+def test_paged_equals_contiguous(dev, lm, page):
+    batch, tok = make_inputs(dev)
+    lm.tokenizer = tok
+    ids, kw = _batch(batch)
+    forced = _forced(tok, 6, 3, 5).to(dev)
+    a = lm.generate(ids, **kw, forced_tokens=forced, return_logits=True)
+    b = lm.generate(ids, **kw, forced_tokens=forced, return_logits=True, kv_page_size=page)
+    assert torch.equal(a.new_position_ids, b.new_position_ids) and torch.equal(a.past_key_values.lens, b.past_key_values.lens)
+    for t in range(6):
+        assert rel(b.logits[t], a.logits[t]) < 1e-2, t
+    # what is cached is the same rows, in other places
+    ca, cb = a.past_key_values, b.past_key_values
+    H, hd = cb.n_heads, cb.head_dim
+    for s in range(3):
+        n = int(ca.lens[s])
+        j = torch.arange(n, device=dev)
+        rows = cb.k[0][cb.block_table[s].long()[j // page], :, j % page]
+        assert rel(rows.reshape(n, H * hd).float(), ca.k[0, s, :n].float()) < 1e-2
+
+
+def test_conversation_goes_on(dev, lm):
+    """second turn: a chunk of further tokens over the filled cache gives the logits of one full forward over everything"""
+    batch, tok = make_inputs(dev)
+    lm.tokenizer = tok
+    kw, img = _sample(batch, 2)
+    n = kw['input_ids'].shape[1]
+    f1, f2 = _forced(tok, 4, 1, 3).to(dev), _forced(tok, 5, 1, 4).to(dev)
+    g = torch.Generator().manual_seed(9)
+    question = torch.randint(3, 150, (1, 7), generator=g).to(dev)
+    cache = lm.new_kv_cache(1, n + 40, dev, page_size=16)                 # room for both turns
+    one = lm.generate(**kw, **img, forced_tokens=f1, return_logits=True, past_key_values=cache)
+    assert one.past_key_values is cache
+    chunk = torch.cat([f1[:, -1:], question], 1)
+    last = one.new_position_ids[:, -1:]
+    pos = torch.cat([last, last + 1 + torch.arange(7, device=dev)], 1)
+    two = lm.generate(chunk, token_type_ids=torch.zeros_like(chunk), position_ids=pos, image=None, patch_size=None, pool_size=None,
+                      forced_tokens=f2, return_logits=True, past_key_values=cache)
+    ids = torch.cat([kw['input_ids'], f1, question, f2[:, :-1]], 1)
+    tt = torch.cat([kw['token_type_ids'], torch.zeros(1, ids.shape[1] - n, dtype=torch.long, device=dev)], 1)
+    allpos = torch.cat([kw['position_ids'], one.new_position_ids, pos[:, 1:], two.new_position_ids[:, :-1]], 1)
+    lm.eval()
+    with torch.no_grad():
+        full = lm(ids, token_type_ids=tt, position_ids=allpos, **img)
+    at = n + f1.shape[1] + 7 - 1
+    for t in range(5):
+        assert rel(two.logits[t][0], full.logits[0, at + t]) < 2e-2, t
+    assert two.past_key_values.lens.tolist() == [ids.shape[1]]
+
+
+def test_single_token_turn(dev, lm):
+    batch, tok = make_inputs(dev)
+    lm.tokenizer = tok
+    kw, img = _sample(batch, 0)
+    f = _forced(tok, 6, 1, 7).to(dev)
+    whole = lm.generate(**kw, **img, forced_tokens=f, return_logits=True, kv_page_size=16)
+    cache = lm.new_kv_cache(1, kw['input_ids'].shape[1] + 10, dev, page_size=16)
+    first = lm.generate(**kw, **img, forced_tokens=f[:, :3], return_logits=True, past_key_values=cache)
+    rest = lm.generate(f[:, 2:3], token_type_ids=torch.zeros_like(f[:, :1]), position_ids=first.new_position_ids[:, -1:], image=None, patch_size=None,
+                       pool_size=None, forced_tokens=f[:, 3:], return_logits=True, past_key_values=cache)
+    for t in range(3):
+        assert rel(rest.logits[t], whole.logits[3 + t]) < 1e-2
+    assert torch.equal(rest.past_key_values.lens, whole.past_key_values.lens)
+
+
+def test_graph_replayed_paged_decode_equals_eager(dev, lm):
+    batch, tok = make_inputs(dev)
+    lm.tokenizer = tok
+    ids, kw = _batch(batch)
+    for extra in ({}, dict(kv_budget=24, kv_recent=8)):
+        eager = lm.generate(ids, **kw, max_new_tokens=40, kv_page_size=16, **extra)
+        graphed = lm.generate(ids, **kw, max_new_tokens=40, kv_page_size=16, use_graph=True, **extra)
+        assert torch.equal(eager.new_tokens, graphed.new_tokens) and torch.equal(eager.new_position_ids, graphed.new_position_ids)
+        assert graphed.past_key_values.lens.tolist() == eager.past_key_values.lens.tolist()
+
+
+def test_finished_samples_store_nothing(dev, lm):
+    batch, tok = make_inputs(dev)
+    lm.tokenizer = tok
+    ids, kw = _batch(batch)
+    free = lm.generate(ids, **kw, max_new_tokens=12, kv_page_size=16)
+    eos = int(free.new_tokens[0, 3])
+    n = kw['attention_mask'].sum(1).tolist()
+    for graph in (False, True):
+        out = lm.generate(ids, **kw, max_new_tokens=12, kv_page_size=16, eos_token_id=eos, eos_check_every=100, use_graph=graph)
+        for s in range(3):
+            toks = out.new_tokens[s].tolist()
+            fed = toks.index(eos) if eos in toks[:-1] else len(toks) - 1        # the eos itself, and what follows it, is not cached
+            assert int(out.past_key_values.lens[s]) == n[s] + fed, (graph, s)
+
+
+def test_budget(dev, lm):
+    batch, tok = make_inputs(dev)
+    lm.tokenizer = tok
+    ids, kw = _batch(batch)
+    longest = int(kw['attention_mask'].sum(1).max())
+    forced = _forced(tok, 40, 3, 6).to(dev)
+    want = lm.generate(ids, **kw, forced_tokens=forced, return_logits=True, kv_page_size=16)
+    wide = lm.generate(ids, **kw, forced_tokens=forced, return_logits=True, kv_page_size=16, kv_budget=longest + 100, kv_recent=8)
+    assert all(torch.equal(a, b) for a, b in zip(want.logits, wide.logits))             # nothing left: the same bits
+    w = wide.past_key_values.weights
+    total = w.sum((1, 2, 3)) if w.dim() == 4 else None
+    fed = wide.past_key_values.lens.sum().item() * wide.past_key_values.n_heads          # every query gives one in all per head
+    assert torch.allclose(total.cpu(), torch.full_like(total.cpu(), fed), rtol=1e-4)
+    cut = lm.generate(ids, **kw, forced_tokens=forced, return_logits=True, kv_page_size=16, kv_budget=24, kv_recent=8)
+    c = cut.past_key_values
+    assert int(c.lens.max()) < 24 + 16 and c.max_len < want.past_key_values.max_len + 16
+    assert all(torch.isfinite(x).all() for x in cut.logits)
+    assert torch.equal(cut.logits[0], want.logits[0])                                    # the prompt itself saw everything
+    with pytest.raises(ValueError):
+        lm.generate(ids, **kw, max_new_tokens=4, kv_budget=24)
+    with pytest.raises(ValueError):
+        lm.generate(ids, **kw, max_new_tokens=4, kv_page_size=16, kv_budget=24, kv_recent=25)
+    with pytest.raises(ValueError):
+        lm.generate(ids, **kw, max_new_tokens=4, past_key_values=lm.new_kv_cache(3, 200, dev))
+    with pytest.raises(ValueError):
+        lm.generate(ids, **kw, max_new_tokens=4, past_key_values=want.past_key_values, kv_budget=24)
