@@ -78,6 +78,19 @@ __device__ __forceinline__ float sum_over_g(float x) {
   swap32(a, b);
   return a + b;
 }
+// Values that are not finite, in a tile that only some rows see: the matrix product would carry them into the rows that do not (0 x inf, 0 x NaN).
+// Such a tile is multiplied with them as zeros, and the rows that see them get their share one key at a time.
+__device__ __forceinline__ bool none_finite2(unsigned m) { return (m >> 16) >= 0x7F80u || (m & 0xFFFFu) >= 0x7F80u; }
+__device__ __forceinline__ unsigned max2(unsigned m, unsigned x) {          // two 16-bit magnitudes at a time
+  typedef unsigned short u16x2_t __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(unsigned, __builtin_elementwise_max(__builtin_bit_cast(u16x2_t, m), __builtin_bit_cast(u16x2_t, x & 0x7FFF7FFFu)));
+}
+__device__ __forceinline__ unsigned finite2(unsigned x) {
+  if ((x & 0x7F80u) == 0x7F80u) x &= 0xFFFF0000u;
+  if ((x & 0x7F800000u) == 0x7F800000u) x &= 0x0000FFFFu;
+  return x;
+}
+
 __device__ __forceinline__ float fast_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
 
 template <int HD>
@@ -179,12 +192,19 @@ __global__ __launch_bounds__(SP_WAVES * 64, 2) void attn_paged_split_k(const Att
 #pragma unroll
       for (int e = 0; e < 4; ++e) sa[jj][e] *= sc;
     }
+    bool strange = false;
     if (j0 + 31 > lim_min || pg.a < 0 || pg.b < 0) {
 #pragma unroll
       for (int jj = 0; jj < 2; ++jj)
 #pragma unroll
         for (int e = 0; e < 4; ++e)
           if ((jj ? pg.b : pg.a) < 0 || j0 + 16 * jj + 4 * g + e > lim) sa[jj][e] = -INFINITY;
+      unsigned most = 0;
+#pragma unroll
+      for (int t = 0; t < B::NV; ++t)
+#pragma unroll
+        for (int w = 0; w < 4; ++w) most = max2(most, __builtin_bit_cast(u32x4_t, cur.v[t])[w]);
+      strange = __builtin_amdgcn_ballot_w64(none_finite2(most)) != 0;
     }
     if (srow && live) {
 #pragma unroll
@@ -193,8 +213,14 @@ __global__ __launch_bounds__(SP_WAVES * 64, 2) void attn_paged_split_k(const Att
     }
     // V -> LDS while the scores settle
 #pragma unroll
-    for (int t = 0; t < B::NV; ++t)
-      *reinterpret_cast<i32x4_t*>(tv + tile_off16(t * B::RPI + lane / B::CPR, lane & (B::CPR - 1))) = cur.v[t];
+    for (int t = 0; t < B::NV; ++t) {
+      u32x4_t v = __builtin_bit_cast(u32x4_t, cur.v[t]);
+      if (__builtin_expect(strange, 0)) {
+#pragma unroll
+        for (int w = 0; w < 4; ++w) v[w] = finite2(v[w]);
+      }
+      *reinterpret_cast<u32x4_t*>(tv + tile_off16(t * B::RPI + lane / B::CPR, lane & (B::CPR - 1))) = v;
+    }
     float mx = fmaxf(fmaxf(fmaxf(sa[0][0], sa[0][1]), fmaxf(sa[0][2], sa[0][3])), fmaxf(fmaxf(sa[1][0], sa[1][1]), fmaxf(sa[1][2], sa[1][3])));
     mx = max_over_g(mx);
     if (__builtin_amdgcn_ballot_w64(mx > m) != 0) {
@@ -223,6 +249,28 @@ __global__ __launch_bounds__(SP_WAVES * 64, 2) void attn_paged_split_k(const Att
       const bf16x8_t vf = frag16_tr(tv, 0, t, lane);
       o[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, ph, o[t], 0, 0, 0);
       o[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pl, o[t], 0, 0, 0);
+    }
+    if (__builtin_expect(strange, 0)) {
+#pragma unroll
+      for (int t = 0; t < B::NV; ++t)
+        *reinterpret_cast<i32x4_t*>(tv + tile_off16(t * B::RPI + lane / B::CPR, lane & (B::CPR - 1))) = cur.v[t];
+#pragma unroll
+      for (int jj = 0; jj < 2; ++jj)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float x = fast_exp2(sa[jj][e] - base);
+          for (int gg = 0; gg < 4; ++gg) {                          // key 16 jj + 4 gg + e of the block: its weight for this lane's row
+            const float w = __shfl(x, ln + 16 * gg, 64);
+            const bool sees = __shfl(sa[jj][e], ln + 16 * gg, 64) != -INFINITY;
+#pragma unroll
+            for (int t = 0; t < ND; ++t) {
+              const u16x4_t v = *reinterpret_cast<const u16x4_t*>(tv + tile_off16(16 * jj + 4 * gg + e, 2 * t + (g >> 1)) + 8 * (g & 1));
+#pragma unroll
+              for (int c = 0; c < 4; ++c)
+                if (sees && (v[c] & 0x7F80) == 0x7F80) o[t][c] = fmaf(w, bf2f(v[c]), o[t][c]);
+            }
+          }
+        }
     }
     cur = nxt;
     pg = pg1;

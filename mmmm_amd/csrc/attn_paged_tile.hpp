@@ -208,6 +208,7 @@ __global__ __launch_bounds__(NW * 64, 2) void tile_k(const AttnPagedP p) {
 #pragma unroll
     for (int e = 0; e < 16; ++e) o[b2][e] = 0.f;
   const float sc = p.scale * LOG2E;
+  int strange = 0x7FFFFFFF;                                        // first tile in which a value that is not finite was taken as zero
   float msc = -INFINITY, base = 0.f, l_run = 0.f;                  // running maximum (log2 domain), what is subtracted, this half's sum
 
   if (nt > 0) {
@@ -283,6 +284,21 @@ __global__ __launch_bounds__(NW * 64, 2) void tile_k(const AttnPagedP p) {
 #pragma unroll
             for (int e = 0; e < 16; ++e)                           // accumulator rows 8 (e >> 2) ..: 16 keys of one page each half
               S[kt][e] = page_ok(pga.all[2 * kt + (e >> 3)], p.c.n_pages) && kv0 + 32 * kt + acc_row(e, hf) <= lim ? S[kt][e] : -INFINITY;
+          unsigned most = 0;
+#pragma unroll
+          for (int i = 0; i < 4 * ND; ++i)
+#pragma unroll
+            for (int w = 0; w < 4; ++w) most = max2(most, __builtin_bit_cast(u32x4_t, kv[i])[w]);
+          if (__builtin_expect(__builtin_amdgcn_ballot_w64(none_finite2(most)) != 0, 0)) {
+            strange = min(strange, t);
+#pragma unroll
+            for (int i = 0; i < 4 * ND; ++i) {
+              u32x4_t x = __builtin_bit_cast(u32x4_t, kv[i]);
+#pragma unroll
+              for (int w = 0; w < 4; ++w) x[w] = finite2(x[w]);
+              kv[i] = __builtin_bit_cast(bf16x8_t, x);
+            }
+          }
         }
         float ma = max32(S), mb = ma;
         a32::swap_halves(ma, mb);
@@ -331,6 +347,41 @@ __global__ __launch_bounds__(NW * 64, 2) void tile_k(const AttnPagedP p) {
   }
 
   if (!wave_live) return;
+  if (__builtin_expect(strange < t_w, 0)) {
+    const table_ptr table = table_of(p.c, b);
+    for (int j = 64 * strange; j < min(64 * t_w, kv_end); ++j) {
+      const int page = table[__builtin_amdgcn_readfirstlane(j >> p.c.shift)];
+      if (!page_ok(page, p.c.n_pages)) continue;
+      const int64_t at = page_row(page, p.c.ld_page, hk, j & p.c.mask, p.c.shift, HD);
+      bool odd = false;
+#pragma unroll 1
+      for (int c = 0; c < HD / 8; ++c) {
+        const u16x4_t v = *reinterpret_cast<const u16x4_t*>(p.c.v + at + 8 * c + 4 * hf);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) odd |= (v[e] & 0x7F80) == 0x7F80;
+      }
+      if (__builtin_amdgcn_ballot_w64(odd) == 0) continue;
+      float dot = 0.f;
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) {
+        const u16x8_t kr = *reinterpret_cast<const u16x8_t*>(p.c.k + at + 16 * ks + 8 * hf), qr = __builtin_bit_cast(u16x8_t, qf[ks]);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) dot = fmaf(bf2f(kr[e]), bf2f(qr[e]), dot);
+      }
+      float da = dot, db = dot;
+      a32::swap_halves(da, db);
+      const float w = fast_exp2(fmaf(da + db, sc, -base));
+#pragma unroll
+      for (int b2 = 0; b2 < ND; ++b2)
+#pragma unroll
+        for (int g4 = 0; g4 < 4; ++g4) {
+          const u16x4_t v = *reinterpret_cast<const u16x4_t*>(p.c.v + at + 32 * b2 + 8 * g4 + 4 * hf);
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (j <= lim && (v[e] & 0x7F80) == 0x7F80) o[b2][4 * g4 + e] = fmaf(w, bf2f(v[e]), o[b2][4 * g4 + e]);
+        }
+    }
+  }
   {
     float a = l_run, c = l_run;
     a32::swap_halves(a, c);

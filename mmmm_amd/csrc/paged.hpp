@@ -7,6 +7,8 @@
 #pragma once
 #include "vm_common.hpp"
 
+typedef __attribute__((ext_vector_type(4))) unsigned u32x4_t;
+
 struct PagedKV {
   const unsigned short* k;
   const unsigned short* v;

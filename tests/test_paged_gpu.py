@@ -265,3 +265,168 @@ def test_append_attend_evict_together(dev, K):
         close(lse, want[2], want[3])
         close(wd, want[4], want[5])
         w = wd.cpu()
+
+
+@pytest.mark.parametrize('new,L', [(4, 40), (13, 13), (37, 100), (200, 330), (300, 300)])
+@pytest.mark.parametrize('hd', [32, 128])
+def test_what_a_query_does_not_see_does_not_reach_it(dev, K, new, L, hd):
+    """inf and NaN in keys and values of LATER tokens of the chunk: earlier queries do not notice, later ones get what arithmetic gives"""
+    g = torch.Generator().manual_seed(new)
+    H, hk, page = 4, 2, 16
+    k, v, table = R.make_cache([L], hk, hd, page, g)
+    q = torch.randn(new, H * hd, generator=g).bfloat16()
+    bad = [L - 1, L - new // 3 - 1, L - new // 2 - 1]
+    for n, (j, x) in enumerate(zip(bad, (NAN, float('inf'), -float('inf')))):
+        v[int(table[0, j // page]), n % hk, j % page, 3 * n:3 * n + 5] = x
+    kb = L - 1
+    k[int(table[0, kb // page]), 1, kb % page, 7] = NAN                      # the newest key too: only the last query sees it
+    w = torch.zeros(1, hk, L)
+    clean_k, clean_v = k.nan_to_num(0.0, 0.0, 0.0), v.nan_to_num(0.0, 0.0, 0.0)
+    scale = hd ** -0.5
+    want = R.attention(q, clean_k, clean_v, table, [new], [L], scale, None, w)
+    dt = table.to(dev)
+    out, lse = K.attn_paged(q.to(dev), k.to(dev), v.to(dev), dt, i32([0, new], dev), i32([L], dev), scale, new, L)
+    got = out.cpu().double().view(new, H, hd)
+    ref, tol = want[0].view(new, H, hd), want[1].view(new, H, hd)
+    touched = torch.zeros(new, H, hd, dtype=torch.bool)
+    kind = torch.zeros(new, H, hd)
+    for n, j in enumerate(bad):
+        i0 = j - (L - new)                                                   # the first query that sees token j
+        heads = slice(2 * (n % hk), 2 * (n % hk) + 2)
+        touched[i0:, heads, 3 * n:3 * n + 5] = True
+        kind[i0:, heads, 3 * n:3 * n + 5] += n
+    touched[new - 1, 2:] = True                                              # NaN score: the whole row
+    assert ((got - ref).abs() <= tol)[~touched].all()
+    assert (~got.isfinite())[touched].all()
+    for n, sign in ((1, 1), (2, -1)):
+        i0, heads = bad[n] - (L - new), slice(2 * (n % hk), 2 * (n % hk) + 2)
+        part = got[i0:new - 1, heads, 3 * n + 3:3 * n + 5] if n == 1 else got[i0:new - 1, heads, 8:11]
+        assert (part == sign * float('inf')).all(), n
+
+
+def _case(K, dev, new, L, seed, H=4, hk=2, hd=128, page=64, weights=False):
+    g = torch.Generator().manual_seed(seed)
+    k, v, table = R.make_cache([L, max(1, L // 2)], hk, hd, page, g)
+    n2 = min(new, max(1, L // 2))
+    q = torch.randn(new + n2, H * hd, generator=g).bfloat16().to(dev)
+    args = [q, k.to(dev), v.to(dev), table.to(dev), i32([0, new, new + n2], dev), i32([L, max(1, L // 2)], dev), hd ** -0.5, new, L]
+    kw = dict(weights=torch.rand(2, hk, L, generator=g).to(dev)) if weights else {}
+    if weights:
+        kw['weights_out'] = torch.zeros_like(kw['weights'])
+    return args, kw
+
+
+def test_two_captured_graphs_and_eager_calls_between(dev, K):
+    """each graph has its own workspace: replays of one do not disturb the other, whatever runs between"""
+    cases = [_case(K, dev, 1, 3000, 1, weights=True), _case(K, dev, 50, 2500, 2, weights=True)]
+    want = []
+    for a, kw in cases:
+        o, lse = K.attn_paged(*a, **kw)
+        want.append((o.clone(), lse.clone(), kw['weights_out'].clone()))
+    torch.cuda.synchronize()
+    graphs = []
+    for a, kw in cases:
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr):
+            o, lse = K.attn_paged(*a, **kw)
+        graphs.append((gr, o, lse, kw['weights_out']))
+    for rep in range(4):
+        for (gr, o, lse, wo), w in zip(graphs if rep % 2 else graphs[::-1], want if rep % 2 else want[::-1]):
+            wo.zero_()
+            gr.replay()
+            K.attn_paged(*cases[rep % 2][0])
+            torch.randn(1 << 16, device=dev).sum()
+            torch.cuda.synchronize()
+            assert torch.equal(o, w[0]) and torch.equal(lse, w[1]) and torch.equal(wo, w[2])
+
+
+def test_on_another_stream(dev, K):
+    args, kw = _case(K, dev, 40, 2000, 3, weights=True)
+    o, lse = K.attn_paged(*args, **kw)
+    w = kw['weights_out'].clone()
+    st = torch.cuda.Stream()
+    st.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(st):
+        kw['weights_out'].zero_()
+        o2, lse2 = K.attn_paged(*args, **kw)
+        x = o2 + 0
+    torch.cuda.current_stream().wait_stream(st)
+    assert torch.equal(x, o) and torch.equal(lse2, lse) and torch.equal(kw['weights_out'], w)
+
+
+def test_pools_beyond_32_bit_offsets(dev, K):
+    """pages behind 2^31 elements (4 GiB) of a pool: stored, attended to in both forms, moved"""
+    g = torch.Generator().manual_seed(4)
+    H, hk, hd, page = 16, 8, 128, 1024
+    pages = 2 * (1 << 31) // (hk * page * hd) // 2 + 12                       # 2060 pages of 2^20 elements
+    assert (pages - 8) * hk * page * hd > 1 << 31
+    k = torch.empty(pages, hk, page, hd, dtype=torch.bfloat16, device=dev)
+    v = torch.empty_like(k)
+    table = torch.tensor([[pages - 1, 3, pages - 4]], dtype=torch.int32)
+    L = 2 * page + 300
+    qkv = torch.randn(L, (H + 2 * hk) * hd, generator=g).bfloat16()
+    ang = torch.rand(16, hd, generator=g)
+    cos, sin = ang.cos(), ang.sin()
+    pos = torch.randint(0, 16, (L,), generator=g).to(torch.int32)
+    seq, idx = torch.zeros(L, dtype=torch.int32), torch.arange(L, dtype=torch.int32)
+    q = K.kv_append_paged(qkv.to(dev), seq.to(dev), idx.to(dev), table.to(dev), k, v, pos.to(dev), cos.to(dev), sin.to(dev), H)
+    few = [pages - 1, 3, pages - 4]
+    ks, vs, small = k[few].cpu(), v[few].cpu(), torch.tensor([[0, 1, 2]], dtype=torch.int32)
+    z = torch.zeros(3, hk, page, hd, dtype=torch.bfloat16)
+    qw, qt, kw, kt, vw = R.append(qkv, seq, idx, small, z, z, pos, cos, sin, H)
+    close(q, qw, qt)
+    for h in range(hk):
+        close(R.tokens(ks, small, 0, L, h)[0], R.tokens(kw, small, 0, L, h)[0], R.tokens(kt, small, 0, L, h)[0])
+        assert torch.equal(R.tokens(vs, small, 0, L, h)[0], R.tokens(vw, small, 0, L, h)[0])
+    for n in (1, 64):
+        qn = q[-n:].contiguous()
+        want = R.attention(qn.cpu(), ks, vs, small, [n], [L], hd ** -0.5)
+        o, lse = K.attn_paged(qn, k, v, table.to(dev), i32([0, n], dev), i32([L], dev), hd ** -0.5, n, L)
+        close(o, want[0], want[1])
+        close(lse, want[2], want[3])
+    w = torch.rand(1, hk, L, generator=g)
+    new = torch.tensor([[pages - 7]], dtype=torch.int32)
+    kept, lens = R.evict(w, table, pages, page, [L], 900, 10)
+    _, _, got = K.kv_evict_paged(k, v, w.to(dev), table.to(dev), i32([L], dev), new.to(dev), 900, 10)
+    for h in range(hk):
+        assert got[0, h].cpu().tolist() == kept[0][h]
+        i = torch.tensor(kept[0][h])
+        assert torch.equal(k[pages - 7, h, :900].cpu(), ks[(i // page), h, i % page])
+        assert torch.equal(v[pages - 7, h, :900].cpu(), vs[(i // page), h, i % page])
+
+
+def test_strides_of_the_pools_and_tables(dev, K):
+    """K and V of a layer interleaved in one allocation, tables and weights that are views"""
+    g = torch.Generator().manual_seed(8)
+    lens, hk, hd, page, H = [70, 130], 2, 64, 32, 4
+    k, v, table = R.make_cache(lens, hk, hd, page, g)
+    both = torch.stack([k, v], 1).to(dev)                                    # [pages, 2, ...]: page stride of two pages
+    wide = torch.full((2, 11), -9, dtype=torch.int32)
+    wide[:, 2:2 + table.shape[1]] = table
+    w = torch.rand(2, hk, 200, generator=g)
+    ww = torch.zeros(2, hk + 1, 260)
+    ww[:, 1:, 30:230] = w
+    q = torch.randn(9, H * hd, generator=g).bfloat16()
+    want = R.attention(q, k, v, table, [4, 5], lens, 0.2, None, w)
+    wd = ww.to(dev)
+    o, lse = K.attn_paged(q.to(dev), both[:, 0], both[:, 1], wide.to(dev)[:, 2:2 + table.shape[1]], i32([0, 4, 9], dev), i32(lens, dev), 0.2, 5, 130,
+                          weights=wd[:, 1:, 30:230])
+    close(o, want[0], want[1])
+    for b in range(2):
+        close(wd[b, 1:, 30:30 + lens[b]], want[4][b, :, :lens[b]], want[5][b, :, :lens[b]])
+    rest = wd.cpu().clone()
+    rest[:, 1:, 30:230] = 0
+    assert (rest == 0).all()
+
+
+def test_bounds_that_are_too_small_stay_inside(dev, K):
+    """max_q below a sample's new tokens: the first of them are computed, nothing is written elsewhere"""
+    g = torch.Generator().manual_seed(6)
+    for new, bound in ((30, 5), (300, 100)):
+        k, v, table = R.make_cache([400], 2, 64, 16, g)
+        q = torch.randn(new, 4 * 64, generator=g).bfloat16()
+        want = R.attention(q, k, v, table, [new], [400], 0.1)
+        out = torch.full((new, 256), 3.0, dtype=torch.bfloat16, device=dev)
+        K.attn_paged(q.to(dev), k.to(dev), v.to(dev), table.to(dev), i32([0, new], dev), i32([400], dev), 0.1, bound, 400, out=out)
+        close(out[:bound], want[0][:bound], want[1][:bound])
+        assert ((out[bound:] == 3.0).all(1) | ((out[bound:].cpu().double() - want[0][bound:]).abs() <= want[1][bound:]).all(1).to(dev)).all()
