@@ -536,9 +536,10 @@ int vm_kv_append_paged_bf16(const vm_paged_kv* cache_host, const void* qkv, int6
 /* Attention of a chunk of new tokens over the paged cache that already holds them (modeling_cogvlm.py:113-141 for one token, a prompt, or
  * anything between). Positions cu_q[b] .. cu_q[b + 1] - 1 are the n_b new tokens of sample b, the last n_b of its kv_lens[b] cached ones:
  * the i-th sees the tokens j <= kv_lens[b] - n_b + i. Query head h reads kv head h / (n_heads / n_kv_heads). Scores and softmax in fp32 (no
- * rounding of the scores), probabilities rounded to bf16 for the P V product. A query that sees nothing gets zeros and lse = -inf.
- * row_of_pos (may be NULL: identity) is the packed row of a position in q and out; lse[h * ld_lse + position]. Rows of no position are left
- * as they were. max_q / max_kv: host upper bounds of n_b and of kv_lens (no device -> host sync).
+ * rounding of the scores), probabilities as bf16 for the P V product (as two bf16 terms where a kv head has up to 16 query rows). A query
+ * that sees nothing gets zeros and lse = -inf. row_of_pos (may be NULL: identity) is the packed row of a position in q and out; outside
+ * [0, n_rows) there is no such query (lse = -inf). lse[h * ld_lse + position]. Rows of no position are left as they were. max_q / max_kv:
+ * host upper bounds of n_b and of kv_lens (no device -> host sync); a bound that is too small leaves queries, or weights of tokens, out.
  * weights_out (may be NULL): weights_out[b][kv head][j] = weights[b][kv head][j] + the sum of the probabilities that token j gets from this
  * call's queries of the heads of that kv head, for j < kv_lens[b]; fp32, fixed order of summation; weights may be the same buffer. */
 typedef struct vm_attn_paged_args {
@@ -568,7 +569,7 @@ int vm_attn_paged_bf16(const vm_attn_paged_args* args_host, void* stream);
 
 /* Eviction: of every sample and kv head the `budget` tokens stay that are among the `recent` newest or have the largest weight (ties: the
  * older one; NaN counts as least; tokens of absent pages never stay). They keep their order and go to the pages of new_table, which nothing
- * else may use; the old pages are not changed. new_lens[b] = how many stayed, new_weights their weights with zeros behind,
+ * else may use and which hold them all; the old pages are not changed. new_lens[b] = how many stayed, new_weights their weights with zeros behind,
  * kept[b][kv head][budget] their old indices with -1 behind. */
 int vm_kv_evict_paged_bf16(const vm_paged_kv* cache_host, const float* weights, int64_t ldw_seq, int64_t ldw_head, int w_cols,
                            const int32_t* kv_lens, const int32_t* new_table, int64_t ld_new_table, int new_pages, int budget, int recent,

@@ -312,7 +312,7 @@ __global__ __launch_bounds__(SP_WAVES * 64, 2) void attn_paged_split_k(const Att
       *reinterpret_cast<u16x4_t*>(p.out + prow * p.ldo + h * HD + 16 * wave + 4 * g) = some ? w : (u16x4_t){0, 0, 0, 0};
     }
     if (writes_row) {
-      const float l2 = some ? m + log2f(l) : -INFINITY;
+      const float l2 = some && prow >= 0 ? m + log2f(l) : -INFINITY;
       p.lse[h * p.ld_lse + s.p0 + i] = l2 * LN2;
       if (p.s_ws) p.l2_ws[slot] = l2;
     }
@@ -350,8 +350,8 @@ __global__ __launch_bounds__(256) void attn_paged_join_k(const AttnPagedP p) {
     }
   }
   const bool some = !(l == 0.f);
-  const float inv = some ? 1.f / l : 0.f, l2 = some ? m + log2f(l) : -INFINITY;
   const int prow = phys_row(p, s.p0 + i);
+  const float inv = some ? 1.f / l : 0.f, l2 = some && prow >= 0 ? m + log2f(l) : -INFINITY;
   if (prow >= 0 && d < HD) {
 #pragma unroll
     for (int e = 0; e < E; ++e) p.out[prow * p.ldo + h * HD + d + e] = some ? f2bf(o[e] * inv) : (unsigned short)0;
@@ -371,7 +371,9 @@ __global__ __launch_bounds__(256) void attn_paged_count_k(const AttnPagedP p) {
   const int R = min(s.nq, p.max_q) * p.G;
   float sum = 0.f;
   // the first row of a query that sees the token: its scores, and those of all later rows, were stored by the wave that walked the block
-  for (int r = max(0, j - (s.len - s.nq)) * p.G; r < R; ++r) {
+  // (max_q bounds it before the product: R fits 32 bits, the number of rows behind a long sample need not). A page that is not there: nothing.
+  const int first = page_ok(p.c.table[b * p.c.ld_table + (j >> p.c.shift)], p.c.n_pages) ? min(max(0, j - (s.len - s.nq)), p.max_q) * p.G : R;
+  for (int r = first; r < R; ++r) {
     const float l2 = p.l2_ws[slot0 + r];
     if (l2 == -INFINITY) continue;
     sum += fast_exp2(p.s_ws[(slot0 + r) * p.s_ld + j] - l2);

@@ -400,7 +400,7 @@ __global__ __launch_bounds__(NW * 64, 2) void tile_k(const AttnPagedP p) {
   }
   const bool some = !(l_run == 0.f);
   const float inv = some ? 1.f / l_run : 0.f;
-  if (live && hf == 0) p.lse[h * p.ld_lse + s.p0 + qi] = some ? (msc + log2f(l_run)) * LN2 : -INFINITY;
+  if (live && hf == 0) p.lse[h * p.ld_lse + s.p0 + qi] = some && prow >= 0 ? (msc + log2f(l_run)) * LN2 : -INFINITY;
   // O^T registers -> this wave's slab [32 rows][HD], then whole rows out
   char* slab = smem + wave * SLAB;
 #pragma unroll
@@ -436,6 +436,7 @@ __global__ __launch_bounds__(256, 2) void weigh_k(const AttnPagedP p) {
   __shared__ __attribute__((aligned(16))) float s_l2[3][64];
   __shared__ __attribute__((aligned(16))) int s_lim[3][64];
   __shared__ int64_t s_off[3][64];                                 // element offset of the row's query, -1: no such row
+  __shared__ int s_gap[3];                                         // one of the tile's rows is no row
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), hf = lane >> 5;
   const int hk = blockIdx.y, b = blockIdx.z;
   const SeqInfo s = seq_info(p, b);
@@ -458,7 +459,7 @@ __global__ __launch_bounds__(256, 2) void weigh_k(const AttnPagedP p) {
   }
   const float sc = p.scale * LOG2E;
   float sum = 0.f;
-  const int rs = max(0, jw - past) * p.G / 64 * 64;                // the first tile with a row that sees one of these tokens
+  const int rs = min(max(0, jw - past), p.max_q) * p.G / 64 * 64;                // the first tile with a row that sees one of these tokens
   const int tiles = R > rs ? (R - rs + 63) / 64 : 0;
   struct Info { int r, i, h, row; float lse; };                    // as loaded: looked at when it is put into LDS, a tile later
   auto info = [&](int r) -> Info {
@@ -477,6 +478,8 @@ __global__ __launch_bounds__(256, 2) void weigh_k(const AttnPagedP p) {
     s_off[slot][tid] = ok ? x.row * p.ldq + x.h * HD : -1;
     s_l2[slot][tid] = ok ? x.lse * LOG2E : INFINITY;               // no such row: exp2(. - inf) = 0
     s_lim[slot][tid] = ok ? past + x.i : -1;
+    const bool gap = __builtin_amdgcn_ballot_w64(!ok) != 0;
+    if (tid == 0) s_gap[slot] = gap;
   };
   i32x4_t qv[NQ];
   auto load_q = [&](int slot) {
@@ -507,7 +510,8 @@ __global__ __launch_bounds__(256, 2) void weigh_k(const AttnPagedP p) {
     __syncthreads();
   }
   const int rb0 = a32::row_base(lane, 0), rb1 = a32::row_base(lane, 1);
-  // 64 rows against the wave's 32 tokens; edge: some rows do not see some of the tokens
+  // 64 rows against the wave's 32 tokens; edge: some rows do not see some of the tokens, or are no rows (whose zeros times an infinite key
+  // would count)
   auto add = [&](const char* qt, int slot, auto edge) {
     f32x16_t acc[2];
 #pragma unroll
@@ -541,7 +545,7 @@ __global__ __launch_bounds__(256, 2) void weigh_k(const AttnPagedP p) {
     const char* qt = qbuf[u & 1];
     const int r_last = min(rs + 64 * u + 63, R - 1);
     if (past + r_last / p.G >= j0) {
-      if (past + (rs + 64 * u) / p.G < j0 + 31) add(qt, slot, std::true_type{});
+      if (s_gap[slot] || past + (rs + 64 * u) / p.G < j0 + 31) add(qt, slot, std::true_type{});
       else add(qt, slot, std::false_type{});
     }
     if (u + 1 < tiles) store_q(qbuf[(u + 1) & 1]);

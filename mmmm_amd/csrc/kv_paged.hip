@@ -265,6 +265,9 @@ int vm_kv_evict_paged_bf16(const vm_paged_kv* cache_host, const float* weights, 
   if (rc != VM_OK) return rc;
   if (budget <= 0 || recent < 0 || recent > budget || w_cols <= 0 || new_pages <= 0 || ld_new_table < new_pages) return VM_ERR_BAD_ARG;
   if (ldw_head < w_cols || ldn_head < w_cols || ldw_seq < 0 || ldn_seq < 0) return VM_ERR_BAD_ARG;
+  const int64_t most = (int64_t)p.c.max_pages << p.c.shift;
+  const int cols = (int)(most < w_cols ? most : w_cols);
+  if ((int64_t)new_pages << p.c.shift < (budget < cols ? budget : cols)) return VM_ERR_BAD_ARG;      // who stays has a place
   if (cache_host->n_seq == 0) return VM_OK;
   if (cache_host->n_seq > 65535 || p.c.n_kv_heads > 65535) return VM_ERR_UNSUPPORTED;
   if (!weights || !kv_lens || !new_table || !new_weights || !new_lens || !kept) return VM_ERR_BAD_ARG;
@@ -277,8 +280,6 @@ int vm_kv_evict_paged_bf16(const vm_paged_kv* cache_host, const float* weights, 
   static bool ok = false;
   std::call_once(once, [] { ok = hipFuncSetAttribute((const void*)kv_evict_select_k, hipFuncAttributeMaxDynamicSharedMemorySize, EV_LDS_KEYS * 4) == hipSuccess; });
   if (!ok) return VM_ERR_LAUNCH;
-  const int64_t most = (int64_t)p.c.max_pages << p.c.shift;
-  const int cols = (int)(most < w_cols ? most : w_cols);
   p.lds_keys = cols < EV_LDS_KEYS ? cols : EV_LDS_KEYS;
   hipLaunchKernelGGL(kv_evict_select_k, dim3(p.c.n_kv_heads, cache_host->n_seq), dim3(EV_THREADS), p.lds_keys * 4, st, p);
   VM_LAUNCH_CHECK();

@@ -41,8 +41,8 @@ inline bool misaligned16(const void* a) { return ((uintptr_t)a & 15) != 0; }
 
 // the checks that every entry on the cache shares; fills `c`
 inline int paged_cache(const vm_paged_kv* a, PagedKV& c) {
-  if (!a || !a->k_pages || !a->v_pages || !a->block_table) return VM_ERR_BAD_ARG;
-  if (a->n_pages <= 0 || a->max_pages <= 0 || a->n_kv_heads <= 0 || a->n_seq < 0) return VM_ERR_BAD_ARG;
+  if (!a || !a->k_pages || !a->v_pages || a->n_seq < 0 || (a->n_seq > 0 && !a->block_table)) return VM_ERR_BAD_ARG;
+  if (a->n_pages <= 0 || a->max_pages <= 0 || a->n_kv_heads <= 0) return VM_ERR_BAD_ARG;
   if (a->head_dim != 32 && a->head_dim != 64 && a->head_dim != 128) return VM_ERR_UNSUPPORTED;
   const int shift = paged_shift(a->page_size);
   if (shift < 0) return VM_ERR_UNSUPPORTED;

@@ -934,6 +934,7 @@ def attn_paged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, bl
         w, ws_, wh, w_cols = _weights_of(weights, n_seq, hk, dev)
         wo, wos, woh, wo_cols = _weights_of(weights if weights_out is None else weights_out, n_seq, hk, dev)
         assert wo_cols == w_cols and w_cols >= min(max_kv, cols * ps), f'{w_cols} columns of weights'
+        assert n_seq <= 1 or wos != 0, 'weights_out: every sample has its own'
     else:
         assert weights_out is None
     _here(k_pages, dev)
@@ -961,7 +962,7 @@ def kv_evict_paged(k_pages: torch.Tensor, v_pages: torch.Tensor, weights: torch.
     assert new_block_table.dtype == torch.int32 and new_block_table.dim() == 2 and new_block_table.shape[0] == n_seq
     new_cols = new_block_table.shape[1]
     row, one = new_block_table.stride()
-    assert (one == 1 or new_cols == 1) and new_block_table.get_device() == dev and new_block_table.data_ptr() != block_table.data_ptr()
+    assert (one == 1 or new_cols == 1) and new_block_table.get_device() == dev and (n_seq == 0 or new_block_table.data_ptr() != block_table.data_ptr())
     most = min(budget, cols * ps, w_cols)
     assert new_cols * ps >= most, f'{most} tokens may stay: the new table holds {new_cols * ps}'
     lens = _i32(kv_lens, n_seq, dev)

@@ -96,7 +96,7 @@ def test_evict_refused(lib):
     names = ['weights', 'ldw_seq', 'ldw_head', 'w_cols', 'lens', 'new_table', 'ld_new', 'new_pages', 'budget', 'recent', 'new_w', 'ldn_seq', 'ldn_head', 'new_lens', 'kept']
     good = [P, 200, 100, 100, P, 2 * P, 3, 3, 64, 8, 2 * P, 200, 100, 2 * P, P]
     for kw in (dict(weights=None), dict(ldw_head=99), dict(w_cols=0), dict(lens=None), dict(new_table=None), dict(ld_new=2), dict(new_pages=0), dict(budget=0),
-               dict(recent=-1), dict(recent=65), dict(new_w=None), dict(ldn_head=99), dict(new_lens=None), dict(kept=None), dict(new_w=P), dict(new_lens=P), dict(new_table=P)):
+               dict(recent=-1), dict(recent=65), dict(new_w=None), dict(ldn_head=99), dict(new_lens=None), dict(kept=None), dict(new_w=P), dict(new_lens=P), dict(new_table=P), dict(new_pages=1, budget=65)):
         c = cache()
         assert lib.vm_kv_evict_paged_bf16(C.addressof(c), *[kw.get(n, g) for n, g in zip(names, good)], None) == BAD, kw
 
@@ -127,3 +127,21 @@ def test_wrappers_refuse_what_they_can_see():
             call(**kw)
     with pytest.raises(hip.HipError):                      # host tensors: there is no CPU path
         call()
+
+
+def test_no_sample_needs_no_table(lib):
+    c = cache(n_seq=0, block_table=None)
+    a = attn(c, n_rows=0, q=None, out=None, lse=None, cu_q=None, kv_lens=None)
+    n = C.c_int64(-1)
+    assert lib.vm_attn_paged_workspace(C.addressof(a), C.addressof(n)) == OK and n.value == 0
+    assert lib.vm_attn_paged_bf16(C.addressof(a), None) == OK
+    assert lib.vm_kv_append_paged_bf16(C.addressof(c), None, 1024, None, None, None, None, None, 10, 0, 4, None, 512, None, None) == OK
+    assert lib.vm_kv_evict_paged_bf16(C.addressof(c), None, 200, 100, 100, None, None, 3, 3, 64, 8, None, 200, 100, None, None, None) == OK
+
+
+def test_weights_out_of_one_sample_for_all_is_refused():
+    k = torch.zeros(4, 2, 16, 64, dtype=torch.bfloat16)
+    w = torch.zeros(1, 2, 48)
+    cu, lens = torch.zeros(3, dtype=torch.int32), torch.zeros(2, dtype=torch.int32)
+    with pytest.raises(AssertionError):
+        K.attn_paged(torch.zeros(3, 256, dtype=torch.bfloat16), k, k.clone(), torch.zeros(2, 3, dtype=torch.int32), cu, lens, 0.1, 3, 40, weights=w.expand(2, 2, 48))

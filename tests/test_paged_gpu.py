@@ -430,3 +430,81 @@ def test_bounds_that_are_too_small_stay_inside(dev, K):
         K.attn_paged(q.to(dev), k.to(dev), v.to(dev), table.to(dev), i32([0, new], dev), i32([400], dev), 0.1, bound, 400, out=out)
         close(out[:bound], want[0][:bound], want[1][:bound])
         assert ((out[bound:] == 3.0).all(1) | ((out[bound:].cpu().double() - want[0][bound:]).abs() <= want[1][bound:]).all(1).to(dev)).all()
+
+
+@pytest.mark.parametrize('new', [3, 37, 130])
+def test_weights_of_infinite_keys(dev, K, new):
+    """a key that no query wants at all (score -inf): it receives nothing, also where the last tile of queries is not full"""
+    g = torch.Generator().manual_seed(new)
+    k, v, table = R.make_cache([400], 1, 128, 64, g)
+    k[int(table[0, 1]), 0, 5, 0] = float('-inf')                             # token 69
+    q = torch.randn(new, 2 * 128, generator=g).bfloat16()
+    q[:, 0::128] = 1.0
+    w = torch.rand(1, 1, 400, generator=g)
+    got = w.to(dev)
+    out, _ = K.attn_paged(q.to(dev), k.to(dev), v.to(dev), table.to(dev), i32([0, new], dev), i32([400], dev), 0.1, new, 400, weights=got)
+    assert bool(out.isfinite().all()) and bool(got.isfinite().all())
+    assert float(got[0, 0, 69]) == float(w[0, 0, 69])
+    assert bool((got.cpu()[0, 0, :69] > w[0, 0, :69]).all())
+
+
+@pytest.mark.parametrize('new', [3, 37])
+def test_absent_pages_receive_nothing_from_strange_queries(dev, K, new):
+    """a query of NaN gives NaN to every token that it sees, and nothing to a token whose page is not there"""
+    g = torch.Generator().manual_seed(new)
+    k, v, table = R.make_cache([400], 1, 64, 16, g)
+    table[0, 3] = -1
+    q = torch.randn(new, 64, generator=g).bfloat16()
+    q[1] = NAN
+    w = torch.rand(1, 1, 400, generator=g)
+    got = w.to(dev)
+    K.attn_paged(q.to(dev), k.to(dev), v.to(dev), table.to(dev), i32([0, new], dev), i32([400], dev), 0.1, new, 400, weights=got)
+    got = got.cpu()[0, 0]
+    assert torch.equal(got[48:64], w[0, 0, 48:64])
+    seen = torch.arange(400) <= 400 - new + 1
+    seen[48:64] = False
+    assert bool(got[seen].isnan().all()) and bool(got[400 - new + 2:].isfinite().all())
+
+
+@pytest.mark.parametrize('new', [4, 37, 300])
+@pytest.mark.parametrize('L', [600, 5000])
+def test_positions_without_a_row(dev, K, new, L):
+    """row_of_pos outside the rows: no such query, lse -inf, and it counts nowhere"""
+    g = torch.Generator().manual_seed(new)
+    k, v, table = R.make_cache([L], 2, 128, 64, g)
+    q = torch.randn(new, 4 * 128, generator=g).bfloat16()
+    rop = torch.randperm(new, generator=g).to(torch.int32)
+    gone = [1, new - 2]
+    w = torch.zeros(1, 2, L)
+    want = R.attention(q, k, v, table, [new], [L], 0.1, rop, w)
+    for n in gone:                                                           # their share of the received weights, taken back
+        kk = [R.tokens(k, table, 0, L, h)[0] for h in range(2)]
+        for h in range(4):
+            x = q[int(rop[n]), h * 128:(h + 1) * 128].double() @ kk[h // 2].T * 0.1
+            x[L - new + n + 1:] = float('-inf')
+            want[4][0, h // 2] -= torch.softmax(x, 0)
+        want[2][:, n] = float('-inf')
+    lost = [int(rop[n]) for n in gone]
+    rop[gone[0]], rop[gone[1]] = -1, new
+    out = torch.full((new, 512), 3.0, dtype=torch.bfloat16, device=dev)
+    got = w.to(dev)
+    o, lse = K.attn_paged(q.to(dev), k.to(dev), v.to(dev), table.to(dev), i32([0, new], dev), i32([L], dev), 0.1, new, L, row_of_pos=rop.to(dev),
+                          weights=got, out=out)
+    keep = torch.ones(new, dtype=torch.bool)
+    keep[lost] = False
+    assert bool((o.cpu()[~keep] == 3.0).all())
+    close(o.cpu()[keep], want[0][keep], want[1][keep])
+    close(lse, want[2], want[3])
+    close(got, want[4], want[5])
+
+
+def test_an_empty_batch(dev, K):
+    """no sample at all: every entry point does nothing and says so"""
+    k = torch.zeros(4, 2, 16, 64, dtype=torch.bfloat16, device=dev)
+    v, t, none = k.clone(), torch.zeros(0, 3, dtype=torch.int32, device=dev), i32([], dev)
+    cs = torch.zeros(8, 64, device=dev)
+    w = torch.zeros(0, 2, 48, device=dev)
+    q = K.kv_append_paged(torch.zeros(0, 8 * 64, dtype=torch.bfloat16, device=dev), none, none, t, k, v, none, cs, cs, 4)
+    o, lse = K.attn_paged(q, k, v, t, i32([0], dev), none, 0.1, 0, 0, weights=w)
+    nw, nl, kept = K.kv_evict_paged(k, v, w, t, none, t.clone(), 8, 2)
+    assert o.shape == (0, 256) and lse.shape == (4, 0) and nw.shape == w.shape and nl.shape == (0,) and kept.shape == (0, 2, 8)
