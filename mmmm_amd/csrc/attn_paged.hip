@@ -3,7 +3,6 @@
 //
 // Query rows of one kv head are taken together: row r of (sample b, kv head hk) is query i = r / G of head hk G + r % G (G heads share the
 // kv head), so grouped heads read K and V once. Query i sees the tokens j <= L - n + i.
-#include <mutex>
 #include "paged.hpp"
 #include "vm_tile.hpp"
 
@@ -459,10 +458,8 @@ int64_t tile_grid(const AttnPagedP& p) {
 
 template <int HD>
 int launch_tile(const AttnPagedP& p, hipStream_t st) {
-  static std::once_flag once;
-  static bool ok = false;
-  std::call_once(once, [] { ok = hipFuncSetAttribute((const void*)apt::tile_k<HD>, hipFuncAttributeMaxDynamicSharedMemorySize, apt::RING_LDS) == hipSuccess; });
-  if (!ok) return VM_ERR_LAUNCH;
+  static std::atomic<uint64_t> set{0};
+  if (!allow_lds((const void*)apt::tile_k<HD>, apt::RING_LDS, set)) return VM_ERR_LAUNCH;
   hipLaunchKernelGGL(apt::tile_k<HD>, dim3((unsigned)tile_grid(p)), dim3(apt::NW * 64), apt::RING_LDS, st, p);
   if (p.n_split > 1) hipLaunchKernelGGL(attn_paged_join_k<HD>, dim3((p.s_rows + 3) / 4, p.c.n_kv_heads, p.n_seq), dim3(256), 0, st, p);
   if (p.w_out && p.max_kv > 0) hipLaunchKernelGGL(apt::weigh_k<HD>, dim3((p.max_kv + 127) / 128, p.c.n_kv_heads, p.n_seq), dim3(256), 0, st, p);

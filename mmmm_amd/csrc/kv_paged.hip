@@ -1,6 +1,5 @@
 // Paged KV cache of the generation path: storing new tokens (with the rotary positions of q and k) and eviction by received attention
 // weight. Replaces, for a paged cache, the rotary call and the torch.cat of /root/reference/mmmm/models/cogvlm/modeling_cogvlm.py:246-262.
-#include <mutex>
 #include "paged.hpp"
 
 namespace {
@@ -276,10 +275,8 @@ int vm_kv_evict_paged_bf16(const vm_paged_kv* cache_host, const float* weights, 
   p.lens = kv_lens; p.new_lens = new_lens; p.new_table = new_table; p.ld_new = ld_new_table; p.new_pages = new_pages;
   p.kept = kept; p.budget = budget; p.recent = recent;
   hipStream_t st = (hipStream_t)stream;
-  static std::once_flag once;
-  static bool ok = false;
-  std::call_once(once, [] { ok = hipFuncSetAttribute((const void*)kv_evict_select_k, hipFuncAttributeMaxDynamicSharedMemorySize, EV_LDS_KEYS * 4) == hipSuccess; });
-  if (!ok) return VM_ERR_LAUNCH;
+  static std::atomic<uint64_t> set{0};
+  if (!allow_lds((const void*)kv_evict_select_k, EV_LDS_KEYS * 4, set)) return VM_ERR_LAUNCH;
   p.lds_keys = cols < EV_LDS_KEYS ? cols : EV_LDS_KEYS;
   hipLaunchKernelGGL(kv_evict_select_k, dim3(p.c.n_kv_heads, cache_host->n_seq), dim3(EV_THREADS), p.lds_keys * 4, st, p);
   VM_LAUNCH_CHECK();

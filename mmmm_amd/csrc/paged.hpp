@@ -5,6 +5,7 @@
 // piece of memory. Token j of sample b lies in page block_table[b][j / page_size], row j % page_size; page_size is a power of two >= 16.
 // A table entry outside [0, n_pages) is a page that is not there: nothing is read or written through it and its tokens are masked.
 #pragma once
+#include <atomic>
 #include "vm_common.hpp"
 
 typedef __attribute__((ext_vector_type(4))) unsigned u32x4_t;
@@ -35,6 +36,17 @@ inline int paged_shift(int page_size) {          // log2 of a legal page size, -
   for (int s = 4; s <= 10; ++s)
     if (page_size == 1 << s) return s;
   return -1;
+}
+
+// allows `fn` that much dynamic LDS on the current device; once per device (`done`: a bit for each of the first 64)
+inline bool allow_lds(const void* fn, int bytes, std::atomic<uint64_t>& done) {
+  int dev = 0;
+  if (hipGetDevice(&dev) != hipSuccess) return false;
+  const uint64_t bit = dev < 64 ? 1ull << dev : 0;
+  if (done.load(std::memory_order_relaxed) & bit) return true;
+  if (hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, bytes) != hipSuccess) return false;
+  done.fetch_or(bit, std::memory_order_relaxed);
+  return true;
 }
 
 inline bool misaligned16(const void* a) { return ((uintptr_t)a & 15) != 0; }

@@ -943,9 +943,9 @@ def attn_paged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, bl
     op, ldo = _rows(out, q.shape, dev)
     lse = torch.empty(n_heads, rows, dtype=torch.float32, device=q.device)
     need = _attn_paged_ws_bytes(n_seq, hk, hd, ps, cols, rows, max_q, max_kv, n_heads, w_cols)
-    ws = torch.empty(need, dtype=torch.uint8, device=q.device).data_ptr() if need else 0
+    buf = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None      # (held until the launch is in the stream)
     hip.call('vm_attn_paged_bf16', hip.ATTN_PAGED.pack(
-        *c, qp, ldq, cu, lens, order, op, ldo, lse.data_ptr(), rows, rows, max_q, max_kv, n_heads, scale, w_cols, w, wo, ws_, wh, wos, woh, ws, need), stream())
+        *c, qp, ldq, cu, lens, order, op, ldo, lse.data_ptr(), rows, rows, max_q, max_kv, n_heads, scale, w_cols, w, wo, ws_, wh, wos, woh, 0 if buf is None else buf.data_ptr(), need), stream())
     return out, lse
 
 

@@ -442,7 +442,8 @@ class CogVLMForCausalLM(nn.Module):
         if past_key_values is not None and len(past_key_values) > 0 and not (isinstance(past_key_values, PagedKVCache) and input_ids.shape[1] > 1):
             # decode step of the generation path (reference :441-442, 253-262): the last column is the new token
             assert labels is None and input_ids.shape[1] >= 1
-            x = self.model.decode_step(input_ids[:, -1], position_ids[:, -1], past_key_values)
+            live = attention_mask[:, -1].bool() if attention_mask is not None and isinstance(past_key_values, PagedKVCache) else None
+            x = self.model.decode_step(input_ids[:, -1], position_ids[:, -1], past_key_values, live)
             logits = linear_decode(x, self.lm_head).float()
             return CausalLMOutputWithPast(logits=logits[:, None], past_key_values=past_key_values, last_hidden_packed=x)
         cache = None

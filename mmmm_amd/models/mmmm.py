@@ -401,7 +401,8 @@ class MMMMForCausalLM(CogVLMForCausalLM):
         `kv_page_size` keeps the cache in pages, for this call; a conversation gives a paged cache of its own as `past_key_values` to every turn
         (`new_kv_cache(batch, max_len, device, page_size=...)`, empty at first): the `input_ids` of a turn follow what is cached (image None or a
         further one). A sample's last new token — its eos, where it has ended — is not cached: the next
-        `input_ids` begin with it. `kv_budget` bounds the cached tokens per sample: after the prompt, and whenever one page more has gathered,
+        `input_ids` begin with it. A sample without valid tokens in `attention_mask` sits the turn out (its new tokens mean
+        nothing). `kv_budget` bounds the cached tokens per sample: after the prompt, and whenever one page more has gathered,
         the tokens that have received the least attention leave (per layer and head; the `kv_recent` newest always stay)."""
         if past_key_values is not None and not isinstance(past_key_values, PagedKVCache):
             raise ValueError('only a paged cache can be continued: kv_page_size')
@@ -447,7 +448,8 @@ class MMMMForCausalLM(CogVLMForCausalLM):
             prev_tok = input_ids[torch.arange(B, device=dev), last_col]
             pos = position_ids[torch.arange(B, device=dev), last_col]
             bop, eop = self.tokenizer.bop_token_id, self.tokenizer.eop_token_id
-            done = torch.zeros(B, dtype=torch.bool, device=dev)
+            # a sample without a valid token in this call says nothing (paged cache: neither are its tokens stored)
+            done = n_valid == 0 if paged else torch.zeros(B, dtype=torch.bool, device=dev)
             head = self.lm_head.weight.detach()
 
             def choose(logits, prev_tok, pos, done, t):
@@ -460,7 +462,7 @@ class MMMMForCausalLM(CogVLMForCausalLM):
 
             if use_graph and forced_tokens is None and not return_logits and steps > 2:
                 new_tokens, new_pos = self._generate_graphed(cache, head, logits, prev_tok, pos, done, steps, eos_token_id, bop, eop,
-                                                             eos_check_every, trim)
+                                                             eos_check_every, trim, past_key_values is not None)
                 return GenerateOutput(new_tokens=new_tokens, new_position_ids=new_pos, prompt_lengths=n_valid, past_key_values=cache)
             new_tokens, new_pos, all_logits = [], [], ([logits] if return_logits else None)
             for t in range(steps):
@@ -471,7 +473,7 @@ class MMMMForCausalLM(CogVLMForCausalLM):
                     break
                 if forced_tokens is None and eos_token_id is not None and (t + 1) % eos_check_every == 0 and bool(done.all()):
                     break
-                live = ~done if paged and eos_token_id is not None else None
+                live = ~done if paged and (eos_token_id is not None or past_key_values is not None) else None
                 logits = linear_decode(self.model.decode_step(tok, pos, cache, live), self.lm_head).float()
                 trim()
                 if return_logits:
@@ -491,7 +493,7 @@ class MMMMForCausalLM(CogVLMForCausalLM):
         most = max(L, min(L + steps, budget + page_size + 1))
         return self.new_kv_cache(B, most, dev, page_size=page_size, n_pages=B * (up(most) + up(budget)), track_weights=True)
 
-    def _generate_graphed(self, cache, head, logits, prev_tok, pos, done, steps, eos_token_id, bop, eop, eos_check_every, trim):
+    def _generate_graphed(self, cache, head, logits, prev_tok, pos, done, steps, eos_token_id, bop, eop, eos_check_every, trim, turn):
         """greedy loop with the decode step captured in a hipGraph. State lives in static device buffers that the graph
         updates in place: (tok, pos, done) of the newest token, a step counter, and the [B, steps] outputs it scatters into.
         One eager step first: it sets the lazily-initialised kernel attributes and warms the allocator outside the capture."""
@@ -510,7 +512,7 @@ class MMMMForCausalLM(CogVLMForCausalLM):
         paged = isinstance(cache, PagedKVCache)
 
         def decode(tok, pos, done):
-            live = ~done if paged and eos_token_id is not None else None
+            live = ~done if paged and (eos_token_id is not None or turn) else None
             return linear_decode(self.model.decode_step(tok, pos, cache, live), self.lm_head).float()
 
         tok, pos, done = choose(logits, prev_tok, pos, done)

@@ -133,3 +133,28 @@ def test_budget(dev, lm):
         lm.generate(ids, **kw, max_new_tokens=4, past_key_values=lm.new_kv_cache(3, 200, dev))
     with pytest.raises(ValueError):
         lm.generate(ids, **kw, max_new_tokens=4, past_key_values=want.past_key_values, kv_budget=24)
+
+
+@pytest.mark.parametrize('graph', [False, True])
+@pytest.mark.parametrize('width', [1, 6])
+def test_a_sample_sits_a_turn_out(dev, lm, width, graph):
+    """one sample has nothing to say in the second turn: nothing of it is stored, the others answer as they would without it"""
+    batch, tok = make_inputs(dev)
+    lm.tokenizer = tok
+    ids, kw = _batch(batch)
+    g = torch.Generator().manual_seed(3)
+    said = torch.randint(3, 150, (3, width), generator=g).to(dev)
+    answers = []
+    for silent in (None, 1):
+        cache = lm.new_kv_cache(3, ids.shape[1] + 40, dev, page_size=16)
+        one = lm.generate(ids, **kw, max_new_tokens=3, past_key_values=cache)
+        before = cache.lens.tolist()
+        mask = torch.ones_like(said)
+        if silent is not None:
+            mask[silent] = 0
+        pos = one.new_position_ids[:, -1:] + torch.arange(width, device=dev)
+        two = lm.generate(said, token_type_ids=torch.zeros_like(said), position_ids=pos, attention_mask=mask, image=None, patch_size=None, pool_size=None,
+                          max_new_tokens=6, past_key_values=cache, use_graph=graph)
+        assert cache.lens.tolist() == [n if s == silent else n + width + 5 for s, n in enumerate(before)]
+        answers.append(two.new_tokens)
+    assert torch.equal(answers[0][[0, 2]], answers[1][[0, 2]])
