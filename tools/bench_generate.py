@@ -1,6 +1,6 @@
 """Generation path at true width: CogVLM-7B + EVA-ViT-E + r64 LoRA, random-init bf16, greedy decoding.
 
-    python tools/bench_generate.py [--batch 1 8] [--new 64] [--image 448]
+    python tools/bench_generate.py [--batch 1 8] [--new 64] [--page-size 0 64] [--budget 512]
 
 Reports prefill time and decode tokens/s. Decode is HBM-bound: one step reads the language-expert weights of every layer
 (the vision expert is never touched by a single-token call), the LoRA factors, lm_head, and the K / V rows of the cache:
@@ -38,17 +38,21 @@ def main():
     ap.add_argument('--text', type=int, default=64)
     ap.add_argument('--depth-scale', type=float, default=1.0)
     ap.add_argument('--graph', type=int, default=1)
+    ap.add_argument('--page-size', type=int, nargs='+', default=[0], help='0: one slab per sample; else the paged cache')
+    ap.add_argument('--budget', type=int, help='paged cache: tokens kept per sample')
     args = ap.parse_args()
     dev = torch.device('cuda:0')
     torch.cuda.set_device(dev)
     w = dict(bench.WORKLOADS['phase-vlm-448'])
     model, tok = bench.build(w, dev, args.depth_scale)
     model.eval()
-    for B in args.batch:
+    for B, page in ((B, page) for B in args.batch for page in args.page_size):
         batch = bench.make_batch(w, tok, B, dev, seed=B)
         vi = batch['vlm_inputs']
         kw = dict(token_type_ids=vi['token_type_ids'], position_ids=vi['position_ids'], attention_mask=vi['attention_mask'],
                   image=batch['image'], patch_size=batch['patch_size'], pool_size=batch['pool_size'])
+        if page:
+            kw.update(kv_page_size=page, kv_budget=args.budget)
         model.generate(vi['input_ids'], **kw, max_new_tokens=4)            # warm-up (lazy kernel attributes, allocator)
         torch.cuda.synchronize()
         t0 = time.perf_counter()
@@ -67,6 +71,7 @@ def main():
             'metric': 'decode tokens/sec', 'value': B / step, 'unit': 'tokens/s', 'batch': B, 'new_tokens': args.new,
             'ms_per_step': step * 1e3, 'prefill_ms': t_prefill * 1e3, 'prompt_tokens': int(vi['attention_mask'].sum(1).max()),
             'dtype': 'bf16', 'data': 'synthetic', 'weights': 'random-init', 'hip_graph': bool(args.graph),
+            **(dict(kv_page_size=page, kv_budget=args.budget) if page else {}),
             'roofline': {'bound': 'hbm', 'achieved': nbytes / step / 1e9, 'peak': 8000.0, 'unit': 'GB/s',
                          'frac': nbytes / step / 8e12, 'algorithmic_bytes_per_step': nbytes},
             'tokens': out.new_tokens[0, :8].tolist(),
