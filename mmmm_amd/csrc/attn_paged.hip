@@ -24,6 +24,7 @@ struct AttnPagedP {
   // split form: n_split key splits; workspace of s_rows query rows per (sample, kv head)
   int n_split, s_rows, s_ld;
   int n_tiles, n_wg;          // tile form: row tiles per (sample, kv head), workgroups
+  int w_blocks;               // weigh_k: 128-token blocks per (sample, kv head)
   float* part;                // [.., s_rows, n_split, hd + 4]: max, sum, -, -, O
   float* s_ws;                // [.., s_rows, s_ld] scores (log2 domain), if the received weights are asked for
   float* l2_ws;               // [.., s_rows] log2 of the rows' sums
@@ -322,36 +323,53 @@ __global__ __launch_bounds__(SP_WAVES * 64, 2) void attn_paged_split_k(const Att
   }
 }
 
-// joins the key splits of a query row: one wave per row, HD / 64 (at least 1) elements per lane, the splits in their order
+// joins the key splits of a query row: out = sum_k 2^(m_k - m) O_k / sum_k 2^(m_k - m) l_k, the splits in their order. One wave per row, HD / 64 (at
+// least 1) elements per lane. Latency-bound for a few rows (4 us of which the launch is most): the partial results are asked for four splits at a
+// time and before anything is known about the sample (a row that does not exist reads its own piece of the workspace and throws it away).
 template <int HD>
 __global__ __launch_bounds__(256) void attn_paged_join_k(const AttnPagedP p) {
-  constexpr int E = HD >= 128 ? 2 : 1;
+  constexpr int E = HD >= 128 ? 2 : 1, U = 4;
+  typedef float fE_t __attribute__((ext_vector_type(E)));
   const int lane = threadIdx.x & 63, hk = blockIdx.y, b = blockIdx.z;
-  const int r = blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int r = blockIdx.x * 4 + (threadIdx.x >> 6), n = p.n_split;
+  const int64_t slot = ((int64_t)b * p.c.n_kv_heads + hk) * p.s_rows + min(r, p.s_rows - 1);
+  const float* part = p.part + slot * n * (HD + 4);
+  const int d = min(lane * E, HD - E);
+  struct Piece { float m[U], l[U]; fE_t o[U]; } x;
+  auto load = [&](int k0) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const float* q = part + (int64_t)min(k0 + u, n - 1) * (HD + 4);
+      const f32x2_t ml = *reinterpret_cast<const f32x2_t*>(q);
+      x.m[u] = ml[0];
+      x.l[u] = ml[1];
+      x.o[u] = *reinterpret_cast<const fE_t*>(q + 4 + d);
+    }
+  };
+  load(0);
+  float m = -INFINITY;
+  for (int k = lane; k < n; k += 64) m = fmaxf(m, part[(int64_t)k * (HD + 4)]);
   const SeqInfo s = seq_info(p, b);
   if (r >= min(s.nq, p.max_q) * p.G) return;
-  const int i = r / p.G, h = hk * p.G + r % p.G;
-  const int64_t slot = ((int64_t)b * p.c.n_kv_heads + hk) * p.s_rows + r;
-  const float* part = p.part + slot * p.n_split * (HD + 4);
-  float m = -INFINITY;
-  for (int k = lane; k < p.n_split; k += 64) m = fmaxf(m, part[k * (HD + 4)]);
+  const int i = r / p.G, h = hk * p.G + r % p.G, prow = phys_row(p, s.p0 + i);
   m = wave_max(m);
   const float base = m == -INFINITY ? 0.f : m;
-  float l = 0.f, o[E] = {0.f};
-  const int d = lane * E;
-  for (int k = 0; k < p.n_split; ++k) {
-    const float* q = part + k * (HD + 4);
-    const float f = fast_exp2(q[0] - base);
-    l += f * q[1];
-    if (d < HD) {
+  float l = 0.f;
+  fE_t o = {0.f};
+  for (int k = 0; k < n; k += U) {
+    if (k > 0) load(k);
 #pragma unroll
-      for (int e = 0; e < E; ++e) o[e] = fmaf(f, q[4 + d + e], o[e]);
+    for (int u = 0; u < U; ++u) {
+      if (k + u >= n) break;
+      const float f = fast_exp2(x.m[u] - base);
+      l += f * x.l[u];
+#pragma unroll
+      for (int e = 0; e < E; ++e) o[e] = fmaf(f, x.o[u][e], o[e]);
     }
   }
   const bool some = !(l == 0.f);
-  const int prow = phys_row(p, s.p0 + i);
   const float inv = some ? 1.f / l : 0.f, l2 = some && prow >= 0 ? m + log2f(l) : -INFINITY;
-  if (prow >= 0 && d < HD) {
+  if (prow >= 0 && lane * E < HD) {
 #pragma unroll
     for (int e = 0; e < E; ++e) p.out[prow * p.ldo + h * HD + d + e] = some ? f2bf(o[e] * inv) : (unsigned short)0;
   }
@@ -457,14 +475,23 @@ int64_t tile_grid(const AttnPagedP& p) {
 }
 
 template <int HD>
-int launch_tile(const AttnPagedP& p, hipStream_t st) {
+int launch_weigh(AttnPagedP& p, hipStream_t st) {
+  p.w_blocks = (p.max_kv + 127) / 128;
+  const int64_t caches = ((int64_t)p.n_seq * p.c.n_kv_heads + 7) / 8 * 8;
+  if (caches * p.w_blocks > 0x7FFFFF00) return VM_ERR_UNSUPPORTED;
+  hipLaunchKernelGGL(apt::weigh_k<HD>, dim3((unsigned)(caches * p.w_blocks)), dim3(256), 0, st, p);
+  VM_LAUNCH_CHECK();
+  return VM_OK;
+}
+
+template <int HD>
+int launch_tile(AttnPagedP& p, hipStream_t st) {
   static std::atomic<uint64_t> set{0};
   if (!allow_lds((const void*)apt::tile_k<HD>, apt::RING_LDS, set)) return VM_ERR_LAUNCH;
   hipLaunchKernelGGL(apt::tile_k<HD>, dim3((unsigned)tile_grid(p)), dim3(apt::NW * 64), apt::RING_LDS, st, p);
   if (p.n_split > 1) hipLaunchKernelGGL(attn_paged_join_k<HD>, dim3((p.s_rows + 3) / 4, p.c.n_kv_heads, p.n_seq), dim3(256), 0, st, p);
-  if (p.w_out && p.max_kv > 0) hipLaunchKernelGGL(apt::weigh_k<HD>, dim3((p.max_kv + 127) / 128, p.c.n_kv_heads, p.n_seq), dim3(256), 0, st, p);
   VM_LAUNCH_CHECK();
-  return VM_OK;
+  return p.w_out && p.max_kv > 0 ? launch_weigh<HD>(p, st) : VM_OK;
 }
 
 }  // namespace
@@ -506,11 +533,7 @@ int vm_attn_paged_bf16(const vm_attn_paged_args* args_host, void* stream) {
     if (hd == 64) return launch_tile<64>(p, st);
     return launch_tile<32>(p, st);
   }
-  if (p.w_out && p.max_kv > 0) {                     // no new token anywhere: the weights stay what they are
-    hipLaunchKernelGGL(apt::weigh_k<32>, dim3((p.max_kv + 127) / 128, p.c.n_kv_heads, p.n_seq), dim3(256), 0, st, p);
-    VM_LAUNCH_CHECK();
-  }
-  return VM_OK;
+  return p.w_out && p.max_kv > 0 ? launch_weigh<32>(p, st) : VM_OK;      // no new token anywhere: the weights stay what they are
 }
 
 }  // extern "C"

@@ -229,15 +229,22 @@ __global__ __launch_bounds__(NW * 64, 2) void tile_k(const AttnPagedP p) {
     st.init(hk, p.c.shift, wave, lane);
     // DMA order per wave (PW instructions a group): K(0) V(0) V(1) K(1); c0(u) issues V(u+2), c1(u) issues K(u+2). At the end of c0(u) V(u)
     // must have landed (V(u+1) K(u+1) V(u+2) may fly: vmcnt(3 PW)), at the end of c2(u) K(u+1) (V(u+2) K(u+2): vmcnt(2 PW)).
+    // the queries were asked for before the tiles: they have arrived when the first of those is waited for (said here, so that no wait for them
+    // stands inside the loop)
+    auto arrived = [&]() {
+#pragma unroll
+      for (int k = 0; k < KS; ++k) asm volatile("" : "+v"(qf[k]));
+    };
     Pages pga = pages_of(t0), pgb = pages_of(t0 + 1), pgc = pages_of(t0 + 2);
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");               // nothing older in the queue
     st.stage(p.c.k, p.c, pga.own, t0, kv_end, kring, wave);
     st.stage(p.c.v, p.c, pga.own, t0, kv_end, vring, wave);
     if (nt > 1) {
       st.stage(p.c.v, p.c, pgb.own, t0 + 1, kv_end, vring + TILE, wave);
       st.stage(p.c.k, p.c, pgb.own, t0 + 1, kv_end, kring + TILE, wave);
+      arrived();
       cluster_end<3 * PW>();
     } else {
+      arrived();
       cluster_end<0>();
     }
     if (late) cluster_end<-1>();
@@ -430,17 +437,26 @@ __global__ __launch_bounds__(NW * 64, 2) void tile_k(const AttnPagedP p) {
 // rows one tile ahead through registers. Bound by the exponentials: 32 x (16 + 8) cycles per 64 x 32 tile beside 512 of the matrix pipe.
 // (The first form had the rows straight from memory as B operands of each wave: 60 us on 8 x 456, bound by the L1's line rate.)
 template <int HD>
-__global__ __launch_bounds__(256, 2) void weigh_k(const AttnPagedP p) {
+__global__ __launch_bounds__(256, 4) void weigh_k(const AttnPagedP p) {
   constexpr int KS = HD / 16, CPR = HD / 8, NQ = CPR / 4;          // 16-byte chunks per row, chunks per thread and tile
   __shared__ __attribute__((aligned(16))) char qbuf[2][TILE];
   __shared__ __attribute__((aligned(16))) float s_l2[3][64];
   __shared__ __attribute__((aligned(16))) int s_lim[3][64];
-  __shared__ int64_t s_off[3][64];                                 // element offset of the row's query, -1: no such row
+  __shared__ int64_t s_off[3][64];                                 // element offset of the row's query (no such row: 0, any query)
   __shared__ int s_gap[3];                                         // one of the tile's rows is no row
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), hf = lane >> 5;
-  const int hk = blockIdx.y, b = blockIdx.z;
+  // 128 tokens of one cache. The blocks of a cache differ in work (early tokens are seen by more rows) and share its queries: every XCD takes whole
+  // caches where there are enough of them (blocks dealt out in order would give one XCD the early blocks of all: 8 x 456 with the attention 69 beside 68 us).
+  int blk, hs;
+  {
+    const int id = blockIdx.x, caches = p.n_seq * p.c.n_kv_heads, slot = id >> 3;
+    blk = caches >= 16 ? slot % p.w_blocks : id % p.w_blocks;
+    hs = caches >= 16 ? (slot / p.w_blocks) * 8 + (id & 7) : id / p.w_blocks;
+    if (hs >= caches) return;
+  }
+  const int hk = hs % p.c.n_kv_heads, b = hs / p.c.n_kv_heads;
   const SeqInfo s = seq_info(p, b);
-  const int n = min(s.len, p.w_cols), jw = blockIdx.x * 128, j0 = jw + wave * 32, j = j0 + (lane & 31);
+  const int n = min(s.len, p.w_cols), jw = blk * 128, j0 = jw + wave * 32, j = j0 + (lane & 31);
   if (jw >= n) return;
   const int R = min(s.nq, p.max_q) * p.G, past = s.len - s.nq;
   bool there = false;
@@ -449,13 +465,10 @@ __global__ __launch_bounds__(256, 2) void weigh_k(const AttnPagedP p) {
     int page = -1;
     if (j < n) page = p.c.table[b * p.c.ld_table + (j >> p.c.shift)];
     there = page_ok(page, p.c.n_pages);
-    // (a token that is not there reads row 0 of the pool and counts as zeros: no branch per load)
+    // (a token that is not there reads row 0 of the pool: its column of the product is thrown away)
     const unsigned short* kr = p.c.k + (there ? page_row(page, p.c.ld_page, hk, j & p.c.mask, p.c.shift, HD) : 0) + 8 * hf;
 #pragma unroll
-    for (int k = 0; k < KS; ++k) {
-      const i32x4_t v = *reinterpret_cast<const i32x4_t*>(kr + 16 * k);
-      kf[k] = __builtin_bit_cast(bf16x8_t, there ? v : (i32x4_t){0, 0, 0, 0});
-    }
+    for (int k = 0; k < KS; ++k) kf[k] = *reinterpret_cast<const bf16x8_t*>(kr + 16 * k);
   }
   const float sc = p.scale * LOG2E;
   float sum = 0.f;
@@ -475,7 +488,7 @@ __global__ __launch_bounds__(256, 2) void weigh_k(const AttnPagedP p) {
   };
   auto put = [&](int slot, const Info& x) {
     const bool ok = x.r < R && (unsigned)x.row < (unsigned)p.n_rows && x.lse != -INFINITY;
-    s_off[slot][tid] = ok ? x.row * p.ldq + x.h * HD : -1;
+    s_off[slot][tid] = ok ? x.row * p.ldq + x.h * HD : 0;
     s_l2[slot][tid] = ok ? x.lse * LOG2E : INFINITY;               // no such row: exp2(. - inf) = 0
     s_lim[slot][tid] = ok ? past + x.i : -1;
     const bool gap = __builtin_amdgcn_ballot_w64(!ok) != 0;
@@ -486,9 +499,7 @@ __global__ __launch_bounds__(256, 2) void weigh_k(const AttnPagedP p) {
 #pragma unroll
     for (int i = 0; i < NQ; ++i) {
       const int c = tid + 256 * i;
-      const int64_t off = s_off[slot][c / CPR];
-      const i32x4_t v = *reinterpret_cast<const i32x4_t*>(p.q + (off < 0 ? 0 : off) + (c % CPR) * 8);
-      qv[i] = off < 0 ? (i32x4_t){0, 0, 0, 0} : v;
+      qv[i] = *reinterpret_cast<const i32x4_t*>(p.q + s_off[slot][c / CPR] + (c % CPR) * 8);
     }
   };
   auto store_q = [&](char* tile) {
@@ -510,32 +521,32 @@ __global__ __launch_bounds__(256, 2) void weigh_k(const AttnPagedP p) {
     __syncthreads();
   }
   const int rb0 = a32::row_base(lane, 0), rb1 = a32::row_base(lane, 1);
-  // 64 rows against the wave's 32 tokens; edge: some rows do not see some of the tokens, or are no rows (whose zeros times an infinite key
-  // would count)
+  // 64 rows against the wave's 32 tokens; edge: some rows do not see some of the tokens, or are no rows
   auto add = [&](const char* qt, int slot, auto edge) {
-    f32x16_t acc[2];
-#pragma unroll
-    for (int rt = 0; rt < 2; ++rt) {
-      acc[rt] = (f32x16_t){0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int k = 0; k < KS; ++k) acc[rt] = a32::mfma32(a32::ld_row(qt + ((k & 1) ? rb1 : rb0), 8192 * rt + 512 * (k >> 1)), kf[k], acc[rt]);
-    }
     float part[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+    for (int rt = 0; rt < 2; ++rt) {                               // (not unrolled: 128 registers, four workgroups per CU)
+      f32x16_t acc = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int g4 = 0; g4 < 8; ++g4) {
-      const int row = 8 * g4 + 4 * hf;
-      const f32x4_t l2 = *reinterpret_cast<const f32x4_t*>(&s_l2[slot][row]);
-      i32x4_t lim;
-      if constexpr (decltype(edge)::value) lim = *reinterpret_cast<const i32x4_t*>(&s_lim[slot][row]);
+      for (int k = 0; k < KS; ++k) acc = a32::mfma32(a32::ld_row(qt + 8192 * rt + ((k & 1) ? rb1 : rb0), 512 * (k >> 1)), kf[k], acc);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float x = fast_exp2(fmaf(acc[g4 >> 2][4 * (g4 & 3) + e], sc, -l2[e]));
-        if constexpr (decltype(edge)::value) part[e] += j <= lim[e] ? x : 0.f;
-        else part[e] += x;
+      for (int g4 = 0; g4 < 4; ++g4) {
+        const int row = 32 * rt + 8 * g4 + 4 * hf;
+        const f32x4_t l2 = *reinterpret_cast<const f32x4_t*>(&s_l2[slot][row]);
+        i32x4_t lim;
+        if constexpr (decltype(edge)::value) lim = *reinterpret_cast<const i32x4_t*>(&s_lim[slot][row]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float x = fast_exp2(fmaf(acc[4 * g4 + e], sc, -l2[e]));
+          if constexpr (decltype(edge)::value) part[e] += j <= lim[e] ? x : 0.f;
+          else part[e] += x;
+        }
       }
     }
     sum += (part[0] + part[1]) + (part[2] + part[3]);
   };
+#pragma unroll
+  for (int k = 0; k < KS; ++k) asm volatile("" : "+v"(kf[k]));       // they are here: no wait for them in the loop, which would be one for the rows too
   int slot = 0;
   for (int u = 0; u < tiles; ++u) {
     const int next = slot == 2 ? 0 : slot + 1, third = next == 2 ? 0 : next + 1;
