@@ -27,7 +27,7 @@ struct AttnPagedP {
   int w_blocks;               // weigh_k: 128-token blocks per (sample, kv head)
   float* part;                // [.., s_rows, n_split, hd + 4]: max, sum, -, -, O
   float* s_ws;                // [.., s_rows, s_ld] scores (log2 domain), if the received weights are asked for
-  float* l2_ws;               // [.., s_rows] log2 of the rows' sums
+  int join_blocks;            // attn_paged_join_k: workgroups (x) that join rows; those behind them count
 };
 
 // what one sample brings, read from the device and held inside the buffers' bounds
@@ -132,6 +132,22 @@ __device__ __forceinline__ void load_block(const AttnPagedP& p, KVBlock<HD>& x, 
   }
 }
 
+// The received weight of token j from the scores that the query rows left behind (log2 domain) and the log2 of their sums, the rows in their order.
+__device__ __forceinline__ void count(const AttnPagedP& p, const SeqInfo& s, int b, int hk, int R, int j, const float* l2) {
+  float sum = 0.f;
+  // the first row of a query that sees the token: its scores, and those of all later rows, were stored by the wave that walked the block
+  // (max_q bounds it before the product: R fits 32 bits, the number of rows behind a long sample need not). A page that is not there: nothing.
+  const int first = page_ok(p.c.table[b * p.c.ld_table + (j >> p.c.shift)], p.c.n_pages) ? min(max(0, j - (s.len - s.nq)), p.max_q) * p.G : R;
+  const float* sc = p.s_ws + ((int64_t)b * p.c.n_kv_heads + hk) * p.s_rows * p.s_ld + j;
+  float x[SP_ROWS];
+#pragma unroll
+  for (int r = 0; r < SP_ROWS; ++r) x[r] = r >= first && r < R ? sc[(int64_t)r * p.s_ld] : -INFINITY;
+#pragma unroll
+  for (int r = 0; r < SP_ROWS; ++r)
+    if (r >= first && r < R && l2[r] != -INFINITY) sum += fast_exp2(x[r] - l2[r]);
+  p.w_out[b * p.ldwo_seq + hk * p.ldwo_head + j] = p.w_in[b * p.ldw_seq + hk * p.ldw_head + j] + sum;
+}
+
 template <int HD>
 __global__ __launch_bounds__(SP_WAVES * 64, 2) void attn_paged_split_k(const AttnPagedP p) {
   typedef KVBlock<HD> B;
@@ -146,7 +162,11 @@ __global__ __launch_bounds__(SP_WAVES * 64, 2) void attn_paged_split_k(const Att
   const int split = blockIdx.x;
   const SeqInfo s = seq_info(p, b);
   const int R = min(min(s.nq, p.max_q) * p.G, SP_ROWS);
-  if (R <= 0) return;
+  if (R <= 0) {                                      // no new token: the weights stay what they are
+    if (p.s_ws && p.n_split == 1)
+      for (int j = threadIdx.x; j < min(s.len, min(p.w_cols, p.s_ld)); j += SP_WAVES * 64) count(p, s, b, hk, 0, j, red[0][0]);
+    return;
+  }
   const int r = ln;
   const bool live = r < R;
   const int i = live ? r / p.G : 0, h = hk * p.G + (live ? r - i * p.G : 0);
@@ -296,30 +316,34 @@ __global__ __launch_bounds__(SP_WAVES * 64, 2) void attn_paged_split_k(const Att
       for (int e = 0; e < 4; ++e) slab[(16 * t + 4 * g + e) * 16 + ln] = o[t][e] * f;
   }
   __syncthreads();
-  if (!live || wave >= ND) return;
-  f32x4_t x = {0.f, 0.f, 0.f, 0.f};                // the wave's 16 columns
+  if (live && wave < ND) {
+    f32x4_t x = {0.f, 0.f, 0.f, 0.f};              // the wave's 16 columns
 #pragma unroll
-  for (int k = 0; k < KW; ++k)
+    for (int k = 0; k < KW; ++k)
 #pragma unroll
-    for (int e = 0; e < 4; ++e) x[e] += reinterpret_cast<const float*>(smem[k])[(16 * wave + 4 * g + e) * 16 + ln];
-  const bool writes_row = wave == 0 && g == 0;
-  const int64_t slot = ((int64_t)b * p.c.n_kv_heads + hk) * p.s_rows + r;
-  if (p.n_split == 1) {
-    const bool some = !(l == 0.f);
-    const float inv = some ? 1.f / l : 0.f;
-    if (prow >= 0) {
-      const u16x4_t w = {f2bf(x[0] * inv), f2bf(x[1] * inv), f2bf(x[2] * inv), f2bf(x[3] * inv)};
-      *reinterpret_cast<u16x4_t*>(p.out + prow * p.ldo + h * HD + 16 * wave + 4 * g) = some ? w : (u16x4_t){0, 0, 0, 0};
+      for (int e = 0; e < 4; ++e) x[e] += reinterpret_cast<const float*>(smem[k])[(16 * wave + 4 * g + e) * 16 + ln];
+    const bool writes_row = wave == 0 && g == 0;
+    if (p.n_split == 1) {
+      const bool some = !(l == 0.f);
+      const float inv = some ? 1.f / l : 0.f;
+      if (prow >= 0) {
+        const u16x4_t w = {f2bf(x[0] * inv), f2bf(x[1] * inv), f2bf(x[2] * inv), f2bf(x[3] * inv)};
+        *reinterpret_cast<u16x4_t*>(p.out + prow * p.ldo + h * HD + 16 * wave + 4 * g) = some ? w : (u16x4_t){0, 0, 0, 0};
+      }
+      if (writes_row) {
+        const float l2 = some && prow >= 0 ? m + log2f(l) : -INFINITY;
+        p.lse[h * p.ld_lse + s.p0 + i] = l2 * LN2;
+        red[0][0][ln] = l2;
+      }
+    } else {
+      float* part = p.part + ((((int64_t)b * p.c.n_kv_heads + hk) * p.s_rows + r) * p.n_split + split) * (HD + 4);
+      if (writes_row) { part[0] = m; part[1] = l; }
+      *reinterpret_cast<f32x4_t*>(part + 4 + 16 * wave + 4 * g) = x;
     }
-    if (writes_row) {
-      const float l2 = some && prow >= 0 ? m + log2f(l) : -INFINITY;
-      p.lse[h * p.ld_lse + s.p0 + i] = l2 * LN2;
-      if (p.s_ws) p.l2_ws[slot] = l2;
-    }
-  } else {
-    float* part = p.part + (slot * p.n_split + split) * (HD + 4);
-    if (writes_row) { part[0] = m; part[1] = l; }
-    *reinterpret_cast<f32x4_t*>(part + 4 + 16 * wave + 4 * g) = x;
+  }
+  if (p.s_ws && p.n_split == 1) {                   // nothing to join: the received weights at once
+    __syncthreads();
+    for (int j = threadIdx.x; j < min(s.len, min(p.w_cols, p.s_ld)); j += SP_WAVES * 64) count(p, s, b, hk, R, j, red[0][0]);
   }
 }
 
@@ -331,7 +355,24 @@ __global__ __launch_bounds__(256) void attn_paged_join_k(const AttnPagedP p) {
   constexpr int E = HD >= 128 ? 2 : 1, U = 4;
   typedef float fE_t __attribute__((ext_vector_type(E)));
   const int lane = threadIdx.x & 63, hk = blockIdx.y, b = blockIdx.z;
-  const int r = blockIdx.x * 4 + (threadIdx.x >> 6), n = p.n_split;
+  const int n = p.n_split;
+  if ((int)blockIdx.x >= p.join_blocks) {            // split form with received weights: the other workgroups take 256 tokens each
+    __shared__ float l2s[SP_ROWS];
+    const SeqInfo s = seq_info(p, b);
+    const int R = min(min(s.nq, p.max_q) * p.G, SP_ROWS), j = ((int)blockIdx.x - p.join_blocks) * 256 + threadIdx.x, t = threadIdx.x;
+    if (t < R) {
+      const float* part = p.part + (((int64_t)b * p.c.n_kv_heads + hk) * p.s_rows + t) * n * (HD + 4);
+      float m = -INFINITY, l = 0.f;
+      for (int k = 0; k < n; ++k) m = fmaxf(m, part[(int64_t)k * (HD + 4)]);
+      const float base = m == -INFINITY ? 0.f : m;
+      for (int k = 0; k < n; ++k) l += fast_exp2(part[(int64_t)k * (HD + 4)] - base) * part[(int64_t)k * (HD + 4) + 1];
+      l2s[t] = !(l == 0.f) && phys_row(p, s.p0 + t / p.G) >= 0 ? m + log2f(l) : -INFINITY;
+    }
+    __syncthreads();
+    if (j < min(s.len, min(p.w_cols, p.s_ld))) count(p, s, b, hk, R, j, l2s);
+    return;
+  }
+  const int r = blockIdx.x * 4 + (threadIdx.x >> 6);
   const int64_t slot = ((int64_t)b * p.c.n_kv_heads + hk) * p.s_rows + min(r, p.s_rows - 1);
   const float* part = p.part + slot * n * (HD + 4);
   const int d = min(lane * E, HD - E);
@@ -373,29 +414,7 @@ __global__ __launch_bounds__(256) void attn_paged_join_k(const AttnPagedP p) {
 #pragma unroll
     for (int e = 0; e < E; ++e) p.out[prow * p.ldo + h * HD + d + e] = some ? f2bf(o[e] * inv) : (unsigned short)0;
   }
-  if (lane == 0) {
-    p.lse[h * p.ld_lse + s.p0 + i] = l2 * LN2;
-    if (p.s_ws) p.l2_ws[slot] = l2;
-  }
-}
-
-// received weights from the scores that the split form left behind: one thread per token, the query rows in their order
-__global__ __launch_bounds__(256) void attn_paged_count_k(const AttnPagedP p) {
-  const int j = blockIdx.x * 256 + threadIdx.x, hk = blockIdx.y, b = blockIdx.z;
-  const SeqInfo s = seq_info(p, b);
-  if (j >= min(s.len, min(p.w_cols, p.s_ld))) return;
-  const int64_t slot0 = ((int64_t)b * p.c.n_kv_heads + hk) * p.s_rows;
-  const int R = min(s.nq, p.max_q) * p.G;
-  float sum = 0.f;
-  // the first row of a query that sees the token: its scores, and those of all later rows, were stored by the wave that walked the block
-  // (max_q bounds it before the product: R fits 32 bits, the number of rows behind a long sample need not). A page that is not there: nothing.
-  const int first = page_ok(p.c.table[b * p.c.ld_table + (j >> p.c.shift)], p.c.n_pages) ? min(max(0, j - (s.len - s.nq)), p.max_q) * p.G : R;
-  for (int r = first; r < R; ++r) {
-    const float l2 = p.l2_ws[slot0 + r];
-    if (l2 == -INFINITY) continue;
-    sum += fast_exp2(p.s_ws[(slot0 + r) * p.s_ld + j] - l2);
-  }
-  p.w_out[b * p.ldwo_seq + hk * p.ldwo_head + j] = p.w_in[b * p.ldw_seq + hk * p.ldw_head + j] + sum;
+  if (lane == 0) p.lse[h * p.ld_lse + s.p0 + i] = l2 * LN2;
 }
 
 }  // namespace
@@ -429,7 +448,7 @@ int fill(const vm_attn_paged_args* a, AttnPagedP& p) {
 }
 
 // ----------------------------------------------------------------------------- which form, and its workspace
-struct Plan { bool split; int64_t part, s_ws, l2_ws, bytes; };
+struct Plan { bool split; int64_t part, s_ws, bytes; };
 
 Plan plan(AttnPagedP& p, int hd) {
   Plan a = {};
@@ -438,7 +457,8 @@ Plan plan(AttnPagedP& p, int hd) {
   // over 2086 tokens 34 us beside 37 us (two row tiles a workgroup), 17 x 4 heads over 8704 28 beside 45, 64 queries 38 beside 53.
   a.split = rows <= SP_ROWS;
   p.n_split = 1; p.s_rows = (int)rows; p.s_ld = (p.max_kv + 31) / 32 * 32;
-  p.part = p.s_ws = p.l2_ws = nullptr;
+  p.part = p.s_ws = nullptr;
+  p.join_blocks = (int)((rows + 3) / 4);
   p.n_tiles = p.n_wg = 0;
   if (rows == 0 || heads == 0) return a;
   if (!a.split) {
@@ -456,7 +476,7 @@ Plan plan(AttnPagedP& p, int hd) {
   if (p.n_split < 1) p.n_split = 1;
   int64_t at = 0;
   if (p.n_split > 1) { a.part = at; at += heads * rows * p.n_split * (hd + 4) * 4; }
-  if (p.w_out) { a.s_ws = at; at += heads * rows * p.s_ld * 4; a.l2_ws = at; at += (heads * rows * 4 + 15) / 16 * 16; }
+  if (p.w_out) { a.s_ws = at; at += heads * rows * p.s_ld * 4; }
   a.bytes = at;
   return a;
 }
@@ -464,8 +484,8 @@ Plan plan(AttnPagedP& p, int hd) {
 template <int HD>
 void launch_split(const AttnPagedP& p, hipStream_t st) {
   hipLaunchKernelGGL(attn_paged_split_k<HD>, dim3(p.n_split, p.c.n_kv_heads, p.n_seq), dim3(SP_WAVES * 64), 0, st, p);
-  if (p.n_split > 1) hipLaunchKernelGGL(attn_paged_join_k<HD>, dim3((p.s_rows + 3) / 4, p.c.n_kv_heads, p.n_seq), dim3(256), 0, st, p);
-  if (p.w_out && p.max_kv > 0) hipLaunchKernelGGL(attn_paged_count_k, dim3((p.max_kv + 255) / 256, p.c.n_kv_heads, p.n_seq), dim3(256), 0, st, p);
+  const int count_blocks = p.w_out ? (p.max_kv + 255) / 256 : 0;
+  if (p.n_split > 1) hipLaunchKernelGGL(attn_paged_join_k<HD>, dim3(p.join_blocks + count_blocks, p.c.n_kv_heads, p.n_seq), dim3(256), 0, st, p);
 }
 
 // workgroups of the tile form: eight XCDs, each as many as the longest piece of the list (tile_k: whole caches where the list is short)
@@ -489,7 +509,7 @@ int launch_tile(AttnPagedP& p, hipStream_t st) {
   static std::atomic<uint64_t> set{0};
   if (!allow_lds((const void*)apt::tile_k<HD>, apt::RING_LDS, set)) return VM_ERR_LAUNCH;
   hipLaunchKernelGGL(apt::tile_k<HD>, dim3((unsigned)tile_grid(p)), dim3(apt::NW * 64), apt::RING_LDS, st, p);
-  if (p.n_split > 1) hipLaunchKernelGGL(attn_paged_join_k<HD>, dim3((p.s_rows + 3) / 4, p.c.n_kv_heads, p.n_seq), dim3(256), 0, st, p);
+  if (p.n_split > 1) hipLaunchKernelGGL(attn_paged_join_k<HD>, dim3(p.join_blocks, p.c.n_kv_heads, p.n_seq), dim3(256), 0, st, p);
   VM_LAUNCH_CHECK();
   return p.w_out && p.max_kv > 0 ? launch_weigh<HD>(p, st) : VM_OK;
 }
@@ -519,7 +539,7 @@ int vm_attn_paged_bf16(const vm_attn_paged_args* args_host, void* stream) {
   char* ws = (char*)args_host->workspace;
   if (a.split && p.max_q > 0) {
     if (p.n_split > 1) p.part = (float*)(ws + a.part);
-    if (p.w_out) { p.s_ws = (float*)(ws + a.s_ws); p.l2_ws = (float*)(ws + a.l2_ws); }
+    if (p.w_out) { p.s_ws = (float*)(ws + a.s_ws); }
     if (hd == 128) launch_split<128>(p, st);
     else if (hd == 64) launch_split<64>(p, st);
     else launch_split<32>(p, st);

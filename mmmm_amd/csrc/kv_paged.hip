@@ -96,6 +96,7 @@ struct EvictP {
   const int32_t* lens; int32_t* new_lens;
   const int32_t* new_table; int64_t ld_new; int new_pages;
   int32_t* kept; int budget, recent, lds_keys;
+  int move_here, log_chunks;  // small budgets: kv_evict_select_k moves the rows itself; log2 of the 16-byte pieces of a row
   PagedKV c;
 };
 
@@ -130,11 +131,26 @@ __device__ __forceinline__ uint2 block_scan2(uint2 v, uint2 (*ws)[EV_WAVES], uin
   return {before.x + x.x - v.x, before.y + x.y - v.y};
 }
 
+// 16 bytes of the row that becomes token j from old token i, K and V, at element e of the row
+__device__ __forceinline__ void evict_move(const EvictP& p, int hk, int b, int j, int i, int e, int head_dim) {
+  if ((j >> p.c.shift) >= p.new_pages) return;
+  const int src = p.c.table[b * p.c.ld_table + (i >> p.c.shift)], dst = p.new_table[b * p.ld_new + (j >> p.c.shift)];
+  if (!page_ok(src, p.c.n_pages) || !page_ok(dst, p.c.n_pages)) return;
+  const int64_t s = page_row(src, p.c.ld_page, hk, i & p.c.mask, p.c.shift, head_dim) + e, d = page_row(dst, p.c.ld_page, hk, j & p.c.mask, p.c.shift, head_dim) + e;
+  if (s == d) return;
+  const u16x8_t kv = *reinterpret_cast<const u16x8_t*>(p.c.k + s), vv = *reinterpret_cast<const u16x8_t*>(p.c.v + s);
+  *reinterpret_cast<u16x8_t*>(const_cast<unsigned short*>(p.c.k) + d) = kv;
+  *reinterpret_cast<u16x8_t*>(const_cast<unsigned short*>(p.c.v) + d) = vv;
+}
+
+constexpr int EV_MOVE = 128;                      // the most rows that kv_evict_select_k moves itself
+
 __global__ __launch_bounds__(EV_THREADS) void kv_evict_select_k(const EvictP p) {
   extern __shared__ unsigned keys[];              // min(n, EV_LDS_KEYS) of them
   __shared__ unsigned hist[2048];
   __shared__ unsigned found[2];
   __shared__ uint2 ws[EV_WAVES];
+  __shared__ int stay[EV_MOVE];
   const int hk = blockIdx.x, b = blockIdx.y, tid = threadIdx.x;
   const int cap = (int)min((int64_t)p.c.max_pages << p.c.shift, (int64_t)p.w_cols);
   const int n = max(0, min(p.lens[b], cap));
@@ -198,6 +214,7 @@ __global__ __launch_bounds__(EV_THREADS) void kv_evict_select_k(const EvictP p) 
       if (key > prefix || (tie && eq < (unsigned)want)) {
         kept[at] = j;
         wn[at] = w[j];
+        if (p.move_here) stay[at] = j;
         ++at;
       }
       eq += tie;
@@ -206,6 +223,13 @@ __global__ __launch_bounds__(EV_THREADS) void kv_evict_select_k(const EvictP p) 
   for (int j = keep + tid; j < p.budget; j += EV_THREADS) kept[j] = -1;
   for (int j = keep + tid; j < p.w_cols; j += EV_THREADS) wn[j] = 0.f;      // the next tokens of this sample start at zero
   if (hk == 0 && tid == 0) p.new_lens[b] = keep;
+  if (p.move_here) {
+    __syncthreads();
+    for (int x = tid; x < keep << p.log_chunks; x += EV_THREADS) {
+      const int j = x >> p.log_chunks;
+      evict_move(p, hk, b, j, stay[j], (x & ((1 << p.log_chunks) - 1)) * 8, 8 << p.log_chunks);
+    }
+  }
 }
 
 // the rows that stay, K and V, into the sample's new pages: HD / 8 lanes per row, 16 bytes each
@@ -216,14 +240,7 @@ __global__ __launch_bounds__(256) void kv_evict_move_k(const EvictP p) {
   const int j = blockIdx.x * RPB + threadIdx.x / LPR, e = (threadIdx.x & (LPR - 1)) * 8;
   if (j >= p.budget) return;
   const int i = p.kept[((int64_t)b * p.c.n_kv_heads + hk) * p.budget + j];
-  if (i < 0 || (j >> p.c.shift) >= p.new_pages) return;
-  const int src = p.c.table[b * p.c.ld_table + (i >> p.c.shift)], dst = p.new_table[b * p.ld_new + (j >> p.c.shift)];
-  if (!page_ok(src, p.c.n_pages) || !page_ok(dst, p.c.n_pages)) return;
-  const int64_t s = page_row(src, p.c.ld_page, hk, i & p.c.mask, p.c.shift, HD) + e, d = page_row(dst, p.c.ld_page, hk, j & p.c.mask, p.c.shift, HD) + e;
-  if (s == d) return;
-  const u16x8_t kv = *reinterpret_cast<const u16x8_t*>(p.c.k + s), vv = *reinterpret_cast<const u16x8_t*>(p.c.v + s);
-  *reinterpret_cast<u16x8_t*>(const_cast<unsigned short*>(p.c.k) + d) = kv;
-  *reinterpret_cast<u16x8_t*>(const_cast<unsigned short*>(p.c.v) + d) = vv;
+  if (i >= 0) evict_move(p, hk, b, j, i, e, HD);
 }
 
 }  // namespace
@@ -278,8 +295,11 @@ int vm_kv_evict_paged_bf16(const vm_paged_kv* cache_host, const float* weights, 
   static std::atomic<uint64_t> set{0};
   if (!allow_lds((const void*)kv_evict_select_k, EV_LDS_KEYS * 4, set)) return VM_ERR_LAUNCH;
   p.lds_keys = cols < EV_LDS_KEYS ? cols : EV_LDS_KEYS;
+  p.log_chunks = cache_host->head_dim == 128 ? 4 : cache_host->head_dim == 64 ? 3 : 2;
+  p.move_here = budget <= EV_MOVE;
   hipLaunchKernelGGL(kv_evict_select_k, dim3(p.c.n_kv_heads, cache_host->n_seq), dim3(EV_THREADS), p.lds_keys * 4, st, p);
   VM_LAUNCH_CHECK();
+  if (p.move_here) return VM_OK;
   const int hd = cache_host->head_dim, rpb = 256 / (hd / 8);
   const dim3 grid((budget + rpb - 1) / rpb, p.c.n_kv_heads, cache_host->n_seq);
   if (hd == 128) hipLaunchKernelGGL(kv_evict_move_k<128>, grid, dim3(256), 0, st, p);

@@ -508,3 +508,16 @@ def test_an_empty_batch(dev, K):
     o, lse = K.attn_paged(q, k, v, t, i32([0], dev), none, 0.1, 0, 0, weights=w)
     nw, nl, kept = K.kv_evict_paged(k, v, w, t, none, t.clone(), 8, 2)
     assert o.shape == (0, 256) and lse.shape == (4, 0) and nw.shape == w.shape and nl.shape == (0,) and kept.shape == (0, 2, 8)
+
+
+@pytest.mark.parametrize('new', [[0, 2, 0], [0, 0, 40], [0, 0, 0]])
+@pytest.mark.parametrize('lens', [[30, 60, 7], [700, 2000, 90]])
+def test_samples_without_new_tokens_keep_their_weights(dev, K, new, lens):
+    lens = [max(n, L) for n, L in zip(new, lens)]
+    run_attention(K, dev, new, lens, 4, 2, 64, 16, weights=True)
+
+
+@pytest.mark.parametrize('L,B', [(40, 8), (511, 8), (1200, 40)])
+def test_weights_of_single_tokens_of_many_heads(dev, K, L, B):
+    """one workgroup per cache: the received weights come from the same launch"""
+    run_attention(K, dev, [1 + b % 2 for b in range(B)], [max(2, L - 3 * b) for b in range(B)], 32, 16, 32, 64, weights=True, packed=True)
