@@ -499,7 +499,14 @@ int launch_weigh(AttnPagedP& p, hipStream_t st) {
   p.w_blocks = (p.max_kv + 127) / 128;
   const int64_t caches = ((int64_t)p.n_seq * p.c.n_kv_heads + 7) / 8 * 8;
   if (caches * p.w_blocks > 0x7FFFFF00) return VM_ERR_UNSUPPORTED;
-  hipLaunchKernelGGL(apt::weigh_k<HD>, dim3((unsigned)(caches * p.w_blocks)), dim3(256), 0, st, p);
+  // four sets of waves per workgroup take a CU's LDS: where the workgroups do not even fill the chip once
+  if (caches * p.w_blocks <= 256 && (int64_t)p.max_q * p.G > 128) {
+    static std::atomic<uint64_t> set{0};
+    if (!allow_lds((const void*)apt::weigh_k<HD, 4>, 4 * sizeof(apt::WeighLds), set)) return VM_ERR_LAUNCH;
+    hipLaunchKernelGGL((apt::weigh_k<HD, 4>), dim3((unsigned)(caches * p.w_blocks)), dim3(1024), 4 * sizeof(apt::WeighLds), st, p);
+  } else {
+    hipLaunchKernelGGL((apt::weigh_k<HD, 1>), dim3((unsigned)(caches * p.w_blocks)), dim3(256), sizeof(apt::WeighLds), st, p);
+  }
   VM_LAUNCH_CHECK();
   return VM_OK;
 }

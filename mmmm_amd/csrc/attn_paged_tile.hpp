@@ -436,15 +436,24 @@ __global__ __launch_bounds__(NW * 64, 2) void tile_k(const AttnPagedP p) {
 // rows is in-lane — per tile first, then onto the running sum, halves last: a fixed order. Row numbers and lse are fetched two tiles ahead, the
 // rows one tile ahead through registers. Bound by the exponentials: 32 x (16 + 8) cycles per 64 x 32 tile beside 512 of the matrix pipe.
 // (The first form had the rows straight from memory as B operands of each wave: 60 us on 8 x 456, bound by the L1's line rate.)
-template <int HD>
-__global__ __launch_bounds__(256, 4) void weigh_k(const AttnPagedP p) {
+// Few caches with many query rows (grouped heads) leave most CUs idle: there a workgroup has four such sets of four waves, each with every fourth
+// tile of rows, and their sums meet in LDS, in order (5 x 433 tokens, 4 heads per kv head of 3, width 32: with the attention 50 -> 34 us; 4 x 2000, 8 heads for one, width 128: 369 -> 229; from 500 workgroups on
+// it gains nothing)..
+struct WeighLds {
+  char q[2][TILE];
+  float l2[3][64];
+  int lim[3][64];
+  int64_t off[3][64];                                              // element offset of the row's query (no such row: 0, any query)
+  int gap[4];                                                      // one of the tile's rows is no row
+};
+
+template <int HD, int SETS>
+__global__ __launch_bounds__(256 * SETS, 4) void weigh_k(const AttnPagedP p) {
   constexpr int KS = HD / 16, CPR = HD / 8, NQ = CPR / 4;          // 16-byte chunks per row, chunks per thread and tile
-  __shared__ __attribute__((aligned(16))) char qbuf[2][TILE];
-  __shared__ __attribute__((aligned(16))) float s_l2[3][64];
-  __shared__ __attribute__((aligned(16))) int s_lim[3][64];
-  __shared__ int64_t s_off[3][64];                                 // element offset of the row's query (no such row: 0, any query)
-  __shared__ int s_gap[3];                                         // one of the tile's rows is no row
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), hf = lane >> 5;
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  const int set = SETS == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 8);
+  WeighLds& L = reinterpret_cast<WeighLds*>(smem)[set];
+  const int tid = threadIdx.x & 255, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), hf = lane >> 5;
   // 128 tokens of one cache. The blocks of a cache differ in work (early tokens are seen by more rows) and share its queries: every XCD takes whole
   // caches where there are enough of them (blocks dealt out in order would give one XCD the early blocks of all: 8 x 456 with the attention 69 beside 68 us).
   int blk, hs;
@@ -473,7 +482,8 @@ __global__ __launch_bounds__(256, 4) void weigh_k(const AttnPagedP p) {
   const float sc = p.scale * LOG2E;
   float sum = 0.f;
   const int rs = min(max(0, jw - past), p.max_q) * p.G / 64 * 64;                // the first tile with a row that sees one of these tokens
-  const int tiles = R > rs ? (R - rs + 63) / 64 : 0;
+  const int tiles = R > rs ? (R - rs + 63) / 64 : 0, mine = (tiles - set + SETS - 1) / SETS, steps = (tiles + SETS - 1) / SETS;
+  auto row0 = [&](int u) { return rs + 64 * (set + SETS * u); };    // of this set's u-th tile
   struct Info { int r, i, h, row; float lse; };                    // as loaded: looked at when it is put into LDS, a tile later
   auto info = [&](int r) -> Info {
     Info x;
@@ -488,18 +498,18 @@ __global__ __launch_bounds__(256, 4) void weigh_k(const AttnPagedP p) {
   };
   auto put = [&](int slot, const Info& x) {
     const bool ok = x.r < R && (unsigned)x.row < (unsigned)p.n_rows && x.lse != -INFINITY;
-    s_off[slot][tid] = ok ? x.row * p.ldq + x.h * HD : 0;
-    s_l2[slot][tid] = ok ? x.lse * LOG2E : INFINITY;               // no such row: exp2(. - inf) = 0
-    s_lim[slot][tid] = ok ? past + x.i : -1;
+    L.off[slot][tid] = ok ? x.row * p.ldq + x.h * HD : 0;
+    L.l2[slot][tid] = ok ? x.lse * LOG2E : INFINITY;               // no such row: exp2(. - inf) = 0
+    L.lim[slot][tid] = ok ? past + x.i : -1;
     const bool gap = __builtin_amdgcn_ballot_w64(!ok) != 0;
-    if (tid == 0) s_gap[slot] = gap;
+    if (tid == 0) L.gap[slot] = gap;
   };
   i32x4_t qv[NQ];
   auto load_q = [&](int slot) {
 #pragma unroll
     for (int i = 0; i < NQ; ++i) {
       const int c = tid + 256 * i;
-      qv[i] = *reinterpret_cast<const i32x4_t*>(p.q + s_off[slot][c / CPR] + (c % CPR) * 8);
+      qv[i] = *reinterpret_cast<const i32x4_t*>(p.q + L.off[slot][c / CPR] + (c % CPR) * 8);
     }
   };
   auto store_q = [&](char* tile) {
@@ -511,13 +521,13 @@ __global__ __launch_bounds__(256, 4) void weigh_k(const AttnPagedP p) {
   };
   if (tiles > 0) {
     if (tid < 64) {
-      const Info a = info(rs + tid), c = info(rs + 64 + tid);
+      const Info a = info(row0(0) + tid), c = info(row0(1) + tid);
       put(0, a);
       put(1, c);
     }
     __syncthreads();
     load_q(0);
-    store_q(qbuf[0]);
+    store_q(L.q[0]);
     __syncthreads();
   }
   const int rb0 = a32::row_base(lane, 0), rb1 = a32::row_base(lane, 1);
@@ -532,9 +542,9 @@ __global__ __launch_bounds__(256, 4) void weigh_k(const AttnPagedP p) {
 #pragma unroll
       for (int g4 = 0; g4 < 4; ++g4) {
         const int row = 32 * rt + 8 * g4 + 4 * hf;
-        const f32x4_t l2 = *reinterpret_cast<const f32x4_t*>(&s_l2[slot][row]);
+        const f32x4_t l2 = *reinterpret_cast<const f32x4_t*>(&L.l2[slot][row]);
         i32x4_t lim;
-        if constexpr (decltype(edge)::value) lim = *reinterpret_cast<const i32x4_t*>(&s_lim[slot][row]);
+        if constexpr (decltype(edge)::value) lim = *reinterpret_cast<const i32x4_t*>(&L.lim[slot][row]);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const float x = fast_exp2(fmaf(acc[4 * g4 + e], sc, -l2[e]));
@@ -548,25 +558,33 @@ __global__ __launch_bounds__(256, 4) void weigh_k(const AttnPagedP p) {
 #pragma unroll
   for (int k = 0; k < KS; ++k) asm volatile("" : "+v"(kf[k]));       // they are here: no wait for them in the loop, which would be one for the rows too
   int slot = 0;
-  for (int u = 0; u < tiles; ++u) {
+  for (int u = 0; u < steps; ++u) {
     const int next = slot == 2 ? 0 : slot + 1, third = next == 2 ? 0 : next + 1;
     Info ahead;
-    if (tid < 64) ahead = info(rs + 64 * (u + 2) + tid);
-    if (u + 1 < tiles) load_q(next);
-    const char* qt = qbuf[u & 1];
-    const int r_last = min(rs + 64 * u + 63, R - 1);
-    if (past + r_last / p.G >= j0) {
-      if (s_gap[slot] || past + (rs + 64 * u) / p.G < j0 + 31) add(qt, slot, std::true_type{});
+    if (tid < 64) ahead = info(row0(u + 2) + tid);
+    if (u + 1 < mine) load_q(next);
+    const char* qt = L.q[u & 1];
+    const int r_last = min(row0(u) + 63, R - 1);
+    if (u < mine && past + r_last / p.G >= j0) {
+      if (L.gap[slot] || past + row0(u) / p.G < j0 + 31) add(qt, slot, std::true_type{});
       else add(qt, slot, std::false_type{});
     }
-    if (u + 1 < tiles) store_q(qbuf[(u + 1) & 1]);
+    if (u + 1 < mine) store_q(L.q[(u + 1) & 1]);
     if (tid < 64) put(third, ahead);
     __syncthreads();
     slot = next;
   }
   float a = sum, c = sum;
   a32::swap_halves(a, c);
-  if (hf == 0 && j < n) p.w_out[b * p.ldwo_seq + hk * p.ldwo_head + j] = p.w_in[b * p.ldw_seq + hk * p.ldw_head + j] + (there ? a + c : 0.f);
+  a += c;
+  if constexpr (SETS > 1) {
+    float* const all = reinterpret_cast<float*>(L.q);               // (the last barrier is behind the last read)
+    if (hf == 0) all[tid >> 6 << 5 | (lane & 31)] = a;
+    __syncthreads();
+    if (set > 0) return;
+    for (int i = 1; i < SETS; ++i) a += reinterpret_cast<const float*>(reinterpret_cast<WeighLds*>(smem)[i].q)[tid >> 6 << 5 | (lane & 31)];
+  }
+  if (hf == 0 && j < n) p.w_out[b * p.ldwo_seq + hk * p.ldwo_head + j] = p.w_in[b * p.ldw_seq + hk * p.ldw_head + j] + (there ? a : 0.f);
 }
 
 }  // namespace apt

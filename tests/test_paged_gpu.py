@@ -521,3 +521,9 @@ def test_samples_without_new_tokens_keep_their_weights(dev, K, new, lens):
 def test_weights_of_single_tokens_of_many_heads(dev, K, L, B):
     """one workgroup per cache: the received weights come from the same launch"""
     run_attention(K, dev, [1 + b % 2 for b in range(B)], [max(2, L - 3 * b) for b in range(B)], 32, 16, 32, 64, weights=True, packed=True)
+
+
+def test_weights_of_chunks_of_many_heads(dev, K):
+    """more blocks of tokens than CUs: one set of waves each"""
+    run_attention(K, dev, [150, 200, 129, 1, 70, 200], [333, 200, 300, 280, 270, 257], 16, 16, 64, 32, weights=True, packed=True)
+    run_attention(K, dev, [300, 40], [300, 130], 64, 64, 32, 64, weights=True)
