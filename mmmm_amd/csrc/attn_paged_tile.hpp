@@ -11,6 +11,10 @@
 //    (scores at -inf, a base of 0 while the maximum is -inf);
 //  * with fewer than one workgroup per CU the keys are split over workgroups too (partial results joined by attn_paged_join_k);
 //  * V^T fragments are read in two assembly statements of 16 ds_read_b64_tr_b16 that end in their own wait.
+// Matrix-bound in theory (4 hd operations per visible pair), in fact by the softmax between the two products and the barriers between the clusters:
+// 4 x 4609 tokens, 32 heads of width 128: 577 us, 820 TFLOP/s of the visible pairs, matrix pipes busy 0.39 of the time, waves waiting 0.34 of
+// theirs; 512 tokens over 8704: 95 us with the join, 750 TFLOP/s. Measured and not taken: 64 rows per wave and four waves (half the LDS reads, but the
+// registers of two row sets: 680 us); V read untransposed, which would be wrong, gains 3 % — its transposed reads are not what costs.
 #pragma once
 #include <type_traits>
 #include "attn32_tile.hpp"
@@ -434,11 +438,13 @@ __global__ __launch_bounds__(NW * 64, 2) void tile_k(const AttnPagedP p) {
 // keeping them would be 4 bytes per row and token). A wave keeps 32 tokens as B operands in registers (straight from the page) and the
 // workgroup's four waves walk the rows that see them, 64 at a time through LDS as A operands: a token sits on the lane, so its sum over the
 // rows is in-lane — per tile first, then onto the running sum, halves last: a fixed order. Row numbers and lse are fetched two tiles ahead, the
-// rows one tile ahead through registers. Bound by the exponentials: 32 x (16 + 8) cycles per 64 x 32 tile beside 512 of the matrix pipe.
-// (The first form had the rows straight from memory as B operands of each wave: 60 us on 8 x 456, bound by the L1's line rate.)
+// rows one tile ahead through registers. Bound by the latency of a tile (eight of them in a row for the earliest tokens of 456) and the vector work
+// on the scores beside it: 8 x 456 tokens, 32 heads of width 128: 22 us (34 us at three workgroups per CU with the rows waited for in front of the
+// products; 60 us with the rows straight from memory as B operands of each wave, bound by the L1's line rate).
 // Few caches with many query rows (grouped heads) leave most CUs idle: there a workgroup has four such sets of four waves, each with every fourth
-// tile of rows, and their sums meet in LDS, in order (5 x 433 tokens, 4 heads per kv head of 3, width 32: with the attention 50 -> 34 us; 4 x 2000, 8 heads for one, width 128: 369 -> 229; from 500 workgroups on
-// it gains nothing)..
+// tile of rows, and their sums meet in LDS, in order (5 x 433 tokens, 4 heads per kv head of 3, width 32: with the attention 50 -> 34 us;
+// 4 x 2000, 8 heads for one, width 128: 369 -> 229; from 500 workgroups on
+// it gains nothing).
 struct WeighLds {
   char q[2][TILE];
   float l2[3][64];
