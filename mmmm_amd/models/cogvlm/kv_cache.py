@@ -123,9 +123,11 @@ class PagedKVCache:
         n = -(-tokens // self.page_size)
         return [self._free.pop() for _ in range(n)]
 
-    def _upload(self, pages: list[list[int]], table: torch.Tensor):
-        if table.is_cuda and torch.cuda.is_current_stream_capturing():
+    def _not_captured(self):
+        if self.block_table.is_cuda and torch.cuda.is_current_stream_capturing():
             raise RuntimeError('the block table changes inside a captured step: reserve() the pages first')
+
+    def _upload(self, pages: list[list[int]], table: torch.Tensor):
         host = torch.full(tuple(table.shape), -1, dtype=torch.int32)
         for b, p in enumerate(pages):
             host[b, :len(p)] = torch.tensor(p, dtype=torch.int32)
@@ -140,6 +142,7 @@ class PagedKVCache:
         if short > len(self._free):
             raise ValueError(f'KV cache overflow: {short} pages wanted, {len(self._free)} free')
         if short:
+            self._not_captured()
             for p in self._pages:
                 p.extend(self._take((want - len(p)) * self.page_size) if want > len(p) else [])
             self._upload(self._pages, self.block_table)
@@ -207,6 +210,7 @@ class PagedKVCache:
         need = -(-left // self.page_size) * self.batch
         if need > len(self._free):
             raise ValueError(f'KV cache overflow: eviction to {budget} tokens wants {need} pages, {len(self._free)} free')
+        self._not_captured()
         pages = [self._take(left) for _ in range(self.batch)]
         table = torch.full_like(self.block_table, -1)
         self._upload(pages, table)

@@ -1,5 +1,9 @@
 """Paged-cache operators on the MI355X against their 64-bit statements (tests/_paged.py), elementwise, with tolerances that count the
 roundings. Rows of the pools that hold no token are NaN throughout: nothing may read them as data."""
+import subprocess
+import sys
+from pathlib import Path
+
 import pytest
 import torch
 
@@ -527,3 +531,49 @@ def test_weights_of_chunks_of_many_heads(dev, K):
     """more blocks of tokens than CUs: one set of waves each"""
     run_attention(K, dev, [150, 200, 129, 1, 70, 200], [333, 200, 300, 280, 270, 257], 16, 16, 64, 32, weights=True, packed=True)
     run_attention(K, dev, [300, 40], [300, 130], 64, 64, 32, 64, weights=True)
+
+
+def test_no_pages_change_hands_inside_a_capture(dev, K):
+    from mmmm_amd.models.cogvlm.kv_cache import PagedKVCache
+    cache = PagedKVCache(1, 2, 256, 2, 64, dev, page_size=16, n_pages=64, track_weights=True)
+    cache.reserve(40)
+    cache.len_bound = 40
+    free, table = cache.free_pages, cache.block_table.clone()
+    x = torch.zeros(4, device=dev)
+    for call in (lambda: cache.reserve(100), lambda: cache.evict(8, 2)):
+        with pytest.raises(RuntimeError, match='captured'):
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                x.add_(1)
+                call()
+        assert cache.free_pages == free and torch.equal(cache.block_table, table)
+
+
+FIRST_CALL = """
+import torch
+from mmmm_amd import kernels as K
+dev = torch.device('cuda', 0)
+g = torch.Generator().manual_seed(0)
+k, v = (torch.randn(16, 2, 64, 128, generator=g).bfloat16().to(dev) for _ in range(2))
+t = torch.arange(14, dtype=torch.int32, device=dev).view(2, 7)
+nt = t.flip(1).contiguous() + 2
+q = torch.randn(400, 4 * 128, generator=g).bfloat16().to(dev)
+cu, lens = torch.tensor([0, 300, 400], dtype=torch.int32, device=dev), torch.tensor([430, 100], dtype=torch.int32, device=dev)
+w = torch.zeros(2, 2, 448, device=dev)
+call = lambda: (K.attn_paged(q, k, v, t, cu, lens, 0.1, 300, 430, weights=w, weights_out=w.clone()), K.kv_evict_paged(k.clone(), v.clone(), w + 1, t, lens, nt, 60, 4))
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    a, b = call()
+for _ in range(3):
+    graph.replay()
+    torch.cuda.synchronize()
+    c, d = call()
+    assert all(torch.equal(x, y) for x, y in zip(a + b, c + d))
+print('equal')
+"""
+
+
+def test_first_call_inside_a_capture():
+    """a process whose first calls are captured: the kernels' attributes are set there"""
+    r = subprocess.run([sys.executable, '-c', FIRST_CALL], cwd=Path(__file__).resolve().parents[1], capture_output=True, text=True, timeout=100)
+    assert r.returncode == 0 and 'equal' in r.stdout, r.stderr[-2000:]
