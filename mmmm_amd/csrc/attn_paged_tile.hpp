@@ -4,7 +4,7 @@
 // clusters per 64-key tile between raw barriers, the two waves of a SIMD one cluster apart; K and V by LDS-DMA into three-slot rings retired
 // by counted vmcnt). What the cache changes:
 //  * a 64-key tile may lie in up to four pages. The unit of the DMA is the 8-row group a wave stages: it never crosses a page (page size
-//    >= 16), its page number is one scalar load, fetched a tile ahead, and the buffer descriptor is made for exactly that group — base in 64
+//    >= 16), its page number is one scalar load, fetched two tiles ahead, and the buffer descriptor is made for exactly that group — base in 64
 //    bits, extent = the rows that exist — so rows behind the last token and pages that are not there arrive as zeros without a compare;
 //  * rows are (query, head of the group) pairs: grouped heads fill the tile together and read K and V once;
 //  * the causal limit of a row is any token, not its own position: the last two tiles of a wave may need the mask, and a row may see nothing
@@ -134,14 +134,19 @@ struct Stager {
       voff[i] = chunk * 8 < HD ? ((lane >> 2) & 7) * HD * 2 + chunk * 16 : 0x7FFFFFF0;
     }
   }
-  __device__ __forceinline__ void stage(const unsigned short* pool, const PagedKV& c, int page, int t, int kv_end, char* tile, int wave) const {
+  // where the wave's group of tile t lies in both pools, and how many bytes of it are there
+  struct Group { uint64_t at; int bytes; };
+  __device__ __forceinline__ Group group(const PagedKV& c, int page, int t, int kv_end, int wave) const {
     const int tok = 64 * t + 8 * wave;
     const bool ok = page_ok(page, c.n_pages);
-    const int there = max(0, min(8, kv_end - tok)), rows = ok ? there : 0, from = ok ? page : 0;      // selects, no branch
-    const uint64_t at = (uint64_t)(pool + (int64_t)from * c.ld_page + head + (int64_t)(tok & c.mask) * HD);
+    const int there = max(0, min(8, kv_end - tok)), rows = ok ? there : 0;      // selects, no branch
+    const uint64_t at = (uint64_t)(unsigned)(ok ? page : 0) * (uint64_t)c.ld_page + (uint64_t)head + (unsigned)((tok & c.mask) * HD);
+    return {at * 2, __builtin_amdgcn_readfirstlane(rows * HD * 2)};
+  }
+  __device__ __forceinline__ void stage(const unsigned short* pool, const Group& g, char* tile, int wave) const {
+    const uint64_t at = (uint64_t)pool + g.at;
     const unsigned lo = __builtin_amdgcn_readfirstlane((unsigned)at), hi = __builtin_amdgcn_readfirstlane((unsigned)(at >> 32));
-    const __amdgpu_buffer_rsrc_t rs =
-        __builtin_amdgcn_make_buffer_rsrc((void*)(((uint64_t)hi << 32) | lo), 0, __builtin_amdgcn_readfirstlane(rows * HD * 2), 0x00020000);
+    const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void*)(((uint64_t)hi << 32) | lo), 0, g.bytes, 0x00020000);
 #pragma unroll
     for (int i = 0; i < PW; ++i)
       __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_vptr_t)(tile + (2 * wave + i) * 1024), 16, voff[i], 0, 0, 0);
@@ -199,6 +204,10 @@ __global__ __launch_bounds__(NW * 64, 2) void tile_k(const AttnPagedP p) {
   const int t_w = wave_live && lim_hi >= 0 ? min(t1, lim_hi / 64 + 1) : t0;      // tiles [t0, t_w) are this wave's
   const bool late = wave >= NW / 2;
 
+  // the range's entries in the table, 64 of them at once: asked for here, looked at behind the first tiles' DMA
+  const int e0 = nt > 0 ? 64 * t0 >> p.c.shift : 0, e1 = nt > 0 ? (min(64 * t1, kv_end) - 1) >> p.c.shift : 0;
+  const int entry = p.c.table[b * p.c.ld_table + min(e0 + lane, e1)];
+
   bf16x8_t qf[KS];
 #pragma unroll
   for (int k = 0; k < KS; ++k) {
@@ -215,18 +224,10 @@ __global__ __launch_bounds__(NW * 64, 2) void tile_k(const AttnPagedP p) {
   int strange = 0x7FFFFFFF;                                        // first tile in which a value that is not finite was taken as zero
   float msc = -INFINITY, base = 0.f, l_run = 0.f;                  // running maximum (log2 domain), what is subtracted, this half's sum
 
+  const table_ptr table = table_of(p.c, b);
   if (nt > 0) {
-    const table_ptr table = table_of(p.c, b);
-    // page numbers of tile t as the table has them: of this wave's group and of the tile's four 16-key groups; read two tiles before the
-    // first use, so that the scalar loads are never waited for
-    struct Pages { int own, all[4]; };
-    auto pages_of = [&](int t) -> Pages {
-      Pages g;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) g.all[i] = table[__builtin_amdgcn_readfirstlane(min(64 * t + 16 * i, kv_end - 1) >> p.c.shift)];
-      g.own = table[__builtin_amdgcn_readfirstlane(min(64 * t + 8 * wave, kv_end - 1) >> p.c.shift)];
-      return g;
-    };
+    // the page of this wave's group of tile t, read two tiles before the first use, so that the scalar load is never waited for
+    auto page_of = [&](int t) -> int { return table_at(table, __builtin_amdgcn_readfirstlane(min(64 * t + 8 * wave, kv_end - 1) >> p.c.shift)); };
     char* const kring = smem;
     char* const vring = smem + NS * TILE;
     St st;
@@ -239,12 +240,16 @@ __global__ __launch_bounds__(NW * 64, 2) void tile_k(const AttnPagedP p) {
 #pragma unroll
       for (int k = 0; k < KS; ++k) asm volatile("" : "+v"(qf[k]));
     };
-    Pages pga = pages_of(t0), pgb = pages_of(t0 + 1), pgc = pages_of(t0 + 2);
-    st.stage(p.c.k, p.c, pga.own, t0, kv_end, kring, wave);
-    st.stage(p.c.v, p.c, pga.own, t0, kv_end, vring, wave);
+    const int pga = page_of(t0), pgb = page_of(t0 + 1);
+    int pgc = page_of(t0 + 2);
+    asm volatile("" : "+s"(pgc));                                  // (no page number is on its way into the loop: nothing there waits for one)
+    typename St::Group grp = st.group(p.c, pga, t0, kv_end, wave);
+    st.stage(p.c.k, grp, kring, wave);
+    st.stage(p.c.v, grp, vring, wave);
     if (nt > 1) {
-      st.stage(p.c.v, p.c, pgb.own, t0 + 1, kv_end, vring + TILE, wave);
-      st.stage(p.c.k, p.c, pgb.own, t0 + 1, kv_end, kring + TILE, wave);
+      grp = st.group(p.c, pgb, t0 + 1, kv_end, wave);
+      st.stage(p.c.v, grp, vring + TILE, wave);
+      st.stage(p.c.k, grp, kring + TILE, wave);
       arrived();
       cluster_end<3 * PW>();
     } else {
@@ -252,6 +257,9 @@ __global__ __launch_bounds__(NW * 64, 2) void tile_k(const AttnPagedP p) {
       cluster_end<0>();
     }
     if (late) cluster_end<-1>();
+    bool bad = !page_ok(entry, p.c.n_pages);
+    for (int i = e0 + 64 + lane; i <= e1; i += 64) bad |= !page_ok(p.c.table[b * p.c.ld_table + i], p.c.n_pages);
+    const bool gaps = __builtin_amdgcn_ballot_w64(bad) != 0;       // some page of the range is not there
     const char* const kb0 = kring + a32::row_base(lane, 0);
     const char* const kb1 = kring + a32::row_base(lane, 1);
     const unsigned vbA = (unsigned)(size_t)(vring + a32::tr_base(lane, 0)), vbB = (unsigned)(size_t)(vring + a32::tr_base(lane, 1));
@@ -262,7 +270,7 @@ __global__ __launch_bounds__(NW * 64, 2) void tile_k(const AttnPagedP p) {
       const int t = t0 + u;
       const bool on = t < t_w;
       const bool more1 = u + 1 < nt, more2 = u + 2 < nt;
-      const Pages pgd = pages_of(t + 3);
+      const int pgd = page_of(t + 3);                              // (here it arrives under the LDS reads, whose wait is its wait)
       // ---- c0: K fragments -> registers; DMA of V(u+2)
       if (on) {
 #pragma unroll
@@ -270,7 +278,10 @@ __global__ __launch_bounds__(NW * 64, 2) void tile_k(const AttnPagedP p) {
 #pragma unroll
           for (int ks = 0; ks < KS; ++ks) kv[kt * KS + ks] = a32::ld_row(((ks & 1) ? kb1 : kb0) + s0, 8192 * kt + 512 * (ks >> 1));
       }
-      if (more2) st.stage(p.c.v, p.c, pgc.own, t + 2, kv_end, vring + s2, wave);
+      if (more2) {
+        grp = st.group(p.c, pgc, t + 2, kv_end, wave);
+        st.stage(p.c.v, grp, vring + s2, wave);
+      }
       if (more2) cluster_end<3 * PW>(); else if (more1) cluster_end<2 * PW>(); else cluster_end<0>();
       // ---- c1: S^T = K Q^T; DMA of K(u+2)
       if (on) {
@@ -282,19 +293,24 @@ __global__ __launch_bounds__(NW * 64, 2) void tile_k(const AttnPagedP p) {
           S[kt] = acc;
         }
       }
-      if (more2) st.stage(p.c.k, p.c, pgc.own, t + 2, kv_end, kring + s2, wave);
+      if (more2) st.stage(p.c.k, grp, kring + s2, wave);
+      pgc = pgd;
       cluster_end<-1>();
       // ---- c2: V fragments -> registers, mask, maximum, rescale
       if (on) {
         ld_v<ND>(vbA + s0, vbB + s0, kv);
         const int kv0 = 64 * t;
-        const bool gap = !(page_ok(pga.all[0], p.c.n_pages) && page_ok(pga.all[1], p.c.n_pages) && page_ok(pga.all[2], p.c.n_pages) && page_ok(pga.all[3], p.c.n_pages));
-        if (__builtin_expect(kv0 + 63 > lim_lo || gap, 0)) {
+        if (__builtin_expect(kv0 + 63 > lim_lo || gaps, 0)) {
+          bool ok[4] = {true, true, true, true};                   // 16 keys of one page each
+          if (gaps) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) ok[i] = page_ok(table_at(table, __builtin_amdgcn_readfirstlane(min(kv0 + 16 * i, kv_end - 1) >> p.c.shift)), p.c.n_pages);
+          }
 #pragma unroll
           for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
-            for (int e = 0; e < 16; ++e)                           // accumulator rows 8 (e >> 2) ..: 16 keys of one page each half
-              S[kt][e] = page_ok(pga.all[2 * kt + (e >> 3)], p.c.n_pages) && kv0 + 32 * kt + acc_row(e, hf) <= lim ? S[kt][e] : -INFINITY;
+            for (int e = 0; e < 16; ++e)
+              S[kt][e] = ok[2 * kt + (e >> 3)] && kv0 + 32 * kt + acc_row(e, hf) <= lim ? S[kt][e] : -INFINITY;
           unsigned most = 0;
 #pragma unroll
           for (int i = 0; i < 4 * ND; ++i)
@@ -350,16 +366,12 @@ __global__ __launch_bounds__(NW * 64, 2) void tile_k(const AttnPagedP p) {
       }
       cluster_end<-1>();
       { const int x = s0; s0 = s1; s1 = s2; s2 = x; }
-      pga = pgb;
-      pgb = pgc;
-      pgc = pgd;
     }
     if (!late) cluster_end<-1>();                // every LDS read is over: the slabs may overlay the rings
   }
 
   if (!wave_live) return;
   if (__builtin_expect(strange < t_w, 0)) {
-    const table_ptr table = table_of(p.c, b);
     for (int j = 64 * strange; j < min(64 * t_w, kv_end); ++j) {
       const int page = table[__builtin_amdgcn_readfirstlane(j >> p.c.shift)];
       if (!page_ok(page, p.c.n_pages)) continue;

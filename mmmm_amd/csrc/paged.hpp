@@ -32,6 +32,9 @@ __device__ __forceinline__ int64_t page_row(int page, int64_t ld_page, int hk, i
 typedef const __attribute__((address_space(4))) int32_t* table_ptr;
 __device__ __forceinline__ table_ptr table_of(const PagedKV& c, int seq) { return (table_ptr)(uintptr_t)(c.table + (int64_t)seq * c.ld_table); }
 
+// (byte offset in 32 bits: one scalar load and no 64-bit address arithmetic; a sample's table is shorter than 2^29 bytes)
+__device__ __forceinline__ int table_at(table_ptr t, int i) { return *(table_ptr)((const __attribute__((address_space(4))) char*)t + (unsigned)i * 4u); }
+
 inline int paged_shift(int page_size) {          // log2 of a legal page size, -1 otherwise
   for (int s = 4; s <= 10; ++s)
     if (page_size == 1 << s) return s;

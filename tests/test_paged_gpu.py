@@ -577,3 +577,10 @@ def test_first_call_inside_a_capture():
     """a process whose first calls are captured: the kernels' attributes are set there"""
     r = subprocess.run([sys.executable, '-c', FIRST_CALL], cwd=Path(__file__).resolve().parents[1], capture_output=True, text=True, timeout=100)
     assert r.returncode == 0 and 'equal' in r.stdout, r.stderr[-2000:]
+
+
+@pytest.mark.parametrize('new', [1, 80, 300])
+def test_absent_pages_of_long_tables(dev, K, new):
+    """more than 64 pages per sample, one of the last ones missing; and a sample that has all of them beside it"""
+    run_attention(K, dev, [new, new], [3000, 1500], 2, 1, 64, 16, weights=True, absent=[(0, 100, -1), (0, 187, 10 ** 8)])
+    run_attention(K, dev, [new, new], [3000, 2100], 2, 2, 128, 32, absent=[(1, 65, -5)])
