@@ -230,9 +230,14 @@ _raw_stream = getattr(torch._C, '_cuda_getCurrentRawStream', None)
 def stream() -> int:
     """hipStream_t of torch's current stream on the current device. The raw accessor avoids building a torch.cuda.Stream
     object per launch (9 us of host time each, ~5k launches per training step)."""
+    return stream_of(torch.cuda.current_device())
+
+
+def stream_of(device: int) -> int:
+    """hipStream_t of torch's current stream on a device that is known to be the current one"""
     if _raw_stream is not None:
-        return _raw_stream(torch.cuda.current_device())
-    return torch.cuda.current_stream().cuda_stream
+        return _raw_stream(device)
+    return torch.cuda.current_stream(device).cuda_stream
 
 
 _STREAM_OBJ: dict = {}

@@ -844,11 +844,12 @@ def _paged(k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: torch.Tens
     return (k_pages.data_ptr(), v_pages.data_ptr(), ld, n, ps, block_table.data_ptr(), row if n_seq > 1 else cols, cols, n_seq, hk, hd), dev
 
 
-def _here(t: torch.Tensor, dev: int):
-    """the launch goes to the current device's stream: what it works on has to lie there"""
+def _here(t: torch.Tensor, dev: int) -> int:
+    """the current stream: the launch goes to the current device, what it works on has to lie there"""
     if dev < 0:
         ptr(t)                                          # raises: there is no CPU path
     assert dev == torch.cuda.current_device(), f'the cache lies on device {dev}, the current one is {torch.cuda.current_device()}'
+    return hip.stream_of(dev)
 
 
 def _i32(t: torch.Tensor, n: int, dev: int) -> int:
@@ -875,13 +876,13 @@ def kv_append_paged(qkv: torch.Tensor, row_seq: torch.Tensor, row_index: torch.T
     assert n_heads > 0 and cos.dtype == torch.float32 and sin.dtype == torch.float32 and cos.is_contiguous() and sin.is_contiguous()
     assert cos.shape == sin.shape and cos.dim() == 2 and cos.shape[1] == hd and cos.get_device() == dev and sin.get_device() == dev
     seq, idx, pos = _i32(row_seq, T, dev), _i32(row_index, T, dev), _i32(row_pos, T, dev)
-    _here(k_pages, dev)
+    here = _here(k_pages, dev)
     if q_out is None:
         q_out = qkv.new_empty((T, n_heads * hd))
     o, ldo = _rows(q_out, (T, n_heads * hd), dev)
     if T:
         hip.call('vm_kv_append_paged_bf16', hip.PAGED_KV.pack(*c), x, ldx, seq, idx, pos,
-                 cos.data_ptr(), sin.data_ptr(), cos.shape[0], T, n_heads, o, ldo, None if nrows is None else _i32(nrows, 1, dev), stream())
+                 cos.data_ptr(), sin.data_ptr(), cos.shape[0], T, n_heads, o, ldo, None if nrows is None else _i32(nrows, 1, dev), here)
     return q_out
 
 
@@ -932,12 +933,12 @@ def attn_paged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, bl
     w = wo = ws_ = wh = wos = woh = w_cols = 0
     if weights is not None:
         w, ws_, wh, w_cols = _weights_of(weights, n_seq, hk, dev)
-        wo, wos, woh, wo_cols = _weights_of(weights if weights_out is None else weights_out, n_seq, hk, dev)
+        wo, wos, woh, wo_cols = (w, ws_, wh, w_cols) if weights_out is None else _weights_of(weights_out, n_seq, hk, dev)
         assert wo_cols == w_cols and w_cols >= min(max_kv, cols * ps), f'{w_cols} columns of weights'
         assert n_seq <= 1 or wos != 0, 'weights_out: every sample has its own'
     else:
         assert weights_out is None
-    _here(k_pages, dev)
+    here = _here(k_pages, dev)
     if out is None:
         out = q.new_empty((rows, width))
     op, ldo = _rows(out, q.shape, dev)
@@ -945,7 +946,7 @@ def attn_paged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, bl
     need = _attn_paged_ws_bytes(n_seq, hk, hd, ps, cols, rows, max_q, max_kv, n_heads, w_cols)
     buf = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None      # (held until the launch is in the stream)
     hip.call('vm_attn_paged_bf16', hip.ATTN_PAGED.pack(
-        *c, qp, ldq, cu, lens, order, op, ldo, lse.data_ptr(), rows, rows, max_q, max_kv, n_heads, scale, w_cols, w, wo, ws_, wh, wos, woh, 0 if buf is None else buf.data_ptr(), need), stream())
+        *c, qp, ldq, cu, lens, order, op, ldo, lse.data_ptr(), rows, rows, max_q, max_kv, n_heads, scale, w_cols, w, wo, ws_, wh, wos, woh, 0 if buf is None else buf.data_ptr(), need), here)
     return out, lse
 
 
@@ -966,12 +967,12 @@ def kv_evict_paged(k_pages: torch.Tensor, v_pages: torch.Tensor, weights: torch.
     most = min(budget, cols * ps, w_cols)
     assert new_cols * ps >= most, f'{most} tokens may stay: the new table holds {new_cols * ps}'
     lens = _i32(kv_lens, n_seq, dev)
-    _here(k_pages, dev)
+    here = _here(k_pages, dev)
     new_w = torch.empty(n_seq, hk, w_cols, dtype=torch.float32, device=weights.device)
     new_lens = torch.empty(n_seq, dtype=torch.int32, device=weights.device)
     kept = torch.empty(n_seq, hk, budget, dtype=torch.int32, device=weights.device)
     hip.call('vm_kv_evict_paged_bf16', hip.PAGED_KV.pack(*c), w, ws_, wh, w_cols, lens, new_block_table.data_ptr(),
-             row if n_seq > 1 else new_cols, new_cols, budget, recent, new_w.data_ptr(), hk * w_cols, w_cols, new_lens.data_ptr(), kept.data_ptr(), stream())
+             row if n_seq > 1 else new_cols, new_cols, budget, recent, new_w.data_ptr(), hk * w_cols, w_cols, new_lens.data_ptr(), kept.data_ptr(), here)
     return new_w, new_lens, kept
 
 
