@@ -879,7 +879,9 @@ def kv_append_paged(qkv: torch.Tensor, row_seq: torch.Tensor, row_index: torch.T
     here = _here(k_pages, dev)
     if q_out is None:
         q_out = qkv.new_empty((T, n_heads * hd))
-    o, ldo = _rows(q_out, (T, n_heads * hd), dev)
+        o, ldo = q_out.data_ptr(), n_heads * hd
+    else:
+        o, ldo = _rows(q_out, (T, n_heads * hd), dev)
     if T:
         hip.call('vm_kv_append_paged_bf16', hip.PAGED_KV.pack(*c), x, ldx, seq, idx, pos,
                  cos.data_ptr(), sin.data_ptr(), cos.shape[0], T, n_heads, o, ldo, None if nrows is None else _i32(nrows, 1, dev), here)
@@ -924,11 +926,11 @@ def attn_paged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, bl
     c, dev = _paged(k_pages, v_pages, block_table)
     ps, cols, n_seq, hk, hd = c[4], c[7], c[8], c[9], c[10]
     assert q.dim() == 2
-    rows, width = q.shape
+    rows, width = shape = q.shape
     n_heads = width // hd
     assert width == n_heads * hd and n_heads > 0 and n_heads % hk == 0, f'q {tuple(q.shape)}: heads of {hd}, a multiple of {hk} of them'
     assert math.isfinite(scale) and scale > 0 and max_q >= 0 and max_kv >= 0
-    qp, ldq = _rows(q, q.shape, dev)
+    qp, ldq = _rows(q, shape, dev)
     cu, lens, order = _i32(cu_q, n_seq + 1, dev), _i32(kv_lens, n_seq, dev), 0 if row_of_pos is None else _i32(row_of_pos, rows, dev)
     w = wo = ws_ = wh = wos = woh = w_cols = 0
     if weights is not None:
@@ -941,7 +943,9 @@ def attn_paged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, bl
     here = _here(k_pages, dev)
     if out is None:
         out = q.new_empty((rows, width))
-    op, ldo = _rows(out, q.shape, dev)
+        op, ldo = out.data_ptr(), width
+    else:
+        op, ldo = _rows(out, shape, dev)
     lse = torch.empty(n_heads, rows, dtype=torch.float32, device=q.device)
     need = _attn_paged_ws_bytes(n_seq, hk, hd, ps, cols, rows, max_q, max_kv, n_heads, w_cols)
     buf = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None      # (held until the launch is in the stream)
