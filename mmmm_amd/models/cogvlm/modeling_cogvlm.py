@@ -303,6 +303,7 @@ class CogVLMModel(nn.Module):
         B = input_ids.shape[0]
         c = kv_cache
         assert B == c.batch
+        assert live is None or isinstance(c, PagedKVCache) and live.shape == (B,), 'live: one flag per sample, of a paged cache'
         if live is None:
             c.begin(c.rows, c.zeros, c.ones, 1)
         else:

@@ -158,3 +158,12 @@ def test_a_sample_sits_a_turn_out(dev, lm, width, graph):
         assert cache.lens.tolist() == [n if s == silent else n + width + 5 for s, n in enumerate(before)]
         answers.append(two.new_tokens)
     assert torch.equal(answers[0][[0, 2]], answers[1][[0, 2]])
+
+
+def test_live_flags_belong_to_a_paged_cache(dev, lm):
+    ids, pos = torch.zeros(2, dtype=torch.long, device=dev), torch.zeros(2, dtype=torch.long, device=dev)
+    live = torch.ones(2, dtype=torch.bool, device=dev)
+    with pytest.raises(AssertionError):
+        lm.model.decode_step(ids, pos, lm.new_kv_cache(2, 32, dev), live)
+    with pytest.raises(AssertionError):
+        lm.model.decode_step(ids, pos, lm.new_kv_cache(2, 32, dev, page_size=16), live[:1])
