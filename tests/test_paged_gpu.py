@@ -584,3 +584,15 @@ def test_absent_pages_of_long_tables(dev, K, new):
     """more than 64 pages per sample, one of the last ones missing; and a sample that has all of them beside it"""
     run_attention(K, dev, [new, new], [3000, 1500], 2, 1, 64, 16, weights=True, absent=[(0, 100, -1), (0, 187, 10 ** 8)])
     run_attention(K, dev, [new, new], [3000, 2100], 2, 2, 128, 32, absent=[(1, 65, -5)])
+
+
+@pytest.mark.parametrize('H,hk', [(32, 1), (40, 2), (17, 1)])
+def test_many_heads_per_kv_head(dev, K, H, hk):
+    """single tokens whose group alone is more than the rows of the form for few"""
+    run_attention(K, dev, [1, 1], [300, 70], H, hk, 64, 32, weights=True, packed=True)
+    run_attention(K, dev, [3, 1], [90, 513], H, hk, 128, 16, weights=True)
+
+
+def test_long_lists_of_row_tiles(dev, K):
+    """more than a thousand row tiles: whole caches one after the other"""
+    run_attention(K, dev, [80, 70, 80, 66, 80], [80, 100, 90, 70, 85], 16 * 48, 48, 32, 16, packed=True)
