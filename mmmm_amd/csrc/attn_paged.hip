@@ -347,14 +347,14 @@ __global__ __launch_bounds__(SP_WAVES * 64, 2) void attn_paged_split_k(const Att
   }
 }
 
-// joins the key splits of a query row: out = sum_k 2^(m_k - m) O_k / sum_k 2^(m_k - m) l_k, the splits in their order. One wave per row, HD / 64 (at
-// least 1) elements per lane. Latency-bound for a few rows (4 us of which the launch is most): the partial results are asked for four splits at a
-// time and before anything is known about the sample (a row that does not exist reads its own piece of the workspace and throws it away).
+// joins the key splits of a query row: out = sum_k 2^(m_k - m) O_k / sum_k 2^(m_k - m) l_k, the splits in their order. HD / 4 lanes per row, 16 bytes
+// each. Latency-bound for a few rows (4 us of which the launch is most): the partial results are asked for four splits at a time and before anything
+// is known about the sample (a row that does not exist reads its own piece of the workspace and throws it away). 32 x 512 rows in four splits,
+// 35 MB: 8 us (one wave per row, 4 bytes a lane and split: 11).
 template <int HD>
 __global__ __launch_bounds__(256) void attn_paged_join_k(const AttnPagedP p) {
-  constexpr int E = HD >= 128 ? 2 : 1, U = 4;
-  typedef float fE_t __attribute__((ext_vector_type(E)));
-  const int lane = threadIdx.x & 63, hk = blockIdx.y, b = blockIdx.z;
+  constexpr int LPR = HD / 4, RPB = 256 / LPR, U = 4;                // lanes per row, rows per workgroup
+  const int hk = blockIdx.y, b = blockIdx.z;
   const int n = p.n_split;
   if ((int)blockIdx.x >= p.join_blocks) {            // split form with received weights: the other workgroups take 256 tokens each
     __shared__ float l2s[SP_ROWS];
@@ -372,11 +372,10 @@ __global__ __launch_bounds__(256) void attn_paged_join_k(const AttnPagedP p) {
     if (j < min(s.len, min(p.w_cols, p.s_ld))) count(p, s, b, hk, R, j, l2s);
     return;
   }
-  const int r = blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int r = blockIdx.x * RPB + threadIdx.x / LPR, sub = threadIdx.x & (LPR - 1), d = 4 * sub;
   const int64_t slot = ((int64_t)b * p.c.n_kv_heads + hk) * p.s_rows + min(r, p.s_rows - 1);
   const float* part = p.part + slot * n * (HD + 4);
-  const int d = min(lane * E, HD - E);
-  struct Piece { float m[U], l[U]; fE_t o[U]; } x;
+  struct Piece { float m[U], l[U]; f32x4_t o[U]; } x;
   auto load = [&](int k0) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
@@ -384,19 +383,20 @@ __global__ __launch_bounds__(256) void attn_paged_join_k(const AttnPagedP p) {
       const f32x2_t ml = *reinterpret_cast<const f32x2_t*>(q);
       x.m[u] = ml[0];
       x.l[u] = ml[1];
-      x.o[u] = *reinterpret_cast<const fE_t*>(q + 4 + d);
+      x.o[u] = *reinterpret_cast<const f32x4_t*>(q + 4 + d);
     }
   };
   load(0);
   float m = -INFINITY;
-  for (int k = lane; k < n; k += 64) m = fmaxf(m, part[(int64_t)k * (HD + 4)]);
+  for (int k = sub; k < n; k += LPR) m = fmaxf(m, part[(int64_t)k * (HD + 4)]);
+#pragma unroll
+  for (int k = 1; k < LPR; k <<= 1) m = fmaxf(m, __shfl_xor(m, k, 64));
   const SeqInfo s = seq_info(p, b);
   if (r >= min(s.nq, p.max_q) * p.G) return;
   const int i = r / p.G, h = hk * p.G + r % p.G, prow = phys_row(p, s.p0 + i);
-  m = wave_max(m);
   const float base = m == -INFINITY ? 0.f : m;
   float l = 0.f;
-  fE_t o = {0.f};
+  f32x4_t o = {0.f, 0.f, 0.f, 0.f};
   for (int k = 0; k < n; k += U) {
     if (k > 0) load(k);
 #pragma unroll
@@ -405,16 +405,16 @@ __global__ __launch_bounds__(256) void attn_paged_join_k(const AttnPagedP p) {
       const float f = fast_exp2(x.m[u] - base);
       l += f * x.l[u];
 #pragma unroll
-      for (int e = 0; e < E; ++e) o[e] = fmaf(f, x.o[u][e], o[e]);
+      for (int e = 0; e < 4; ++e) o[e] = fmaf(f, x.o[u][e], o[e]);
     }
   }
   const bool some = !(l == 0.f);
   const float inv = some ? 1.f / l : 0.f, l2 = some && prow >= 0 ? m + log2f(l) : -INFINITY;
-  if (prow >= 0 && lane * E < HD) {
-#pragma unroll
-    for (int e = 0; e < E; ++e) p.out[prow * p.ldo + h * HD + d + e] = some ? f2bf(o[e] * inv) : (unsigned short)0;
+  if (prow >= 0) {
+    const u16x4_t w = {f2bf(o[0] * inv), f2bf(o[1] * inv), f2bf(o[2] * inv), f2bf(o[3] * inv)};
+    *reinterpret_cast<u16x4_t*>(p.out + prow * p.ldo + h * HD + d) = some ? w : (u16x4_t){0, 0, 0, 0};
   }
-  if (lane == 0) p.lse[h * p.ld_lse + s.p0 + i] = l2 * LN2;
+  if (sub == 0) p.lse[h * p.ld_lse + s.p0 + i] = l2 * LN2;
 }
 
 }  // namespace
@@ -458,7 +458,7 @@ Plan plan(AttnPagedP& p, int hd) {
   a.split = rows <= SP_ROWS;
   p.n_split = 1; p.s_rows = (int)rows; p.s_ld = (p.max_kv + 31) / 32 * 32;
   p.part = p.s_ws = nullptr;
-  p.join_blocks = (int)((rows + 3) / 4);
+  p.join_blocks = (int)((rows * hd + 1023) / 1024);
   p.n_tiles = p.n_wg = 0;
   if (rows == 0 || heads == 0) return a;
   if (!a.split) {
