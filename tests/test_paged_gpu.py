@@ -596,3 +596,31 @@ def test_many_heads_per_kv_head(dev, K, H, hk):
 def test_long_lists_of_row_tiles(dev, K):
     """more than a thousand row tiles: whole caches one after the other"""
     run_attention(K, dev, [80, 70, 80, 66, 80], [80, 100, 90, 70, 85], 16 * 48, 48, 32, 16, packed=True)
+
+
+@pytest.mark.parametrize('new', [20, 200])
+@pytest.mark.parametrize('hd', [32, 128])
+def test_the_largest_probability_is_not_rounded(dev, K, new, hd):
+    """a key in every later 64-key tile scores a little (0.4 to 4.9 log2 units) more than all before it, and only the last one has values in
+    the first column: there the result is v / sum with one rounding, the result's own (2^-8), if the subtracted maximum is the maximum"""
+    g = torch.Generator().manual_seed(new + hd)
+    H, L = 4, 64 * 6
+    k = torch.zeros(6, H, 64, hd)
+    v = torch.randn(6, H, 64, hd, generator=g).bfloat16()
+    v[:, :, :, 0] = 0
+    step = torch.rand(6, H, generator=g) * 4.5 + 0.4
+    height = step.cumsum(0)
+    k[:, :, 5, 0] = height.bfloat16().float()                                # token 5 of a tile stands out
+    v[5, :, 5, 0] = 1 + torch.rand(H, generator=g).bfloat16()
+    q = torch.zeros(new, H, hd)
+    q[:, :, 0] = 1 + torch.rand(new, H, generator=g) / 16                    # every row another sum
+    k, q = k.bfloat16(), q.view(new, H * hd).bfloat16()
+    table, scale = torch.arange(6, dtype=torch.int32)[None], 0.6931471805599453
+    rest = R.attention(q, k, v, table, [new], [L], scale)
+    out, _ = K.attn_paged(q.to(dev), k.to(dev), v.to(dev), table.to(dev), i32([0, new], dev), i32([L], dev), scale, new, L)
+    got, want = out.cpu().double().view(new, H, hd)[..., 0], rest[0].view(new, H, hd)[..., 0]
+    seen = torch.arange(L - new, L) >= 5 * 64 + 5                            # the rows that see the last one that stands out
+    assert (got[~seen] == 0).all()
+    # numerator: exactly v; sum and quotient in fp32 (scores: one product, base and scale rounded), then one rounding
+    tol = want.abs() * (R.U_BF16 + (L + 64) * R.U_F32)
+    assert ((got - want).abs() <= tol)[seen].all(), float(((got - want).abs() / want.abs())[seen].max() / R.U_BF16)
