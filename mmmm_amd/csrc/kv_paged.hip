@@ -259,7 +259,7 @@ int vm_kv_append_paged_bf16(const vm_paged_kv* cache_host, const void* qkv, int6
   const int rc = paged_cache(cache_host, p.c);
   if (rc != VM_OK) return rc;
   if (rows < 0 || n_heads <= 0 || n_pos <= 0) return VM_ERR_BAD_ARG;
-  if (rows == 0 || cache_host->n_seq == 0) return VM_OK;
+  if (rows == 0) return VM_OK;                    // (rows without a sample still have a rotated q)
   if (!qkv || !row_seq || !row_index || !row_pos || !cos_tab || !sin_tab || !q_out) return VM_ERR_BAD_ARG;
   const int hd = cache_host->head_dim, total = n_heads + 2 * p.c.n_kv_heads;
   if (misaligned16(qkv) || misaligned16(q_out) || misaligned16(cos_tab) || misaligned16(sin_tab) || (ld & 7) || (ldq & 7)) return VM_ERR_BAD_ARG;

@@ -624,3 +624,19 @@ def test_the_largest_probability_is_not_rounded(dev, K, new, hd):
     # numerator: exactly v; sum and quotient in fp32 (scores: one product, base and scale rounded), then one rounding
     tol = want.abs() * (R.U_BF16 + (L + 64) * R.U_F32)
     assert ((got - want).abs() <= tol)[seen].all(), float(((got - want).abs() / want.abs())[seen].max() / R.U_BF16)
+
+
+def test_append_of_rows_without_a_sample(dev, K):
+    """a table of no sample: nothing is stored, the rows' q is rotated all the same"""
+    g = torch.Generator().manual_seed(2)
+    H, hk, hd, T = 4, 2, 64, 5
+    k = torch.full((4, hk, 16, hd), 2.0, dtype=torch.bfloat16, device=dev)
+    v, table = k.clone(), torch.zeros(0, 3, dtype=torch.int32)
+    qkv = torch.randn(T, (H + 2 * hk) * hd, generator=g).bfloat16()
+    ang = torch.rand(8, hd, generator=g) * 6
+    seq, idx, pos = torch.zeros(T, dtype=torch.int32), torch.arange(T, dtype=torch.int32), torch.arange(1, T + 1, dtype=torch.int32)
+    want = R.append(qkv, seq, idx, table, k.cpu(), v.cpu(), pos, ang.cos(), ang.sin(), H)
+    q = torch.full((T, H * hd), 5.0, dtype=torch.bfloat16, device=dev)
+    K.kv_append_paged(qkv.to(dev), seq.to(dev), idx.to(dev), table.to(dev), k, v, pos.to(dev), ang.cos().to(dev), ang.sin().to(dev), H, q_out=q)
+    close(q, want[0], want[1])
+    assert (k == 2).all() and (v == 2).all()
