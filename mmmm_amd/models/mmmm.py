@@ -462,7 +462,7 @@ class MMMMForCausalLM(CogVLMForCausalLM):
 
             if use_graph and forced_tokens is None and not return_logits and steps > 2:
                 new_tokens, new_pos = self._generate_graphed(cache, head, logits, prev_tok, pos, done, steps, eos_token_id, bop, eop,
-                                                             eos_check_every, trim, past_key_values is not None)
+                                                             eos_check_every, trim)
                 return GenerateOutput(new_tokens=new_tokens, new_position_ids=new_pos, prompt_lengths=n_valid, past_key_values=cache)
             new_tokens, new_pos, all_logits = [], [], ([logits] if return_logits else None)
             for t in range(steps):
@@ -473,7 +473,7 @@ class MMMMForCausalLM(CogVLMForCausalLM):
                     break
                 if forced_tokens is None and eos_token_id is not None and (t + 1) % eos_check_every == 0 and bool(done.all()):
                     break
-                live = ~done if paged and (eos_token_id is not None or past_key_values is not None) else None
+                live = ~done if paged else None
                 logits = linear_decode(self.model.decode_step(tok, pos, cache, live), self.lm_head).float()
                 trim()
                 if return_logits:
@@ -493,7 +493,7 @@ class MMMMForCausalLM(CogVLMForCausalLM):
         most = max(L, min(L + steps, budget + page_size + 1))
         return self.new_kv_cache(B, most, dev, page_size=page_size, n_pages=B * (up(most) + up(budget)), track_weights=True)
 
-    def _generate_graphed(self, cache, head, logits, prev_tok, pos, done, steps, eos_token_id, bop, eop, eos_check_every, trim, turn):
+    def _generate_graphed(self, cache, head, logits, prev_tok, pos, done, steps, eos_token_id, bop, eop, eos_check_every, trim):
         """greedy loop with the decode step captured in a hipGraph. State lives in static device buffers that the graph
         updates in place: (tok, pos, done) of the newest token, a step counter, and the [B, steps] outputs it scatters into.
         One eager step first: it sets the lazily-initialised kernel attributes and warms the allocator outside the capture."""
@@ -512,7 +512,7 @@ class MMMMForCausalLM(CogVLMForCausalLM):
         paged = isinstance(cache, PagedKVCache)
 
         def decode(tok, pos, done):
-            live = ~done if paged and (eos_token_id is not None or turn) else None
+            live = ~done if paged else None
             return linear_decode(self.model.decode_step(tok, pos, cache, live), self.lm_head).float()
 
         tok, pos, done = choose(logits, prev_tok, pos, done)

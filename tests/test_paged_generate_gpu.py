@@ -167,3 +167,20 @@ def test_live_flags_belong_to_a_paged_cache(dev, lm):
         lm.model.decode_step(ids, pos, lm.new_kv_cache(2, 32, dev), live)
     with pytest.raises(AssertionError):
         lm.model.decode_step(ids, pos, lm.new_kv_cache(2, 32, dev, page_size=16), live[:1])
+
+
+@pytest.mark.parametrize('graph', [False, True])
+def test_a_silent_sample_of_the_first_call_stores_nothing(dev, lm, graph):
+    """a cache made by the call itself, no eos: a sample without a valid token is not cached, and the conversation goes on without it"""
+    batch, tok = make_inputs(dev)
+    lm.tokenizer = tok
+    g = torch.Generator().manual_seed(5)
+    ids = torch.randint(3, 150, (3, 9), generator=g).to(dev)
+    mask = torch.ones_like(ids)
+    mask[1] = 0
+    mask[2, 6:] = 0
+    kw = dict(token_type_ids=torch.zeros_like(ids), position_ids=torch.arange(9, device=dev).expand(3, 9).contiguous(), image=None, patch_size=None, pool_size=None)
+    out = lm.generate(ids, attention_mask=mask, **kw, max_new_tokens=6, kv_page_size=16, use_graph=graph)
+    assert out.past_key_values.lens.tolist() == [9 + 5, 0, 6 + 5]
+    alone = lm.generate(ids[:1], **{k: v[:1] if v is not None else None for k, v in kw.items()}, max_new_tokens=6, kv_page_size=16, use_graph=graph)
+    assert torch.equal(out.new_tokens[:1], alone.new_tokens)
