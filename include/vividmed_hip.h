@@ -569,7 +569,8 @@ int vm_attn_paged_bf16(const vm_attn_paged_args* args_host, void* stream);
 
 /* Eviction: of every sample and kv head the `budget` tokens stay that are among the `recent` newest or have the largest weight (ties: the
  * older one; NaN counts as least; tokens of absent pages never stay). They keep their order and go to the pages of new_table, which nothing
- * else may use and which hold them all; the old pages are not changed. new_lens[b] = how many stayed, new_weights their weights with zeros behind,
+ * else may use and which hold them all (a sample all of whose tokens stay may name its own pages: nothing of it is moved); the old pages are not
+ * changed. new_lens[b] = how many stayed, new_weights their weights with zeros behind,
  * kept[b][kv head][budget] their old indices with -1 behind. */
 int vm_kv_evict_paged_bf16(const vm_paged_kv* cache_host, const float* weights, int64_t ldw_seq, int64_t ldw_head, int w_cols,
                            const int32_t* kv_lens, const int32_t* new_table, int64_t ld_new_table, int new_pages, int budget, int recent,

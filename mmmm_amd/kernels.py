@@ -958,7 +958,7 @@ def kv_evict_paged(k_pages: torch.Tensor, v_pages: torch.Tensor, weights: torch.
                    new_block_table: torch.Tensor, budget: int, recent: int):
     """of every sample and kv head the `budget` tokens stay that are among the `recent` newest or have received the most attention weight
     (weights fp32 [samples, kv heads, cols], a column for every cached token; ties: the older token), in their order, in the pages of
-    new_block_table — pages that nothing else uses; the old ones are not changed (vm_kv_evict_paged_bf16). -> (new weights, new lens int32
+    new_block_table — pages that nothing else uses (a sample all of whose tokens stay may name its own); the old ones are not changed (vm_kv_evict_paged_bf16). -> (new weights, new lens int32
     [samples], kept int32 [samples, kv heads, budget]: old indices, -1 behind the last)"""
     c, dev = _paged(k_pages, v_pages, block_table)
     ps, cols, n_seq, hk = c[4], c[7], c[8], c[9]

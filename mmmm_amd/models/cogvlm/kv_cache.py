@@ -77,9 +77,11 @@ class PagedKVCache:
 
     `k`, `v` `[n_layers, n_pages, n_heads, page_size, head_dim]` bf16: a page holds the same tokens in every layer, so there is one
     `block_table` int32 `[batch, pages per sample]` (token j of a sample lies in page `block_table[b, j // page_size]`), kept on the host
-    (which owns the list of free pages) and uploaded when it changes. As in `KVCache` only valid tokens are stored, lengths live on the
-    device, the host knows upper bounds (`len_bound`), and a step that needs no new page uploads nothing and does not synchronise — `reserve`
-    ahead of a captured step. `track_weights` keeps `weights` fp32 `[n_layers, batch, n_heads, tokens]`, which `evict` needs."""
+    (which owns the list of free pages) and uploaded when it changes. As in `KVCache` only valid tokens are stored and lengths live on the
+    device. The host knows an upper bound of each sample's length and hands out pages by it; a step that needs no new page uploads nothing
+    and does not synchronise — `reserve` ahead of a captured step. Where the bounds ask for more than the pool or `max_len` holds, the lengths
+    are read back (one synchronisation) before the call is refused. `track_weights` keeps `weights` fp32 `[n_layers, batch, n_heads, tokens]`
+    (`max_len` of them for every sample), which `evict` needs."""
 
     def __init__(self, n_layers: int, batch: int, max_len: int, n_heads: int, head_dim: int, device, *, page_size: int = 64,
                  n_pages: int | None = None, track_weights: bool = False, dtype=torch.bfloat16):
@@ -97,10 +99,12 @@ class PagedKVCache:
         self.lens = torch.zeros(batch, dtype=torch.int32, device=device)
         self.block_table = torch.full((batch, cols), -1, dtype=torch.int32, device=device)
         self.weights = torch.zeros(n_layers, batch, n_heads, self.max_len, dtype=torch.float32, device=device) if track_weights else None
-        self.len_bound = 0            # host upper bound of lens
+        self._bounds = [0] * batch    # host upper bounds of lens
         self.launch_bound: int | None = None            # as in KVCache
+        self.launch_new: list[int] | None = None        # of a captured step: new tokens per sample that prepare_step() has found pages for
         self._free = list(range(n_pages - 1, -1, -1))
         self._pages: list[list[int]] = [[] for _ in range(batch)]
+        self._reserved = [0] * batch  # tokens whose pages stay until tighten()
         self._pending: torch.Tensor | None = None
         self.rows = torch.arange(batch, device=device, dtype=torch.int32)
         self.zeros = torch.zeros(batch, device=device, dtype=torch.int32)
@@ -119,12 +123,35 @@ class PagedKVCache:
     def free_pages(self) -> int:
         return len(self._free)
 
+    @property
+    def len_bound(self) -> int:
+        """host upper bound of the longest sample's length"""
+        return max(self._bounds, default=0)
+
+    @len_bound.setter
+    def len_bound(self, n: int):
+        self._bounds = [n] * self.batch
+
+    @property
+    def len_bounds(self) -> list[int]:
+        """the same for every sample"""
+        return list(self._bounds)
+
+    @len_bounds.setter
+    def len_bounds(self, n: list[int]):
+        self._bounds = list(n)
+
+    def _up(self, tokens: int) -> int:
+        return -(-tokens // self.page_size)
+
     def _take(self, tokens: int) -> list[int]:
-        n = -(-tokens // self.page_size)
-        return [self._free.pop() for _ in range(n)]
+        return [self._free.pop() for _ in range(self._up(tokens))]
+
+    def _capturing(self) -> bool:
+        return self.block_table.is_cuda and torch.cuda.is_current_stream_capturing()
 
     def _not_captured(self):
-        if self.block_table.is_cuda and torch.cuda.is_current_stream_capturing():
+        if self._capturing():
             raise RuntimeError('the block table changes inside a captured step: reserve() the pages first')
 
     def _upload(self, pages: list[list[int]], table: torch.Tensor):
@@ -133,29 +160,62 @@ class PagedKVCache:
             host[b, :len(p)] = torch.tensor(p, dtype=torch.int32)
         table.copy_(host)
 
-    def reserve(self, tokens: int):
-        """pages for `tokens` tokens of every sample (those it has counted): later steps up to that length upload nothing"""
-        if tokens > self.max_len:
-            raise ValueError(f'KV cache overflow: {tokens} > {self.max_len}')
-        want = -(-tokens // self.page_size)
-        short = sum(max(0, want - len(p)) for p in self._pages)
-        if short > len(self._free):
-            raise ValueError(f'KV cache overflow: {short} pages wanted, {len(self._free)} free')
-        if short:
+    def _grant(self, want: list[int]) -> bool:
+        """pages for want[b] tokens of sample b; False, and nothing changes, if there is no room for all"""
+        short = [max(0, self._up(n) - len(p)) for n, p in zip(want, self._pages)]
+        if max(want, default=0) > self.max_len or sum(short) > len(self._free):
+            return False
+        if any(short):
             self._not_captured()
-            for p in self._pages:
-                p.extend(self._take((want - len(p)) * self.page_size) if want > len(p) else [])
+            for p, n in zip(self._pages, short):
+                p.extend(self._take(n * self.page_size))
             self._upload(self._pages, self.block_table)
+        return True
+
+    def _overflow(self, want: list[int]) -> ValueError:
+        if max(want) > self.max_len:
+            return ValueError(f'KV cache overflow: {max(want)} > {self.max_len}')
+        short = sum(max(0, self._up(n) - len(p)) for n, p in zip(want, self._pages))
+        return ValueError(f'KV cache overflow: {short} pages wanted, {len(self._free)} free')
+
+    def reserve(self, tokens: int):
+        """pages for `tokens` tokens of every sample (those it has counted): later steps up to that length upload nothing. They stay until
+        tighten()."""
+        want = [tokens] * self.batch
+        if not self._grant(want):
+            raise self._overflow(want)
+        self._reserved = [max(n, tokens) for n in self._reserved]
+
+    def _room(self, most: list[int], rows_per_seq: torch.Tensor) -> list[int]:
+        """pages for at most most[b] further tokens of sample b, or, where the bounds leave no room for so many, for the rows_per_seq (device)
+        there are behind the lengths there are -> host upper bounds of the new tokens"""
+        want = [n + m for n, m in zip(self._bounds, most)]
+        if self._grant(want):
+            return most
+        if not self._capturing():
+            self._settle()
+            most = rows_per_seq.tolist()
+            want = [n + m for n, m in zip(self._bounds, most)]
+            if self._grant(want):
+                return most
+        raise self._overflow(want)
 
     def begin(self, seq_of_row: torch.Tensor, offset_in_seq: torch.Tensor, rows_per_seq: torch.Tensor, max_new: int):
         """as KVCache.begin: row r of the call is the offset_in_seq[r]-th new token of sample seq_of_row[r] (-1: of none, nothing is stored);
         a sample without new rows is left out of the call altogether (its queries see nothing and count nowhere)"""
-        self.reserve(self.len_bound + max_new)
+        self._pending_bounds = self._room([max_new] * self.batch if self.launch_new is None else self.launch_new, rows_per_seq)
         self._row_seq = seq_of_row.to(torch.int32).contiguous()
         self._row_index = (self.lens[self._row_seq.long()] + offset_in_seq.to(torch.int32)).contiguous()
         self._pending = rows_per_seq.to(torch.int32)
-        self._pending_bound = max_new
         self._lens_after = torch.where(self._pending > 0, self.lens + self._pending, self.zeros)
+
+    def prepare_step(self, live: torch.Tensor):
+        """ahead of the capture or a replay of a decode step: pages for its tokens (live bool [batch]: the samples that may still have one)"""
+        self.launch_new = self._room([1] * self.batch, live)
+
+    def count_step(self):
+        """a captured step has been replayed: its tokens"""
+        self._bounds = [n + m for n, m in zip(self._bounds, self.launch_new)]
 
     def append(self, layer: int, qkv: torch.Tensor, row_pos: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor,
                nrows: torch.Tensor | None = None) -> torch.Tensor:
@@ -174,21 +234,20 @@ class PagedKVCache:
         return self._lens_after
 
     def attn_bound(self) -> int:
-        return self.launch_bound if self.launch_bound is not None else self.len_bound + self._pending_bound
+        return self.launch_bound if self.launch_bound is not None else max((n + m for n, m in zip(self._bounds, self._pending_bounds)), default=0)
 
     def commit(self):
         self.lens.add_(self._pending)
-        self.len_bound += self._pending_bound
+        self._bounds = [n + m for n, m in zip(self._bounds, self._pending_bounds)]
         self._pending = None
 
-    def tighten(self) -> list[int]:
-        """read the lengths back (the one call that synchronises), give pages behind them back -> lengths"""
-        assert self._pending is None, 'tighten() between begin() and commit()'
+    def _settle(self) -> list[int]:
+        """the lengths as they are on the device; pages behind them (and behind what is reserved) are free again"""
         lens = self.lens.tolist()
-        self.len_bound = max(lens, default=0)
+        self._bounds = list(lens)
         changed = False
-        for p, n in zip(self._pages, lens):
-            keep = -(-n // self.page_size)
+        for p, n, r in zip(self._pages, lens, self._reserved):
+            keep = self._up(max(n, r))
             changed |= len(p) > keep
             while len(p) > keep:
                 self._free.append(p.pop())
@@ -196,22 +255,33 @@ class PagedKVCache:
             self._upload(self._pages, self.block_table)
         return lens
 
+    def tighten(self) -> list[int]:
+        """read the lengths back (synchronises), give pages behind them back, reserved ones too -> lengths"""
+        assert self._pending is None, 'tighten() between begin() and commit()'
+        self._reserved = [0] * self.batch
+        return self._settle()
+
+    def pages_to_evict(self, budget: int) -> int:
+        """free pages that evict() to `budget` tokens needs while it runs: those of the samples that are over it"""
+        return sum(self._up(budget) for n in self._bounds if n > budget)
+
     def evict(self, budget: int, recent: int):
         """cut every sample to the `budget` tokens (per layer and head) that are among its `recent` newest or have received the most
-        attention; they keep their order and their rotary positions. Needs ceil(budget / page_size) free pages per sample while it runs."""
+        attention; they keep their order and their rotary positions. Needs ceil(budget / page_size) free pages for every sample over the
+        budget while it runs; the others stay where they are."""
         assert self._pending is None, 'evict() between begin() and commit()'
         if self.weights is None:
             raise ValueError('evict() needs the received attention weights: track_weights=True')
         if budget <= 0 or not 0 <= recent <= budget:
             raise ValueError(f'budget {budget}, recent {recent}: 0 <= recent <= budget, budget > 0')
-        left = min(budget, self.len_bound)
-        if left == self.len_bound:
+        need = self.pages_to_evict(budget)
+        if need == 0:
             return                                       # nobody is over the budget
-        need = -(-left // self.page_size) * self.batch
         if need > len(self._free):
             raise ValueError(f'KV cache overflow: eviction to {budget} tokens wants {need} pages, {len(self._free)} free')
         self._not_captured()
-        pages = [self._take(left) for _ in range(self.batch)]
+        # (who is not over the budget keeps every token in its place: source and destination are the same rows)
+        pages = [self._take(budget) if n > budget else p for n, p in zip(self._bounds, self._pages)]
         table = torch.full_like(self.block_table, -1)
         self._upload(pages, table)
         for layer in range(self.k.shape[0]):
@@ -219,7 +289,8 @@ class PagedKVCache:
             self.weights[layer].copy_(w)
         self.lens.copy_(lens)
         self.block_table.copy_(table)                    # (in place: a captured step reads these buffers)
-        for p in self._pages:
-            self._free.extend(p)
+        for n, p in zip(self._bounds, self._pages):
+            if n > budget:
+                self._free.extend(p)
         self._pages = pages
-        self.len_bound = left
+        self._bounds = [min(n, budget) for n in self._bounds]

@@ -429,8 +429,11 @@ class MMMMForCausalLM(CogVLMForCausalLM):
             paged = isinstance(cache, PagedKVCache)
 
             def trim():      # after the prompt, and when a page more than the budget has gathered
-                if kv_budget is not None and cache.len_bound >= kv_budget + cache.page_size:
-                    cache.evict(kv_budget, kv_recent)
+                if kv_budget is None or cache.len_bound < kv_budget + cache.page_size:
+                    return
+                if cache.pages_to_evict(kv_budget) > cache.free_pages:      # (as far as the host knows the lengths)
+                    cache.tighten()
+                cache.evict(kv_budget, kv_recent)
             out = self(input_ids, image=image, patch_size=patch_size, pool_size=pool_size, token_type_ids=token_type_ids,
                        attention_mask=attention_mask, position_ids=position_ids, past_key_values=cache, use_cache=True,
                        materialize_logits=False)
@@ -521,10 +524,6 @@ class MMMMForCausalLM(CogVLMForCausalLM):
         s_prev, s_pos, s_done = tok.clone(), pos.clone(), done.clone()
         s_logits = logits.clone()
         s_col = torch.ones(B, 1, dtype=torch.long, device=dev)
-        cache.launch_bound = cache.max_len
-        if paged:                                 # no page may be handed out inside the captured step
-            trim()
-            cache.reserve(min(cache.max_len, cache.len_bound + 1))
 
         def step():
             tok, pos, done = choose(s_logits, s_prev, s_pos, s_done)
@@ -534,22 +533,37 @@ class MMMMForCausalLM(CogVLMForCausalLM):
             s_logits.copy_(decode(tok, pos, done))
             s_prev.copy_(tok); s_pos.copy_(pos); s_done.copy_(done)
 
-        torch.cuda.synchronize()
-        graph = torch.cuda.CUDAGraph()
-        bound0 = cache.len_bound
-        with torch.cuda.graph(graph):
-            step()
-        cache.len_bound = bound0                  # the capture ran the host bookkeeping once without executing anything
-        t = 1
-        while t < steps - 1:
+        def ahead():                              # no page may be handed out inside the captured step
             if paged:
                 trim()
-                cache.reserve(cache.len_bound + 1)
-            graph.replay()
-            cache.len_bound += 1
-            t += 1
-            if eos_token_id is not None and t % eos_check_every == 0 and bool(s_done.all()):
-                break
+                cache.prepare_step(~s_done)
+
+        cache.launch_bound = cache.max_len
+        try:
+            ahead()
+            torch.cuda.synchronize()
+            graph = torch.cuda.CUDAGraph()
+            bounds = cache.len_bounds if paged else cache.len_bound
+            with torch.cuda.graph(graph):
+                step()
+            if paged:                             # the capture ran the host bookkeeping once without executing anything
+                cache.len_bounds = bounds
+            else:
+                cache.len_bound = bounds
+            t = 1
+            while t < steps - 1:
+                ahead()
+                graph.replay()
+                if paged:
+                    cache.count_step()
+                else:
+                    cache.len_bound += 1
+                t += 1
+                if eos_token_id is not None and t % eos_check_every == 0 and bool(s_done.all()):
+                    break
+        finally:
+            if paged:
+                cache.launch_new = None
         if t == steps - 1:                        # the last token needs no decode step after it
             tok, pos, _ = choose(s_logits, s_prev, s_pos, s_done)
             out_tok[:, t], out_pos[:, t] = tok, pos

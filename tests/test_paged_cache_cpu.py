@@ -62,3 +62,89 @@ def test_refusals():
     t.begin(t.rows, t.zeros, t.ones, 0)
     with pytest.raises(AssertionError):
         t.tighten()
+
+
+def turn(c, new, most=None):
+    """one call with new[b] further tokens of sample b, of which the host knows that they are at most `most`"""
+    rows = [(b, i) for b, n in enumerate(new) for i in range(n)]
+    seq, off = (torch.tensor(x, dtype=torch.int32) for x in zip(*rows))
+    c.begin(seq, off, torch.tensor(new, dtype=torch.int32), max(new) if most is None else most)
+    pages = [[int(c.block_table[b, int(j) // c.page_size]) for b, j in zip(seq.tolist(), c._row_index.tolist())]]
+    assert min(pages[0]) >= 0                               # every row has its page
+    c.commit()
+
+
+@pytest.mark.parametrize('lens,page,n_pages', [((4000, 100), 64, 65), ((1000, 10), 16, 64), ((1, 700, 33), 16, 48)])
+def test_samples_of_different_lengths_share_a_pool_that_just_holds_them(lens, page, n_pages):
+    c = PagedKVCache(1, len(lens), 4096, 2, 32, 'cpu', page_size=page, n_pages=n_pages)
+    turn(c, lens)
+    left = [-(-n // page) * page - n for n in lens]          # room in the last pages
+    for _ in range(min(left)):
+        turn(c, [1] * len(lens))
+    assert c.lens.tolist() == [n + min(left) for n in lens] and c.free_pages == n_pages - sum(-(-n // page) for n in lens)
+    used = c.block_table[c.block_table >= 0].tolist()
+    assert len(set(used)) == len(used)
+    before = c.tighten()
+    with pytest.raises(ValueError):                          # one more does not fit, and nothing has changed
+        turn(c, [page * n_pages] * len(lens))
+    assert c.lens.tolist() == before and c.tighten() == before
+
+
+def test_a_short_sample_goes_on_beside_a_long_one():
+    c = PagedKVCache(1, 2, 112, 2, 32, 'cpu', page_size=16)
+    turn(c, [100, 10])
+    turn(c, [0, 20])
+    assert c.lens.tolist() == [100, 30]
+    for _ in range(12):
+        turn(c, [1, 1])
+    turn(c, [0, 1])                                          # the long one is full
+    assert c.lens.tolist() == [112, 43] and c.attn_bound is not None and c.len_bound == 112
+    with pytest.raises(ValueError):
+        turn(c, [1, 1])
+    assert c.lens.tolist() == [112, 43]
+
+
+def test_bounds_are_a_samples_own():
+    c = PagedKVCache(1, 3, 256, 2, 32, 'cpu', page_size=16, n_pages=16)
+    turn(c, [200, 3, 0], most=200)                           # 13 + 1 pages
+    assert c.len_bounds == [200, 3, 0] and c.free_pages == 2 and c.len_bound == 200
+    c.begin(torch.tensor([0, 1], dtype=torch.int32), torch.zeros(2, dtype=torch.int32), torch.tensor([1, 1, 0], dtype=torch.int32), 1)
+    assert c.attn_bound() == 201
+    c.commit()
+    c.prepare_step(torch.tensor([True, True, True]))
+    assert c.launch_new == [1, 1, 1]
+    c.count_step()
+    assert c.len_bounds == [202, 5, 2]
+    c.launch_new = None
+    assert c.tighten() == [201, 4, 0] and c.len_bounds == [201, 4, 0]
+
+
+def test_a_captured_steps_pages_go_to_the_samples_that_go_on():
+    c = PagedKVCache(1, 2, 64, 2, 32, 'cpu', page_size=16, n_pages=3)
+    turn(c, [16, 16])                                        # both at the end of a page, one page left
+    with pytest.raises(ValueError):
+        c.prepare_step(torch.tensor([True, True]))
+    c.prepare_step(torch.tensor([False, True]))
+    assert c.launch_new == [0, 1] and (c.block_table >= 0).sum(1).tolist() == [1, 2]
+    c.count_step()
+    assert c.len_bounds == [16, 17]
+
+
+def test_reserved_pages_stay_until_tighten():
+    c = PagedKVCache(1, 2, 64, 2, 32, 'cpu', page_size=16, n_pages=5)
+    c.reserve(32)
+    turn(c, [20, 3])
+    with pytest.raises(ValueError):
+        turn(c, [13, 30], most=30)                           # 3 + 3 pages
+    assert (c.block_table >= 0).sum(1).tolist() == [2, 2]    # (the lengths were read; what is reserved stayed)
+    turn(c, [13, 1], most=30)
+    assert c.tighten() == [33, 4] and c.free_pages == 1
+
+
+def test_eviction_needs_pages_for_those_over_the_budget_only():
+    c = PagedKVCache(1, 3, 256, 2, 32, 'cpu', page_size=16, track_weights=True)
+    c.lens.copy_(torch.tensor([200, 20, 0]))
+    c.len_bounds = [200, 20, 0]
+    assert c.pages_to_evict(32) == 2 and c.pages_to_evict(16) == 2 and c.pages_to_evict(200) == 0
+    c.evict(200, 8)                                          # nobody is over it: nothing to do (no kernel here)
+    assert c.len_bounds == [200, 20, 0]

@@ -184,3 +184,45 @@ def test_a_silent_sample_of_the_first_call_stores_nothing(dev, lm, graph):
     assert out.past_key_values.lens.tolist() == [9 + 5, 0, 6 + 5]
     alone = lm.generate(ids[:1], **{k: v[:1] if v is not None else None for k, v in kw.items()}, max_new_tokens=6, kv_page_size=16, use_graph=graph)
     assert torch.equal(out.new_tokens[:1], alone.new_tokens)
+
+
+@pytest.mark.parametrize('graph', [False, True])
+def test_a_ragged_batch_in_a_pool_that_just_holds_it(dev, lm, graph):
+    """pages for the tokens there are, not for batch x longest: the same tokens as in a pool with room for all, one page less is refused"""
+    batch, tok = make_inputs(dev)
+    lm.tokenizer = tok
+    g = torch.Generator().manual_seed(6)
+    lens, steps, page = [90, 7, 30], 20, 16
+    ids = torch.randint(3, 150, (3, 90), generator=g).to(dev)
+    mask = (torch.arange(90)[None] < torch.tensor(lens)[:, None]).long().to(dev)
+    kw = dict(token_type_ids=torch.zeros_like(ids), position_ids=torch.arange(90, device=dev).expand(3, 90).contiguous(), attention_mask=mask,
+              image=None, patch_size=None, pool_size=None, max_new_tokens=steps, use_graph=graph)
+    want = lm.generate(ids, **kw, kv_page_size=page)
+    need = sum(-(-(n + steps - 1) // page) for n in lens)
+    assert need < want.past_key_values.k.shape[1] * 2 // 3
+    cache = lm.new_kv_cache(3, 90 + steps, dev, page_size=page, n_pages=need)
+    out = lm.generate(ids, **kw, past_key_values=cache)
+    assert torch.equal(out.new_tokens, want.new_tokens) and cache.lens.tolist() == [n + steps - 1 for n in lens] and cache.launch_new is None
+    small = lm.new_kv_cache(3, 90 + steps, dev, page_size=page, n_pages=need - 1)
+    with pytest.raises(ValueError, match='overflow'):
+        lm.generate(ids, **kw, past_key_values=small)
+    assert small.launch_new is None
+
+
+@pytest.mark.parametrize('graph', [False, True])
+def test_a_finished_sample_takes_no_pages(dev, lm, graph):
+    batch, tok = make_inputs(dev)
+    lm.tokenizer = tok
+    g = torch.Generator().manual_seed(8)
+    ids = torch.randint(3, 150, (2, 14), generator=g).to(dev)
+    kw = dict(token_type_ids=torch.zeros_like(ids), position_ids=torch.arange(14, device=dev).expand(2, 14).contiguous(), image=None, patch_size=None,
+              pool_size=None, max_new_tokens=40, use_graph=graph)
+    free = lm.generate(ids, **kw, kv_page_size=16)
+    first = [int(free.new_tokens[0, 0]), int(free.new_tokens[1, 0])]
+    s = 0 if first[0] not in free.new_tokens[1].tolist() else 1 if first[1] not in free.new_tokens[0].tolist() else None
+    if s is None:
+        pytest.skip('both samples say the same')
+    cache = lm.new_kv_cache(2, 14 + 40, dev, page_size=16, n_pages=1 + 4)    # 14 tokens of the one that ends at once, 53 of the other
+    out = lm.generate(ids, **kw, past_key_values=cache, eos_token_id=first[s], eos_check_every=100)
+    assert cache.lens.tolist()[s] == 14 and cache.lens.tolist()[1 - s] == 53
+    assert torch.equal(out.new_tokens[1 - s], free.new_tokens[1 - s])

@@ -640,3 +640,56 @@ def test_append_of_rows_without_a_sample(dev, K):
     K.kv_append_paged(qkv.to(dev), seq.to(dev), idx.to(dev), table.to(dev), k, v, pos.to(dev), ang.cos().to(dev), ang.sin().to(dev), H, q_out=q)
     close(q, want[0], want[1])
     assert (k == 2).all() and (v == 2).all()
+
+
+@pytest.mark.parametrize('budget', [64, 200])
+def test_who_is_not_over_the_budget_keeps_its_pages(dev, K, budget):
+    """the new table names the old pages of a sample all of whose tokens stay: its rows, weights and indices are what they were"""
+    g = torch.Generator().manual_seed(budget)
+    lens, hk, hd, page = [50, 700, budget, 0], 2, 64, 16
+    k, v, tab = R.make_cache(lens + [budget], hk, hd, page, g)
+    table, new_table = tab[:4], tab[:4].clone()
+    new_table[1] = tab[4]
+    w = torch.rand(4, hk, 720, generator=g)
+    kept, new = R.evict(w, table, k.shape[0], page, lens, budget, 8)
+    kd, vd = k.to(dev), v.to(dev)
+    nw, nl, got = K.kv_evict_paged(kd, vd, w.to(dev), table.to(dev), i32(lens, dev), new_table.to(dev), budget, 8)
+    assert nl.tolist() == new == [50, budget, budget, 0]
+    ke, ve = k.clone(), v.clone()
+    at = torch.arange(budget)
+    for h in range(hk):
+        for b in range(4):
+            assert got[b, h].tolist() == kept[b][h] + [-1] * (budget - new[b])
+            assert torch.equal(nw[b, h].cpu()[:new[b]], w[b, h][kept[b][h]]) and (nw[b, h, new[b]:] == 0).all()
+        idx = torch.tensor(kept[1][h])
+        src, dst = table[1].long()[idx // page], new_table[1].long()[at // page]
+        ke[dst, h, at % page], ve[dst, h, at % page] = k[src, h, idx % page], v[src, h, idx % page]
+    assert torch.equal(kd.cpu().view(torch.int16), ke.view(torch.int16)) and torch.equal(vd.cpu().view(torch.int16), ve.view(torch.int16))
+
+
+def test_cache_evicts_a_ragged_batch(dev):
+    """one sample over the budget, one under it: free pages are needed for the first only, the second stays where it is"""
+    from mmmm_amd.models.cogvlm.kv_cache import PagedKVCache
+    c = PagedKVCache(2, 2, 256, 2, 64, dev, page_size=16, n_pages=16, track_weights=True)
+    lens = [180, 20]                                         # 12 + 2 pages: two are free
+    c.begin(torch.cat([torch.zeros(180), torch.ones(20)]).to(dev), torch.cat([torch.arange(180), torch.arange(20)]).to(dev), i32(lens, dev), 180)
+    c.commit()
+    assert c.lens.tolist() == lens and c.free_pages == 2 and c.len_bounds == lens
+    c.k.normal_()
+    c.v.normal_()
+    c.weights[:, 0, :, :180].uniform_()
+    c.weights[:, 1, :, :20].uniform_()
+    rows = lambda x, b, idx: torch.stack([x[c.block_table[b].long()[j // 16], :, j % 16] for j in idx], 1)      # noqa: E731  [heads, tokens, hd]
+    old = [[[rows(x[layer], b, range(n)) for x in (c.k, c.v)] for b, n in enumerate(lens)] for layer in range(2)]
+    w, table = c.weights.clone(), c.block_table.cpu().clone()
+    c.evict(24, 4)
+    assert c.lens.tolist() == [24, 20] == c.len_bounds and c.free_pages == 12 and torch.equal(c.block_table[1].cpu(), table[1])
+    assert torch.equal(c.weights[:, 1], w[:, 1])
+    for layer in range(2):
+        kept, _ = R.evict(w[layer].cpu(), table, 16, 16, lens, 24, 4)
+        for b in range(2):
+            for n, x in enumerate((c.k, c.v)):
+                now = rows(x[layer], b, range(c.lens.tolist()[b]))
+                for h in range(2):
+                    assert torch.equal(now[h], old[layer][b][n][h][kept[b][h]])
+                    assert torch.equal(c.weights[layer, b, h, :len(kept[b][h])], w[layer, b, h][kept[b][h]])
