@@ -106,6 +106,8 @@ class PagedKVCache:
         self._pages: list[list[int]] = [[] for _ in range(batch)]
         self._reserved = [0] * batch  # tokens whose pages stay until tighten()
         self._pending: torch.Tensor | None = None
+        self._counting = False        # this call has added to `weights`
+        self._miscounted = False      # a call that was dropped has
         self.rows = torch.arange(batch, device=device, dtype=torch.int32)
         self.zeros = torch.zeros(batch, device=device, dtype=torch.int32)
         self.ones = torch.ones(batch, device=device, dtype=torch.int32)
@@ -203,6 +205,8 @@ class PagedKVCache:
     def begin(self, seq_of_row: torch.Tensor, offset_in_seq: torch.Tensor, rows_per_seq: torch.Tensor, max_new: int):
         """as KVCache.begin: row r of the call is the offset_in_seq[r]-th new token of sample seq_of_row[r] (-1: of none, nothing is stored);
         a sample without new rows is left out of the call altogether (its queries see nothing and count nowhere)"""
+        self.abort()
+        self._in_capture = self._capturing()
         self._pending_bounds = self._room([max_new] * self.batch if self.launch_new is None else self.launch_new, rows_per_seq)
         self._row_seq = seq_of_row.to(torch.int32).contiguous()
         self._row_index = (self.lens[self._row_seq.long()] + offset_in_seq.to(torch.int32)).contiguous()
@@ -226,6 +230,7 @@ class PagedKVCache:
     def attend(self, layer: int, q: torch.Tensor, cu_q: torch.Tensor, row_of_pos: torch.Tensor | None, max_q: int, scale: float) -> torch.Tensor:
         """attention of the appended rows over everything cached (their own tokens included, causally)"""
         w = self.weights[layer] if self.weights is not None else None
+        self._counting = w is not None and not self._in_capture
         return K.attn_paged(q, self.k[layer], self.v[layer], self.block_table, cu_q, self._lens_after, scale, max_q, self.attn_bound(),
                             row_of_pos=row_of_pos, weights=w)[0]
 
@@ -240,6 +245,14 @@ class PagedKVCache:
         self.lens.add_(self._pending)
         self._bounds = [n + m for n, m in zip(self._bounds, self._pending_bounds)]
         self._pending = None
+        self._counting = False
+
+    def abort(self):
+        """drop the call that begin() has declared, if there is one: the lengths stay what they are, what it has stored lies behind them. The
+        weights that its layers have added up are not taken back: evict() refuses from then on."""
+        self._miscounted |= self._counting
+        self._pending = None
+        self._counting = False
 
     def _settle(self) -> list[int]:
         """the lengths as they are on the device; pages behind them (and behind what is reserved) are free again"""
@@ -272,6 +285,8 @@ class PagedKVCache:
         assert self._pending is None, 'evict() between begin() and commit()'
         if self.weights is None:
             raise ValueError('evict() needs the received attention weights: track_weights=True')
+        if self._miscounted:
+            raise RuntimeError('the received weights count a call that failed half way: this cache cannot be evicted from, start another one')
         if budget <= 0 or not 0 <= recent <= budget:
             raise ValueError(f'budget {budget}, recent {recent}: 0 <= recent <= budget, budget > 0')
         need = self.pages_to_evict(budget)

@@ -238,7 +238,15 @@ class CogVLMModel(nn.Module):
     def forward(self, input_ids, *, image=None, patch_size=None, pool_size=None, token_type_ids=None, attention_mask=None,
                 position_ids=None, output_hidden_states: bool = False, kv_cache: KVCache | PagedKVCache | None = None):
         """kv_cache: an EMPTY cache to fill (prefill of the generation path, `use_cache=True` with no past), or a PagedKVCache that already
-        holds a conversation: the tokens of this call follow it"""
+        holds a conversation: the tokens of this call follow it (if the call fails, the cache is what it was)"""
+        try:
+            return self._forward(input_ids, image, patch_size, pool_size, token_type_ids, attention_mask, position_ids, output_hidden_states, kv_cache)
+        except BaseException:
+            if isinstance(kv_cache, PagedKVCache):
+                kv_cache.abort()
+            raise
+
+    def _forward(self, input_ids, image, patch_size, pool_size, token_type_ids, attention_mask, position_ids, output_hidden_states, kv_cache):
         B, L = input_ids.shape
         dev = input_ids.device
         if token_type_ids is None:
@@ -311,11 +319,16 @@ class CogVLMModel(nn.Module):
         rt = Routing(counts=c.decode_counts, row_of_tok=c.rows, tok_of_row=c.rows, cu_seqlens=c.cu_rows, row_of_pos=c.rows,
                      expert_mask=None, row_pos=position_ids.to(torch.int32).contiguous(), n_rows=c.decode_counts[1:2],
                      B=B, L=1, n_pos=int(self.config.max_position_embeddings), kv=c, kv_lens=c.lens_after())
-        x = Fh.embedding_rows(self.embed_tokens.weight, input_ids.to(torch.int32).contiguous())
-        for layer in self.layers:
-            x = layer(x, rt)
-        x = self.norm(x, rt.n_rows)
-        kv_cache.commit()
+        try:
+            x = Fh.embedding_rows(self.embed_tokens.weight, input_ids.to(torch.int32).contiguous())
+            for layer in self.layers:
+                x = layer(x, rt)
+            x = self.norm(x, rt.n_rows)
+            kv_cache.commit()
+        except BaseException:
+            if isinstance(kv_cache, PagedKVCache):
+                kv_cache.abort()
+            raise
         return x
 
 

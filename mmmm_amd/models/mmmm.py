@@ -562,12 +562,12 @@ class MMMMForCausalLM(CogVLMForCausalLM):
                 if eos_token_id is not None and t % eos_check_every == 0 and bool(s_done.all()):
                     break
         finally:
+            cache.launch_bound = None
             if paged:
                 cache.launch_new = None
         if t == steps - 1:                        # the last token needs no decode step after it
             tok, pos, _ = choose(s_logits, s_prev, s_pos, s_done)
             out_tok[:, t], out_pos[:, t] = tok, pos
-        cache.launch_bound = None
         return out_tok, out_pos
 
 

@@ -148,3 +148,22 @@ def test_eviction_needs_pages_for_those_over_the_budget_only():
     assert c.pages_to_evict(32) == 2 and c.pages_to_evict(16) == 2 and c.pages_to_evict(200) == 0
     c.evict(200, 8)                                          # nobody is over it: nothing to do (no kernel here)
     assert c.len_bounds == [200, 20, 0]
+
+
+def test_a_dropped_call():
+    c = cache(track_weights=True)
+    turn(c, [5, 6, 7])
+    one = torch.zeros(1, dtype=torch.int32)
+    c.begin(one, one, torch.tensor([1, 0, 0], dtype=torch.int32), 1)
+    c.abort()
+    assert c.tighten() == [5, 6, 7] and c.len_bounds == [5, 6, 7]
+    turn(c, [1, 1, 1])
+    assert c.tighten() == [6, 7, 8]
+    c.evict(8, 2)                                            # nobody is over it, and nothing was counted by the dropped call
+    c.begin(one, one, torch.tensor([1, 0, 0], dtype=torch.int32), 1)
+    c._counting = True                                       # a layer has added its weights
+    c.abort()
+    with pytest.raises(RuntimeError, match='received weights'):
+        c.evict(8, 2)
+    turn(c, [1, 1, 1])                                       # the conversation itself goes on
+    assert c.tighten() == [7, 8, 9]

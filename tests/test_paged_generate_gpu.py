@@ -226,3 +226,70 @@ def test_a_finished_sample_takes_no_pages(dev, lm, graph):
     out = lm.generate(ids, **kw, past_key_values=cache, eos_token_id=first[s], eos_check_every=100)
     assert cache.lens.tolist()[s] == 14 and cache.lens.tolist()[1 - s] == 53
     assert torch.equal(out.new_tokens[1 - s], free.new_tokens[1 - s])
+
+
+class _Stop(Exception):
+    pass
+
+
+def _fails_after(f, good):
+    """f, whose call number `good` (from 0) raises"""
+    def call(*args):
+        nonlocal good
+        good -= 1
+        if good < 0:
+            raise _Stop
+        return f(*args)
+    return call
+
+
+@pytest.mark.parametrize('graph', [False, True])
+def test_a_failed_turn_leaves_the_conversation_as_it_was(dev, lm, graph, monkeypatch):
+    batch, tok = make_inputs(dev)
+    lm.tokenizer = tok
+    ids, kw = _batch(batch)
+    g = torch.Generator().manual_seed(4)
+    said = torch.randint(3, 150, (3, 5), generator=g).to(dev)
+    answers = []
+    for failing in (False, True):
+        cache = lm.new_kv_cache(3, ids.shape[1] + 40, dev, page_size=16)
+        one = lm.generate(ids, **kw, max_new_tokens=3, past_key_values=cache)
+        turn = dict(token_type_ids=torch.zeros_like(said), position_ids=one.new_position_ids[:, -1:] + torch.arange(5, device=dev), patch_size=None, pool_size=None,
+                    max_new_tokens=6, past_key_values=cache, use_graph=graph)
+        if failing:
+            before = cache.lens.tolist()
+            with pytest.raises(AssertionError):
+                lm.generate(said, **{**turn, 'image': batch['image'][:1], 'patch_size': batch['patch_size'][:1], 'pool_size': batch['pool_size'][:1]})
+            layers = len(lm.model.layers)
+            for calls in (0, 1, 2):                          # in the last layer of the chunk; of the first step; of the next (the captured one)
+                with monkeypatch.context() as m:
+                    m.setattr(type(cache), 'attend', _fails_after(type(cache).attend, calls * layers + layers - 1))
+                    with pytest.raises(_Stop):
+                        lm.generate(said, **turn, image=None)
+                assert cache.launch_bound is None and cache.launch_new is None
+                assert cache.tighten() == [n + (0, 5, 6)[calls] for n in before]
+                cache.lens.copy_(torch.tensor(before, dtype=torch.int32))      # the finished calls of the turn are taken back
+                cache.tighten()
+        answers.append(lm.generate(said, **turn, image=None).new_tokens)
+    assert torch.equal(*answers)
+
+
+def test_weights_that_count_a_failed_call_are_not_evicted_by(dev, lm, monkeypatch):
+    batch, tok = make_inputs(dev)
+    lm.tokenizer = tok
+    ids, kw = _batch(batch)
+    cache = lm.new_kv_cache(3, ids.shape[1] + 200, dev, page_size=16, track_weights=True)
+    with pytest.raises(AssertionError):                      # before the first layer: nothing was counted
+        lm.generate(ids, **{**kw, 'image': batch['image'][:1]}, max_new_tokens=3, past_key_values=cache)
+    lm.generate(ids, **kw, max_new_tokens=3, past_key_values=cache, kv_budget=24, kv_recent=8)
+    assert int(cache.lens.max()) < 24 + 16
+    said = ids[:, :4].clone()
+    turn = dict(token_type_ids=torch.zeros_like(said), position_ids=torch.arange(4, device=dev).expand(3, 4).contiguous(), image=None, patch_size=None,
+                pool_size=None, max_new_tokens=30, past_key_values=cache)
+    with monkeypatch.context() as m:
+        m.setattr(type(cache), 'append', _fails_after(type(cache).append, 1))
+        with pytest.raises(_Stop):
+            lm.generate(said, **turn)
+    with pytest.raises(RuntimeError, match='received weights'):
+        lm.generate(said, **turn, kv_budget=24, kv_recent=8)
+    assert lm.generate(said, **turn).new_tokens.shape == (3, 30)
