@@ -286,7 +286,7 @@ class PagedKVCache:
         if self.weights is None:
             raise ValueError('evict() needs the received attention weights: track_weights=True')
         if self._miscounted:
-            raise RuntimeError('the received weights count a call that failed half way: this cache cannot be evicted from, start another one')
+            raise RuntimeError('the received weights are those of a call that failed half way: this cache cannot be evicted from, start another one')
         if budget <= 0 or not 0 <= recent <= budget:
             raise ValueError(f'budget {budget}, recent {recent}: 0 <= recent <= budget, budget > 0')
         need = self.pages_to_evict(budget)
@@ -297,11 +297,17 @@ class PagedKVCache:
         self._not_captured()
         # (who is not over the budget keeps every token in its place: source and destination are the same rows)
         pages = [self._take(budget) if n > budget else p for n, p in zip(self._bounds, self._pages)]
-        table = torch.full_like(self.block_table, -1)
-        self._upload(pages, table)
-        for layer in range(self.k.shape[0]):
-            w, lens, _ = K.kv_evict_paged(self.k[layer], self.v[layer], self.weights[layer], self.block_table, self.lens, table, budget, recent)
-            self.weights[layer].copy_(w)
+        layer = 0
+        try:
+            table = torch.full_like(self.block_table, -1)
+            self._upload(pages, table)
+            for layer in range(self.k.shape[0]):
+                w, lens, _ = K.kv_evict_paged(self.k[layer], self.v[layer], self.weights[layer], self.block_table, self.lens, table, budget, recent)
+                self.weights[layer].copy_(w)
+        except BaseException:                            # nothing has moved out of the old pages; the weights of the first layers have
+            self._free.extend(i for n, p in zip(self._bounds, pages) if n > budget for i in p)
+            self._miscounted |= layer > 0
+            raise
         self.lens.copy_(lens)
         self.block_table.copy_(table)                    # (in place: a captured step reads these buffers)
         for n, p in zip(self._bounds, self._pages):

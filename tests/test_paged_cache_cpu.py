@@ -167,3 +167,32 @@ def test_a_dropped_call():
         c.evict(8, 2)
     turn(c, [1, 1, 1])                                       # the conversation itself goes on
     assert c.tighten() == [7, 8, 9]
+
+
+@pytest.mark.parametrize('good', [0, 1])
+def test_a_failed_eviction_gives_its_pages_back(monkeypatch, good):
+    from mmmm_amd.models.cogvlm import kv_cache
+    c = cache(track_weights=True)
+    c.lens.copy_(torch.tensor([60, 50, 3]))
+    c.len_bounds = [60, 50, 3]
+    c.reserve(60)
+    free, table = c.free_pages, c.block_table.clone()
+    calls = []
+
+    def evict(k, v, w, t, lens, new, budget, recent):
+        if len(calls) == good:
+            raise MemoryError
+        calls.append(1)
+        return w, lens, None
+    monkeypatch.setattr(kv_cache.K, 'kv_evict_paged', evict)
+    with pytest.raises(MemoryError):
+        c.evict(16, 4)
+    assert c.free_pages == free and torch.equal(c.block_table, table) and c.len_bounds == [60, 50, 3] and c.lens.tolist() == [60, 50, 3]
+    assert len(set(c._free)) == free
+    good = 2
+    if calls:
+        with pytest.raises(RuntimeError, match='received weights'):
+            c.evict(16, 4)
+    else:
+        c.evict(16, 4)
+        assert c.len_bounds == [16, 16, 3]
