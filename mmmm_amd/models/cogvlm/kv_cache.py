@@ -100,6 +100,8 @@ class PagedKVCache:
         self.block_table = torch.full((batch, cols), -1, dtype=torch.int32, device=device)
         self.weights = torch.zeros(n_layers, batch, n_heads, self.max_len, dtype=torch.float32, device=device) if track_weights else None
         self._bounds = [0] * batch    # host upper bounds of lens
+        self.pos_bound = 0            # host upper bound of the rotary positions: all of them so far are below it
+        self._pos_reserved = 0        # ... and those that reserve_positions() has announced
         self.launch_bound: int | None = None            # as in KVCache
         self.launch_new: list[int] | None = None        # of a captured step: new tokens per sample that prepare_step() has found pages for
         self._free = list(range(n_pages - 1, -1, -1))
@@ -181,12 +183,24 @@ class PagedKVCache:
         return ValueError(f'KV cache overflow: {short} pages wanted, {len(self._free)} free')
 
     def reserve(self, tokens: int):
-        """pages for `tokens` tokens of every sample (those it has counted): later steps up to that length upload nothing. They stay until
-        tighten()."""
+        """pages for `tokens` tokens of every sample (those it has counted), and rotary tables for positions that go on as far: later steps up
+        to that length upload nothing. The pages stay until tighten(); tables that have to grow for it do so in the next step, which then
+        must not be a captured one."""
         want = [tokens] * self.batch
         if not self._grant(want):
             raise self._overflow(want)
+        self.reserve_positions(self.pos_bound + max(0, tokens - min(self._bounds, default=0)))
         self._reserved = [max(n, tokens) for n in self._reserved]
+
+    def reserve_positions(self, n: int):
+        """rotary positions below n are to come"""
+        self._pos_reserved = max(self._pos_reserved, n)
+
+    def rope_len(self, least: int) -> int:
+        """rows of rotary tables that hold the positions so far and the announced ones: `least`, doubled as often as it takes"""
+        while least < max(self.pos_bound, self._pos_reserved):
+            least *= 2
+        return least
 
     def _room(self, most: list[int], rows_per_seq: torch.Tensor) -> list[int]:
         """pages for at most most[b] further tokens of sample b, or, where the bounds leave no room for so many, for the rows_per_seq (device)
@@ -206,7 +220,7 @@ class PagedKVCache:
         """as KVCache.begin: row r of the call is the offset_in_seq[r]-th new token of sample seq_of_row[r] (-1: of none, nothing is stored);
         a sample without new rows is left out of the call altogether (its queries see nothing and count nowhere)"""
         self.abort()
-        self._in_capture = self._capturing()
+        self.in_capture = self._capturing()
         self._pending_bounds = self._room([max_new] * self.batch if self.launch_new is None else self.launch_new, rows_per_seq)
         self._row_seq = seq_of_row.to(torch.int32).contiguous()
         self._row_index = (self.lens[self._row_seq.long()] + offset_in_seq.to(torch.int32)).contiguous()
@@ -219,6 +233,7 @@ class PagedKVCache:
 
     def count_step(self):
         """a captured step has been replayed: its tokens"""
+        self.pos_bound += 1
         self._bounds = [n + m for n, m in zip(self._bounds, self.launch_new)]
 
     def append(self, layer: int, qkv: torch.Tensor, row_pos: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor,
@@ -230,7 +245,7 @@ class PagedKVCache:
     def attend(self, layer: int, q: torch.Tensor, cu_q: torch.Tensor, row_of_pos: torch.Tensor | None, max_q: int, scale: float) -> torch.Tensor:
         """attention of the appended rows over everything cached (their own tokens included, causally)"""
         w = self.weights[layer] if self.weights is not None else None
-        self._counting = w is not None and not self._in_capture
+        self._counting = w is not None and not self.in_capture
         return K.attn_paged(q, self.k[layer], self.v[layer], self.block_table, cu_q, self._lens_after, scale, max_q, self.attn_bound(),
                             row_of_pos=row_of_pos, weights=w)[0]
 

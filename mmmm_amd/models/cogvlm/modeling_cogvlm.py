@@ -86,17 +86,20 @@ class RotaryEmbedding(nn.Module):
         super().__init__()
         self.dim, self.base = dim, base
         self.register_buffer('inv_freq', 1.0 / (base ** (torch.arange(0, dim, 2) / dim)), persistent=False)
-        self._cache: tuple | None = None
+        self._tables: dict = {}       # all that were ever asked for: a captured graph may still read the shorter ones
+
+    def has_tables(self, n_pos: int, device) -> bool:
+        return (n_pos, self.inv_freq.dtype, str(device)) in self._tables
 
     def tables(self, n_pos: int, device) -> tuple[torch.Tensor, torch.Tensor]:
         key = (n_pos, self.inv_freq.dtype, str(device))
-        if self._cache is None or self._cache[0] != key:
+        if key not in self._tables:
             inv = self.inv_freq.to(device)
             t = torch.arange(n_pos, device=device, dtype=inv.dtype)
             freqs = torch.einsum('i,j->ij', t, inv)
             emb = torch.cat((freqs, freqs), dim=-1)
-            self._cache = (key, emb.cos().float().contiguous(), emb.sin().float().contiguous())
-        return self._cache[1], self._cache[2]
+            self._tables[key] = (emb.cos().float().contiguous(), emb.sin().float().contiguous())
+        return self._tables[key]
 
 
 @dataclass
@@ -246,6 +249,13 @@ class CogVLMModel(nn.Module):
                 kv_cache.abort()
             raise
 
+    def _rope_len(self, cache: PagedKVCache, dev) -> int:
+        """length of the rotary tables of a call over a conversation: they grow with its positions (as the reference's do, :255)"""
+        n = cache.rope_len(int(self.config.max_position_embeddings))
+        if cache.in_capture and not all(layer.self_attn.rotary_emb.has_tables(n, dev) for layer in self.layers):
+            raise RuntimeError('the rotary tables grow inside a captured step: run a step outside of it first (after reserve())')
+        return n
+
     def _forward(self, input_ids, image, patch_size, pool_size, token_type_ids, attention_mask, position_ids, output_hidden_states, kv_cache):
         B, L = input_ids.shape
         dev = input_ids.device
@@ -266,6 +276,10 @@ class CogVLMModel(nn.Module):
             kv_cache.begin(torch.div(tok, L, rounding_mode='floor').to(torch.int32), rank[tok],
                            rt.cu_seqlens[1:] - rt.cu_seqlens[:-1], L)
             rt.kv = kv_cache
+            if isinstance(kv_cache, PagedKVCache):
+                if not kv_cache.in_capture and B * L > 0:      # (one synchronisation per prompt or chunk; inside a capture what is reserved counts)
+                    kv_cache.pos_bound = max(kv_cache.pos_bound, int((position_ids * (attention_mask != 0)).max()) + 1)
+                rt.n_pos = self._rope_len(kv_cache, dev)
         # token ids per packed row; rows that will be overwritten by image features look up nothing (-1)
         ids = input_ids.reshape(-1).to(torch.int32)
         feats = None
@@ -304,7 +318,8 @@ class CogVLMModel(nn.Module):
     @torch.no_grad()
     def decode_step(self, input_ids: torch.Tensor, position_ids: torch.Tensor, kv_cache: KVCache | PagedKVCache,
                     live: torch.Tensor | None = None) -> torch.Tensor:
-        """one new token per sample against the cache: input_ids, position_ids [B] (device); live bool [B] (paged cache): the samples that
+        """one new token per sample against the cache: input_ids, position_ids [B] (device; paged cache: none of them above the largest so far
+        by more than one, or announced by `reserve_positions`); live bool [B] (paged cache): the samples that
         still go on, the others store nothing and their rows mean nothing. A single-token call never
         touches the vision expert (get_expert_mask with L == 1, reference :58-70) and skips the padding-masked norms
         (:306-309), so every row is a language row. No host synchronisation. -> final hidden [B, h]"""
@@ -320,6 +335,9 @@ class CogVLMModel(nn.Module):
                      expert_mask=None, row_pos=position_ids.to(torch.int32).contiguous(), n_rows=c.decode_counts[1:2],
                      B=B, L=1, n_pos=int(self.config.max_position_embeddings), kv=c, kv_lens=c.lens_after())
         try:
+            if isinstance(c, PagedKVCache):
+                c.pos_bound += not c.in_capture
+                rt.n_pos = self._rope_len(c, input_ids.device)
             x = Fh.embedding_rows(self.embed_tokens.weight, input_ids.to(torch.int32).contiguous())
             for layer in self.layers:
                 x = layer(x, rt)

@@ -427,6 +427,8 @@ class MMMMForCausalLM(CogVLMForCausalLM):
             else:
                 cache = self.new_kv_cache(B, L + steps, dev)
             paged = isinstance(cache, PagedKVCache)
+            if paged:                          # the rotary tables hold the whole turn: they do not grow inside a captured step
+                cache.reserve_positions(max(cache.pos_bound, int((position_ids * (attention_mask != 0)).max()) + 1) + steps)
 
             def trim():      # after the prompt, and when a page more than the budget has gathered
                 if kv_budget is None or cache.len_bound < kv_budget + cache.page_size:

@@ -196,3 +196,32 @@ def test_a_failed_eviction_gives_its_pages_back(monkeypatch, good):
     else:
         c.evict(16, 4)
         assert c.len_bounds == [16, 16, 3]
+
+
+def test_rotary_tables_grow_without_changing():
+    from mmmm_amd.models.cogvlm.modeling_cogvlm import RotaryEmbedding
+    for dtype in (torch.float32, torch.bfloat16):
+        r = RotaryEmbedding(32).to(dtype)
+        short = r.tables(64, 'cpu')
+        long = r.tables(256, 'cpu')
+        assert all(torch.equal(a, b[:64]) for a, b in zip(short, long)) and not torch.equal(long[0][63], long[0][200])
+        assert r.tables(64, 'cpu')[0] is short[0] and r.has_tables(256, 'cpu') and not r.has_tables(128, 'cpu')      # the shorter ones stay
+
+
+def test_how_long_the_rotary_tables_are():
+    c = cache()
+    assert c.rope_len(64) == 64
+    c.pos_bound = 64
+    assert c.rope_len(64) == 64
+    c.pos_bound = 65
+    assert c.rope_len(64) == 128
+    c.reserve_positions(300)
+    c.reserve_positions(10)
+    assert c.rope_len(64) == 512
+    d = cache()
+    d.pos_bound = 1000                                       # positions may be ahead of the cached tokens (eviction)
+    d.len_bounds = [10, 40, 40]
+    d.reserve(60)
+    assert d.rope_len(1) == 2048 and d.pos_bound == 1000
+    d.reserve(100)
+    assert d.rope_len(1090) == 1090 and d.rope_len(1089) == 2178

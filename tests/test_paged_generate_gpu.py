@@ -293,3 +293,61 @@ def test_weights_that_count_a_failed_call_are_not_evicted_by(dev, lm, monkeypatc
     with pytest.raises(RuntimeError, match='received weights'):
         lm.generate(said, **turn, kv_budget=24, kv_recent=8)
     assert lm.generate(said, **turn).new_tokens.shape == (3, 30)
+
+
+@pytest.mark.parametrize('graph', [False, True])
+@pytest.mark.parametrize('budget', [None, 24])
+def test_positions_beyond_the_configured_ones(dev, lm, monkeypatch, graph, budget):
+    """a conversation that crosses max_position_embeddings, in a step and in a chunk: the same answers as where the limit is far away"""
+    batch, tok = make_inputs(dev)
+    lm.tokenizer = tok
+    ids, kw = _batch(batch)
+    top = int((kw['position_ids'] * kw['attention_mask']).max()) + 1
+    g = torch.Generator().manual_seed(12)
+    said = torch.randint(3, 150, (3, 9), generator=g).to(dev)
+    runs = []
+    for limit in (2048, top + 5):                            # crossed in the fifth step
+        monkeypatch.setattr(lm.config, 'max_position_embeddings', limit)
+        cache = lm.new_kv_cache(3, ids.shape[1] + 120, dev, page_size=16, track_weights=budget is not None)
+        extra = dict(past_key_values=cache, use_graph=graph, **(dict(kv_budget=budget, kv_recent=8) if budget else {}))
+        one = lm.generate(ids, **kw, max_new_tokens=30, **extra)
+        pos = one.new_position_ids[:, -1:] + torch.arange(9, device=dev)
+        two = lm.generate(said, token_type_ids=torch.zeros_like(said), position_ids=pos, image=None, patch_size=None, pool_size=None, max_new_tokens=25, **extra)
+        last = lm.generate(said[:, :1], token_type_ids=torch.zeros_like(said[:, :1]), position_ids=two.new_position_ids[:, -1:] + 40, image=None,
+                           patch_size=None, pool_size=None, max_new_tokens=5, **extra)
+        runs.append([one, two, last, cache.k[:, cache.block_table[0, 0].long()].clone()])
+    for a, b in zip(runs[0][:3], runs[1][:3]):
+        assert torch.equal(a.new_tokens, b.new_tokens) and torch.equal(a.new_position_ids, b.new_position_ids)
+    assert torch.equal(runs[0][3], runs[1][3])
+
+
+def test_tables_do_not_grow_inside_a_capture(dev, lm, monkeypatch):
+    batch, tok = make_inputs(dev)
+    lm.tokenizer = tok
+    ids, kw = _batch(batch)
+    top = int((kw['position_ids'] * kw['attention_mask']).max()) + 1
+    monkeypatch.setattr(lm.config, 'max_position_embeddings', top + 1)
+    cache = lm.new_kv_cache(3, ids.shape[1] + 4 * top, dev, page_size=16)
+    lm.eval()
+    with torch.no_grad():
+        lm(ids, **kw, past_key_values=cache, use_cache=True)
+        tok1, pos = ids[:, 0].contiguous(), torch.full((3,), top, device=dev)
+        cache.reserve(ids.shape[1] + 3 * top)
+        x = torch.zeros(4, device=dev)
+        with pytest.raises(RuntimeError, match='captured'):
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                x.add_(1)
+                lm.model.decode_step(tok1, pos, cache)
+        before = cache.tighten()
+        cache.reserve(ids.shape[1] + 3 * top)
+        eager = lm.model.decode_step(tok1, pos, cache)       # the tables grow here
+        assert cache.lens.tolist() == [n + 1 for n in before]
+        cache.lens.copy_(torch.tensor(before, dtype=torch.int32))
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = lm.model.decode_step(tok1, pos, cache)
+        for _ in range(3):
+            cache.lens.copy_(torch.tensor(before, dtype=torch.int32))
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(out, eager)
