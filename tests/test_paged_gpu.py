@@ -693,3 +693,73 @@ def test_cache_evicts_a_ragged_batch(dev):
                 for h in range(2):
                     assert torch.equal(now[h], old[layer][b][n][h][kept[b][h]])
                     assert torch.equal(c.weights[layer, b, h, :len(kept[b][h])], w[layer, b, h][kept[b][h]])
+
+
+@pytest.mark.parametrize('budget,recent', [(100, 10), (33001, 5000), (39999, 0)])
+@pytest.mark.parametrize('kind', ['random', 'ties'])
+def test_evict_of_more_tokens_than_lds_holds_keys(dev, K, budget, recent, kind):
+    """beyond 32768 tokens the keys are made again in every pass; the shorter sample beside it keeps its keys in LDS"""
+    g = torch.Generator().manual_seed(budget)
+    lens, hk, hd, page = [40000, 700], 2, 32, 256
+    k, v, tab = R.make_cache(lens + [min(n, budget) for n in lens], hk, hd, page, g)
+    table, new_table = tab[:2], tab[2:]
+    table[0, 1] = -1                                                         # 256 tokens that are not there
+    w = torch.rand(2, hk, 40000, generator=g)
+    if kind == 'ties':
+        w = (w * 50).floor()
+    kept, new = R.evict(w, table, k.shape[0], page, lens, budget, recent)
+    kd, vd = k.to(dev), v.to(dev)
+    nw, nl, got = K.kv_evict_paged(kd, vd, w.to(dev), table.to(dev), i32(lens, dev), new_table.to(dev), budget, recent)
+    assert nl.tolist() == new
+    ke, ve = k.clone(), v.clone()
+    for b in range(2):
+        for h in range(hk):
+            idx = torch.tensor(kept[b][h])
+            n = len(idx)
+            assert torch.equal(got[b, h, :n].cpu().long(), idx) and (got[b, h, n:] == -1).all()
+            assert torch.equal(nw[b, h, :n].cpu(), w[b, h][idx]) and (nw[b, h, n:] == 0).all()
+            at = torch.arange(n)
+            src, dst = table[b].long()[idx // page], new_table[b].long()[at // page]
+            ke[dst, h, at % page], ve[dst, h, at % page] = k[src, h, idx % page], v[src, h, idx % page]
+    assert torch.equal(kd.cpu().view(torch.int16), ke.view(torch.int16)) and torch.equal(vd.cpu().view(torch.int16), ve.view(torch.int16))
+
+
+FIRST_EVICTION = """
+import torch
+from mmmm_amd import kernels as K
+dev = torch.device('cuda', 0)
+g = torch.Generator().manual_seed(0)
+k, v = (torch.randn(20, 2, 64, 128, generator=g).bfloat16().to(dev) for _ in range(2))
+t = torch.arange(14, dtype=torch.int32, device=dev).view(2, 7)
+nt = torch.tensor([[15, 17, 18], [14, 16, -1]], dtype=torch.int32, device=dev)     # pages that nothing else uses
+lens = torch.tensor([430, 100], dtype=torch.int32, device=dev)
+w = torch.rand(2, 2, 448, generator=g).to(dev)
+torch.cuda.synchronize()
+for budget in (60, 129):                                  # rows moved by the select itself; by a launch of their own
+    k1, v1 = k.clone(), v.clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        a = K.kv_evict_paged(k1, v1, w, t, lens, nt, budget, 4)
+    for _ in range(3):
+        k1.copy_(k)
+        v1.copy_(v)
+        graph.replay()
+        torch.cuda.synchronize()
+        k2, v2 = k.clone(), v.clone()
+        b = K.kv_evict_paged(k2, v2, w, t, lens, nt, budget, 4)
+        assert all(torch.equal(x, y) for x, y in zip(a + (k1, v1), b + (k2, v2)))
+    for s in range(2):
+        for h in range(2):
+            for j, i in enumerate(a[2][s, h].tolist()):
+                if i >= 0:
+                    assert torch.equal(k1[int(nt[s, j // 64]), h, j % 64], k[int(t[s, i // 64]), h, i % 64])
+                    assert torch.equal(v1[int(nt[s, j // 64]), h, j % 64], v[int(t[s, i // 64]), h, i % 64])
+    assert torch.equal(k1[:14], k[:14]) and torch.equal(v1[:14], v[:14])
+print('equal')
+"""
+
+
+def test_first_eviction_inside_a_capture_moves_the_rows():
+    """a process whose first call is a captured eviction, into pages of its own: indices, weights and the moved rows on every replay"""
+    r = subprocess.run([sys.executable, '-c', FIRST_EVICTION], cwd=Path(__file__).resolve().parents[1], capture_output=True, text=True, timeout=100)
+    assert r.returncode == 0 and 'equal' in r.stdout, r.stderr[-2000:]
