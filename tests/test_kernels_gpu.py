@@ -1271,3 +1271,27 @@ def test_sumsq_partials_is_the_sum_of_squares_and_deterministic(dev, K, dtype, n
     assert torch.equal(a, b) and torch.isfinite(a).all()
     ref = x.double().pow(2).sum().item()
     assert abs(a.double().sum().item() - ref) <= 2e-6 * ref
+
+
+@pytest.mark.parametrize('cols', [64, 256, 768, 1792, 2048])
+@pytest.mark.parametrize('affine', [True, False])
+def test_norm_forms_have_the_same_bits_in_fp32(dev, K, cols, affine):
+    """the fused multiply-adds are written out in both loop forms: no exemption for fp32 or for the RMSNorm"""
+    from mmmm_amd import hip
+    g = torch.Generator().manual_seed(cols)
+    x, dy, add, res = (torch.randn(203, cols, generator=g).to(dev) for _ in range(4))
+    w, b = ((1 + 0.1 * torch.randn(cols, generator=g)).to(dev) for _ in range(2))
+    out = []
+    try:
+        for on in (1, 0):
+            assert hip.lib().vm_norm_register_rows_(on) == 0
+            y, rstd = K.rmsnorm_fwd(x, w, 1e-6)
+            dx, _ = K.rmsnorm_bwd(x, w, dy, rstd, need_dw=False, dx_add=add)
+            dx1, _ = K.rmsnorm_bwd(x, w, dy, rstd, need_dw=False)
+            y2, mean, rstd2 = K.layernorm_fwd(x, w if affine else None, b if affine else None, 1e-5, residual=res)
+            dx2, _, _ = K.layernorm_bwd(x, w if affine else None, dy, mean, rstd2, need_dw=False, dx_add=add)
+            out.append(dict(y=y, rstd=rstd, dx=dx, dx1=dx1, y2=y2, mean=mean, rstd2=rstd2, dx2=dx2))
+    finally:
+        hip.lib().vm_norm_register_rows_(1)
+    for n in out[0]:
+        assert torch.equal(out[0][n], out[1][n]), (n, float((out[0][n] - out[1][n]).abs().max()))
