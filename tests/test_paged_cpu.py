@@ -145,3 +145,24 @@ def test_weights_out_of_one_sample_for_all_is_refused():
     cu, lens = torch.zeros(3, dtype=torch.int32), torch.zeros(2, dtype=torch.int32)
     with pytest.raises(AssertionError):
         K.attn_paged(torch.zeros(3, 256, dtype=torch.bfloat16), k, k.clone(), torch.zeros(2, 3, dtype=torch.int32), cu, lens, 0.1, 3, 40, weights=w.expand(2, 2, 48))
+
+
+@pytest.mark.parametrize('kw,want', [
+    (dict(max_q=1, max_kv=12000), 2 * 2 * 2 * 24 * (128 + 4) * 4),                        # few rows: 24 key splits of 512 tokens, 2 rows per cache
+    (dict(max_q=1, max_kv=12000, w_cols=12800), 2 * 2 * 2 * (24 * (128 + 4) + 12000) * 4),        # ... and their scores
+    (dict(max_q=1, max_kv=400), 0),
+    (dict(max_q=10, max_kv=12000), 2 * 2 * 20 * 24 * (128 + 4) * 4),                      # many rows: 24 splits again
+])
+def test_the_workspace_is_asked_for_and_missed(lib, kw, want):
+    """what the plan needs, and the call without it, or with a byte less, or misaligned, refused"""
+    if 'w_cols' in kw:
+        kw = dict(kw, weights=P, weights_out=P, ldw_head=12800, ldwo_head=12800)
+    a = attn(cache(max_pages=200, ld_table=200, n_pages=4), **kw)
+    n = C.c_int64(-1)
+    assert lib.vm_attn_paged_workspace(C.addressof(a), C.addressof(n)) == OK and n.value == want
+    if want:
+        assert lib.vm_attn_paged_bf16(C.addressof(a), None) == BAD
+        a.workspace, a.workspace_bytes = P, want - 1
+        assert lib.vm_attn_paged_bf16(C.addressof(a), None) == BAD
+        a.workspace, a.workspace_bytes = P + 8, want
+        assert lib.vm_attn_paged_bf16(C.addressof(a), None) == BAD
