@@ -260,11 +260,13 @@ def self_launch(n: int) -> int:
 
 
 def gemm_source_digest() -> str:
-    """sha256 (first 16 hex digits) over the sources of the dominant GEMM kernel: ties a committed PMC measurement to the code it measured"""
+    """sha256 (first 16 hex digits) over the sources of the dominant GEMM kernel and the flags they are compiled with: ties a committed PMC
+    measurement to the code it measured. (The library's version number stands in one of the files and says nothing about the kernel.)"""
     import hashlib
-    h = hashlib.sha256()
+    from mmmm_amd.build import CFLAGS
+    h = hashlib.sha256(' '.join(CFLAGS).encode())
     for f in ('gemm256.hip', 'gemm256w.hpp', 'gemm.hip', 'gemm_common.hpp', 'vm_tile.hpp'):
-        h.update((ROOT / 'mmmm_amd' / 'csrc' / f).read_bytes())
+        h.update(b'\n'.join(x for x in (ROOT / 'mmmm_amd' / 'csrc' / f).read_bytes().split(b'\n') if not x.startswith(b'int vm_version(void)')))
     return h.hexdigest()[:16]
 
 
@@ -694,7 +696,7 @@ def main():
                 if tj.get('source_digest') == digest:      # ... if it was taken on THESE kernel sources
                     traffic, traffic_src = tj['bytes_per_launch'], f'profiles/{tf.name}: ' + tj['source']
                 else:
-                    traffic_src = (f'profiles/{tf.name} is STALE (kernel sources changed since it was measured: digest {tj.get("source_digest")} '
+                    traffic_src = (f'profiles/{tf.name} is STALE (kernel sources or compile flags changed since it was measured: digest {tj.get("source_digest")} '
                                    f'vs {digest}; it held {tj["bytes_per_launch"]:.3e} bytes per launch) — re-run tools/pmc_traffic.sh')
             out['roofline'] = {'bound': 'mfma', 'kernel': 'gemm256_k / gemm256w_k / gemm_nt_k<bf16> (vm_gemm_bf16)', 'achieved': ach, 'peak': PEAK_BF16_TFLOPS,
                                'unit': 'TFLOP/s', 'frac': ach / PEAK_BF16_TFLOPS,

@@ -9,7 +9,7 @@ R=$PWD; cd /tmp && export TMPDIR=/tmp
 export AMD_SERIALIZE_KERNEL=3
 for c in FETCH_SIZE WRITE_SIZE; do
   rm -rf $R/gpurun_out/pmc_$c
-  timeout 900 rocprofv3 --pmc $c --output-format csv -d $R/gpurun_out/pmc_$c -o t -- python3 $R/bench.py --steps 2 --warmup 0 --no-cpu-baseline --no-kernel-events --no-peak-probe --also "" > $R/gpurun_out/pmc_$c.log 2>&1
+  timeout -s KILL ${VM_PMC_SECONDS:-900} rocprofv3 --pmc $c --output-format csv -d $R/gpurun_out/pmc_$c -o t -- python3 $R/bench.py --steps 2 --warmup 0 --no-cpu-baseline --no-kernel-events --no-peak-probe --also "" > $R/gpurun_out/pmc_$c.log 2>&1 || { tail -5 $R/gpurun_out/pmc_$c.log; exit 1; }
 done
 cd $R
 python3 - <<PY
