@@ -202,15 +202,15 @@ class PagedKVCache:
             least *= 2
         return least
 
-    def _room(self, most: list[int], rows_per_seq: torch.Tensor) -> list[int]:
-        """pages for at most most[b] further tokens of sample b, or, where the bounds leave no room for so many, for the rows_per_seq (device)
-        there are behind the lengths there are -> host upper bounds of the new tokens"""
+    def _room(self, most: list[int], rows_per_seq) -> list[int]:
+        """pages for at most most[b] further tokens of sample b, or, where the bounds leave no room for so many, for the rows there are (read
+        from the device by rows_per_seq()) behind the lengths there are -> host upper bounds of the new tokens"""
         want = [n + m for n, m in zip(self._bounds, most)]
         if self._grant(want):
             return most
         if not self._capturing():
             self._settle()
-            most = rows_per_seq.tolist()
+            most = rows_per_seq()
             want = [n + m for n, m in zip(self._bounds, most)]
             if self._grant(want):
                 return most
@@ -221,15 +221,15 @@ class PagedKVCache:
         a sample without new rows is left out of the call altogether (its queries see nothing and count nowhere)"""
         self.abort()
         self.in_capture = self._capturing()
-        self._pending_bounds = self._room([max_new] * self.batch if self.launch_new is None else self.launch_new, rows_per_seq)
+        self._pending_bounds = self._room([max_new] * self.batch if self.launch_new is None else self.launch_new, rows_per_seq.tolist)
         self._row_seq = seq_of_row.to(torch.int32).contiguous()
         self._row_index = (self.lens[self._row_seq.long()] + offset_in_seq.to(torch.int32)).contiguous()
         self._pending = rows_per_seq.to(torch.int32)
         self._lens_after = torch.where(self._pending > 0, self.lens + self._pending, self.zeros)
 
-    def prepare_step(self, live: torch.Tensor):
-        """ahead of the capture or a replay of a decode step: pages for its tokens (live bool [batch]: the samples that may still have one)"""
-        self.launch_new = self._room([1] * self.batch, live)
+    def prepare_step(self, done: torch.Tensor):
+        """ahead of the capture or a replay of a decode step: pages for its tokens (done bool [batch]: the samples that have none)"""
+        self.launch_new = self._room([1] * self.batch, lambda: [int(not d) for d in done.tolist()])
 
     def count_step(self):
         """a captured step has been replayed: its tokens"""

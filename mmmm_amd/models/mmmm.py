@@ -538,7 +538,7 @@ class MMMMForCausalLM(CogVLMForCausalLM):
         def ahead():                              # no page may be handed out inside the captured step
             if paged:
                 trim()
-                cache.prepare_step(~s_done)
+                cache.prepare_step(s_done)
 
         cache.launch_bound = cache.max_len
         try:

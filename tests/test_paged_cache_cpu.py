@@ -111,7 +111,7 @@ def test_bounds_are_a_samples_own():
     c.begin(torch.tensor([0, 1], dtype=torch.int32), torch.zeros(2, dtype=torch.int32), torch.tensor([1, 1, 0], dtype=torch.int32), 1)
     assert c.attn_bound() == 201
     c.commit()
-    c.prepare_step(torch.tensor([True, True, True]))
+    c.prepare_step(torch.tensor([False, False, False]))
     assert c.launch_new == [1, 1, 1]
     c.count_step()
     assert c.len_bounds == [202, 5, 2]
@@ -123,8 +123,8 @@ def test_a_captured_steps_pages_go_to_the_samples_that_go_on():
     c = PagedKVCache(1, 2, 64, 2, 32, 'cpu', page_size=16, n_pages=3)
     turn(c, [16, 16])                                        # both at the end of a page, one page left
     with pytest.raises(ValueError):
-        c.prepare_step(torch.tensor([True, True]))
-    c.prepare_step(torch.tensor([False, True]))
+        c.prepare_step(torch.tensor([False, False]))
+    c.prepare_step(torch.tensor([True, False]))
     assert c.launch_new == [0, 1] and (c.block_table >= 0).sum(1).tolist() == [1, 2]
     c.count_step()
     assert c.len_bounds == [16, 17]
