@@ -184,7 +184,7 @@ class PagedKVCache:
 
     def reserve(self, tokens: int):
         """pages for `tokens` tokens of every sample (those it has counted), and rotary tables for positions that go on as far: later steps up
-        to that length upload nothing. The pages stay until tighten(); tables that have to grow for it do so in the next step, which then
+        to that length upload nothing. The pages stay, over further turns and evictions, until tighten(); tables that have to grow for it do so in the next step, which then
         must not be a captured one."""
         want = [tokens] * self.batch
         if not self._grant(want):
@@ -209,7 +209,7 @@ class PagedKVCache:
         if self._grant(want):
             return most
         if not self._capturing():
-            self._settle()
+            self.settle()
             most = rows_per_seq()
             want = [n + m for n, m in zip(self._bounds, most)]
             if self._grant(want):
@@ -269,8 +269,9 @@ class PagedKVCache:
         self._pending = None
         self._counting = False
 
-    def _settle(self) -> list[int]:
-        """the lengths as they are on the device; pages behind them (and behind what is reserved) are free again"""
+    def settle(self) -> list[int]:
+        """read the lengths back (synchronises), give pages behind them back that are not reserved -> lengths"""
+        assert self._pending is None, 'settle() between begin() and commit()'
         lens = self.lens.tolist()
         self._bounds = list(lens)
         changed = False
@@ -284,10 +285,10 @@ class PagedKVCache:
         return lens
 
     def tighten(self) -> list[int]:
-        """read the lengths back (synchronises), give pages behind them back, reserved ones too -> lengths"""
+        """settle(), and reserved pages go back too: a step that was captured on them must not be replayed any more -> lengths"""
         assert self._pending is None, 'tighten() between begin() and commit()'
         self._reserved = [0] * self.batch
-        return self._settle()
+        return self.settle()
 
     def pages_to_evict(self, budget: int) -> int:
         """free pages that evict() to `budget` tokens needs while it runs: those of the samples that are over it"""
@@ -330,3 +331,4 @@ class PagedKVCache:
                 self._free.extend(p)
         self._pages = pages
         self._bounds = [min(n, budget) for n in self._bounds]
+        self._grant([max(n, r) for n, r in zip(self._bounds, self._reserved)])      # (out of the pages that have just come back)

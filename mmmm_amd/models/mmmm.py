@@ -421,7 +421,7 @@ class MMMMForCausalLM(CogVLMForCausalLM):
             steps = max_new_tokens if forced_tokens is None else forced_tokens.shape[1]
             if past_key_values is not None:
                 cache = past_key_values
-                cache.tighten()
+                cache.settle()
             elif kv_page_size is not None:
                 cache = self._new_paged_cache(B, L, steps, dev, kv_page_size, kv_budget)
             else:
@@ -434,7 +434,7 @@ class MMMMForCausalLM(CogVLMForCausalLM):
                 if kv_budget is None or cache.len_bound < kv_budget + cache.page_size:
                     return
                 if cache.pages_to_evict(kv_budget) > cache.free_pages:      # (as far as the host knows the lengths)
-                    cache.tighten()
+                    cache.settle()
                 cache.evict(kv_budget, kv_recent)
             out = self(input_ids, image=image, patch_size=patch_size, pool_size=pool_size, token_type_ids=token_type_ids,
                        attention_mask=attention_mask, position_ids=position_ids, past_key_values=cache, use_cache=True,

@@ -225,3 +225,18 @@ def test_how_long_the_rotary_tables_are():
     assert d.rope_len(1) == 2048 and d.pos_bound == 1000
     d.reserve(100)
     assert d.rope_len(1090) == 1090 and d.rope_len(1089) == 2178
+
+
+def test_eviction_leaves_the_reserved_pages(monkeypatch):
+    from mmmm_amd.models.cogvlm import kv_cache
+    monkeypatch.setattr(kv_cache.K, 'kv_evict_paged', lambda k, v, w, t, lens, new, budget, recent: (w, lens.clamp(max=budget), None))
+    c = PagedKVCache(2, 2, 128, 4, 32, 'cpu', page_size=16, track_weights=True, n_pages=16)
+    c.reserve(96)
+    turn(c, [90, 20])
+    assert c.settle() == [90, 20] and (c.block_table >= 0).sum(1).tolist() == [6, 6] and c.free_pages == 4
+    c.evict(32, 4)
+    assert c.len_bounds == [32, 20] and c.lens.tolist() == [32, 20]
+    assert (c.block_table >= 0).sum(1).tolist() == [6, 6] and c.free_pages == 4
+    used = c.block_table[c.block_table >= 0].tolist()
+    assert len(set(used)) == 12 and not set(used) & set(c._free)
+    assert c.tighten() == [32, 20] and c.free_pages == 12

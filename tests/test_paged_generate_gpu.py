@@ -351,3 +351,32 @@ def test_tables_do_not_grow_inside_a_capture(dev, lm, monkeypatch):
             graph.replay()
             torch.cuda.synchronize()
             assert torch.equal(out, eager)
+
+
+def test_a_turn_leaves_the_pages_of_a_captured_step(dev, lm):
+    """pages reserved for a captured step stay through generate(): its replays store their tokens"""
+    batch, tok = make_inputs(dev)
+    lm.tokenizer = tok
+    ids, kw = _batch(batch)
+    cache = lm.new_kv_cache(3, ids.shape[1] + 100, dev, page_size=16)
+    lm.generate(ids, **kw, max_new_tokens=2, past_key_values=cache)
+    cache.reserve(ids.shape[1] + 90)
+    tok1, pos = ids[:, 0].contiguous(), torch.full((3,), 40, device=dev)
+    lm.eval()
+    lm.model.decode_step(tok1, pos, cache)
+    bounds = cache.len_bounds
+    graph = torch.cuda.CUDAGraph()
+    with torch.no_grad(), torch.cuda.graph(graph):
+        lm.model.decode_step(tok1, pos, cache)
+    cache.len_bounds = bounds
+    free = cache.free_pages
+    said = ids[:, :1].clone()
+    lm.generate(said, token_type_ids=torch.zeros_like(said), position_ids=pos[:, None], image=None, patch_size=None, pool_size=None, max_new_tokens=3,
+                past_key_values=cache)
+    assert cache.free_pages == free
+    before = cache.settle()
+    for _ in range(40):
+        graph.replay()
+    now = cache.settle()
+    assert now == [n + 40 for n in before]
+    assert all(int(p) >= 0 for b in range(3) for p in cache.block_table[b, :-(-now[b] // 16)])
