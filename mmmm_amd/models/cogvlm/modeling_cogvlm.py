@@ -98,7 +98,10 @@ class RotaryEmbedding(nn.Module):
             t = torch.arange(n_pos, device=device, dtype=inv.dtype)
             freqs = torch.einsum('i,j->ij', t, inv)
             emb = torch.cat((freqs, freqs), dim=-1)
-            self._tables[key] = (emb.cos().float().contiguous(), emb.sin().float().contiguous())
+            made = emb.cos().float().contiguous(), emb.sin().float().contiguous()
+            if made[0].is_cuda and not torch.cuda.is_current_stream_capturing():
+                torch.cuda.current_stream(made[0].device).synchronize()      # the next reader may be on another stream
+            self._tables[key] = made
         return self._tables[key]
 
 

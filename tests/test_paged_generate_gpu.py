@@ -380,3 +380,20 @@ def test_a_turn_leaves_the_pages_of_a_captured_step(dev, lm):
     now = cache.settle()
     assert now == [n + 40 for n in before]
     assert all(int(p) >= 0 for b in range(3) for p in cache.block_table[b, :-(-now[b] // 16)])
+
+
+def test_rotary_tables_are_whole_on_every_stream(dev):
+    """tables that were asked for first on a busy stream are read on another one"""
+    from mmmm_amd.models.cogvlm.modeling_cogvlm import RotaryEmbedding
+    r = RotaryEmbedding(64).to(dev)
+    r.tables(16, dev)                                        # (the kernels are loaded)
+    want = RotaryEmbedding(64).to(dev).tables(4096, dev)
+    busy, other = torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(busy):
+        torch.cuda._sleep(200_000_000)                       # a tenth of a second
+        r.tables(4096, dev)
+    with torch.cuda.stream(other):
+        got = [t.clone() for t in r.tables(4096, dev)]
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
