@@ -268,6 +268,11 @@ class CogVLMModel(nn.Module):
             attention_mask = torch.ones_like(input_ids)
         if position_ids is None:
             position_ids = torch.arange(L, device=dev)[None].expand(B, L)
+        if isinstance(kv_cache, PagedKVCache):
+            attention_mask = attention_mask[:, -L:]      # (that of the whole conversation will do: the cache holds valid tokens only)
+            for x in (token_type_ids, attention_mask, position_ids):
+                if x.shape != (B, L):
+                    raise ValueError(f'a call of {B} x {L} tokens with {tuple(x.shape)} token types, mask or positions')
         rt = self.build_routing(token_type_ids, attention_mask, position_ids)
         if kv_cache is not None:
             assert not torch.is_grad_enabled() or not self.training, 'the KV cache is an inference-only structure'

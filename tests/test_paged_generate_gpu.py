@@ -397,3 +397,27 @@ def test_rotary_tables_are_whole_on_every_stream(dev):
         got = [t.clone() for t in r.tables(4096, dev)]
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_a_chunk_with_the_mask_of_the_whole_conversation(dev, lm):
+    batch, tok = make_inputs(dev)
+    lm.tokenizer = tok
+    g = torch.Generator().manual_seed(15)
+    ids, said = (torch.randint(3, 150, (2, n), generator=g).to(dev) for n in (11, 6))
+    mask, now = torch.ones_like(ids), torch.ones_like(said)
+    mask[1, 4:] = 0
+    now[0, 5] = 0
+    lm.eval()
+    out = []
+    with torch.no_grad():
+        for m in (now, torch.cat([mask, now], 1)):
+            cache = lm.new_kv_cache(2, 40, dev, page_size=16)
+            lm(ids, token_type_ids=torch.zeros_like(ids), attention_mask=mask, position_ids=torch.arange(11, device=dev).expand(2, 11), past_key_values=cache, use_cache=True)
+            kw = dict(token_type_ids=torch.zeros_like(said), attention_mask=m, position_ids=11 + torch.arange(6, device=dev).expand(2, 6), past_key_values=cache)
+            out.append(lm(said, **kw).logits)
+            assert cache.lens.tolist() == [16, 10]
+        assert torch.equal(out[0][now.bool()], out[1][now.bool()])
+        for bad in (dict(attention_mask=now[:, :3]), dict(position_ids=torch.arange(17, device=dev).expand(2, 17)), dict(token_type_ids=torch.zeros(2, 17, dtype=torch.long, device=dev))):
+            with pytest.raises(ValueError):
+                lm(said, **{**kw, **bad})
+        assert cache.settle() == [16, 10]
