@@ -541,7 +541,8 @@ int vm_kv_append_paged_bf16(const vm_paged_kv* cache_host, const void* qkv, int6
  * [0, n_rows) there is no such query (lse = -inf). lse[h * ld_lse + position]. Rows of no position are left as they were. max_q / max_kv:
  * host upper bounds of n_b and of kv_lens (no device -> host sync); a bound that is too small leaves queries, or weights of tokens, out.
  * weights_out (may be NULL): weights_out[b][kv head][j] = weights[b][kv head][j] + the sum of the probabilities that token j gets from this
- * call's queries of the heads of that kv head, for j < kv_lens[b]; fp32, fixed order of summation; weights may be the same buffer. */
+ * call's queries of the heads of that kv head, for j < kv_lens[b]; fp32, fixed order of summation; weights may be the same buffer. out may be q where no weights are asked for; no two
+ * positions have the same row. */
 typedef struct vm_attn_paged_args {
   vm_paged_kv cache;
   const void* q;

@@ -538,6 +538,8 @@ int vm_attn_paged_bf16(const vm_attn_paged_args* args_host, void* stream) {
   AttnPagedP p;
   const int rc = fill(args_host, p);
   if (rc != VM_OK) return rc;
+  // the weights of many rows need the queries once more
+  if (p.w_out && p.n_rows > 0 && args_host->out == args_host->q) return VM_ERR_BAD_ARG;
   hipStream_t st = (hipStream_t)stream;
   const int hd = args_host->cache.head_dim;
   const Plan a = plan(p, hd);

@@ -922,7 +922,8 @@ def attn_paged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, bl
     q [rows, heads hd] bf16 (rotated); positions cu_q[b] .. cu_q[b+1]-1 are the last tokens of the kv_lens[b] cached ones (int32, device);
     row_of_pos: packed row of a position. max_q / max_kv: host upper bounds of the new and of the cached tokens of a sample.
     weights [samples, kv heads, >= max_kv] fp32: the attention weight every token has received so far; with this call's added it goes to
-    weights_out (default: in place). -> (out [rows, heads hd], lse fp32 [heads, rows] by position)"""
+    weights_out (default: in place). -> (out [rows, heads hd], lse fp32 [heads, rows] by position; rows and positions that no sample has are
+    not written)"""
     c, dev = _paged(k_pages, v_pages, block_table)
     ps, cols, n_seq, hk, hd = c[4], c[7], c[8], c[9], c[10]
     assert q.dim() == 2
@@ -946,6 +947,7 @@ def attn_paged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, bl
         op, ldo = out.data_ptr(), width
     else:
         op, ldo = _rows(out, shape, dev)
+        assert weights is None or op != qp or rows == 0, 'the weights need the queries after the output is written'
     lse = torch.empty(n_heads, rows, dtype=torch.float32, device=q.device)
     need = _attn_paged_ws_bytes(n_seq, hk, hd, ps, cols, rows, max_q, max_kv, n_heads, w_cols)
     buf = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None      # (held until the launch is in the stream)

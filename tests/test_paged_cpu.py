@@ -166,3 +166,9 @@ def test_the_workspace_is_asked_for_and_missed(lib, kw, want):
         assert lib.vm_attn_paged_bf16(C.addressof(a), None) == BAD
         a.workspace, a.workspace_bytes = P + 8, want
         assert lib.vm_attn_paged_bf16(C.addressof(a), None) == BAD
+
+
+def test_weights_with_the_output_over_the_queries_are_refused(lib):
+    kw = dict(weights=2 * P, weights_out=2 * P, w_cols=192, ldw_head=192, ldwo_head=192, workspace=P, workspace_bytes=1 << 40)
+    a = attn(**kw)
+    assert lib.vm_attn_paged_bf16(C.addressof(a), None) == BAD

@@ -763,3 +763,15 @@ def test_first_eviction_inside_a_capture_moves_the_rows():
     """a process whose first call is a captured eviction, into pages of its own: indices, weights and the moved rows on every replay"""
     r = subprocess.run([sys.executable, '-c', FIRST_EVICTION], cwd=Path(__file__).resolve().parents[1], capture_output=True, text=True, timeout=100)
     assert r.returncode == 0 and 'equal' in r.stdout, r.stderr[-2000:]
+
+
+@pytest.mark.parametrize('new,L', [(1, 3000), (3, 100), (40, 2500), (300, 700)])
+def test_output_over_the_queries(dev, K, new, L):
+    """out=q without weights: the same bits; with weights it is refused"""
+    args, kw = _case(K, dev, new, L, 7, weights=True)
+    want, lse = K.attn_paged(*args)
+    q = args[0].clone()
+    got, lse2 = K.attn_paged(q, *args[1:], out=q)
+    assert got is q and torch.equal(got, want) and torch.equal(lse, lse2)
+    with pytest.raises(AssertionError):
+        K.attn_paged(q, *args[1:], out=q, **kw)
