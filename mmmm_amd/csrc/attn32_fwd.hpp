@@ -293,7 +293,7 @@ __global__ __launch_bounds__(NW * 64, 2) void fwd_k(const AttnP p) {
           float e0 = fast_exp2(x[0]), e1 = fast_exp2(x[1]);
           w[j] = f2bf(e0);
           w[j + 1] = f2bf(e1);
-          // plain single adds (assembly: left to itself hipcc packs them into v_pk_add_f32 fed by ~45 v_mov per tile)
+          // plain single adds (assembly, from the time when hipcc packed them in pairs fed by ~45 v_mov per tile; packed fp32 is off in every compile now)
           asm("v_add_f32 %0, %1, %0" : "+v"(rs0) : "v"(e0));
           asm("v_add_f32 %0, %1, %0" : "+v"(rs1) : "v"(e1));
         }

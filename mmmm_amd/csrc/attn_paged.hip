@@ -454,7 +454,7 @@ Plan plan(AttnPagedP& p, int hd) {
   Plan a = {};
   const int64_t rows = (int64_t)p.max_q * p.G, heads = (int64_t)p.n_seq * p.c.n_kv_heads;
   // 16 rows are what the split form's matrix tile holds. Beyond it the tile form wins although most of its 256 rows are empty: 4 x 17 queries
-  // over 2086 tokens 34 us beside 37 us (two row tiles a workgroup), 17 x 4 heads over 8704 28 beside 45, 64 queries 38 beside 53.
+  // over 2086 tokens 31 us beside 37 us (two row tiles a workgroup), 17 x 4 heads over 8704 26 beside 45, 64 queries 37 beside 53.
   a.split = rows <= SP_ROWS;
   p.n_split = 1; p.s_rows = (int)rows; p.s_ld = (p.max_kv + 31) / 32 * 32;
   p.part = p.s_ws = nullptr;

@@ -12,9 +12,9 @@
 //  * with fewer than one workgroup per CU the keys are split over workgroups too (partial results joined by attn_paged_join_k);
 //  * V^T fragments are read in two assembly statements of 16 ds_read_b64_tr_b16 that end in their own wait.
 // Matrix-bound in theory (4 hd operations per visible pair), in fact by the softmax between the two products and the barriers between the clusters:
-// 4 x 4609 tokens, 32 heads of width 128: 554 us, 853 TFLOP/s of the visible pairs, matrix pipes busy 0.43 of the time, waves waiting 0.37 of
-// theirs; 512 tokens over 8704: 90 us with the join, 785 TFLOP/s. Measured and not taken: 64 rows per wave and four waves (half the LDS reads, but the
-// registers of two row sets: 680 us); V read untransposed, which would be wrong, gains 3 % — its transposed reads are not what costs.
+// 4 x 4609 tokens, 32 heads of width 128: 585-603 us on three boxes, 785-810 TFLOP/s of the visible pairs, matrix pipes busy 0.39 of the time, waves
+// waiting 0.38 of theirs; 512 tokens over 8704: 96 us with the join, 740 TFLOP/s. Measured and not taken: 64 rows per wave and four waves (half the LDS reads, but the
+// registers of two row sets: 680 us beside 583-607); V read untransposed, which would be wrong, gains 3 % — its transposed reads are not what costs.
 #pragma once
 #include <type_traits>
 #include "attn32_tile.hpp"

@@ -403,7 +403,8 @@ class MMMMForCausalLM(CogVLMForCausalLM):
         further one). A sample's last new token — its eos, where it has ended — is not cached: the next
         `input_ids` begin with it. A sample without valid tokens in `attention_mask` sits the turn out (its new tokens mean
         nothing). `kv_budget` bounds the cached tokens per sample: after the prompt, and whenever one page more has gathered,
-        the tokens that have received the least attention leave (per layer and head; the `kv_recent` newest always stay)."""
+        the tokens that have received the least attention leave (per layer and head; the `kv_recent` newest always stay). They move to pages
+        of their own, so a sample over the budget needs pages for its prompt and for the budget together."""
         if past_key_values is not None and not isinstance(past_key_values, PagedKVCache):
             raise ValueError('only a paged cache can be continued: kv_page_size')
         if kv_budget is not None:
