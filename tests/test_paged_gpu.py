@@ -775,3 +775,27 @@ def test_output_over_the_queries(dev, K, new, L):
     assert got is q and torch.equal(got, want) and torch.equal(lse, lse2)
     with pytest.raises(AssertionError):
         K.attn_paged(q, *args[1:], out=q, **kw)
+
+
+@pytest.mark.parametrize('new', [[1, 1, 1], [3, 0, 1], [40, 1, 20], [300, 30, 1]])
+@pytest.mark.parametrize('H,hk,hd', [(4, 2, 128), (3, 3, 64)])
+def test_bounds_far_above_the_lengths(dev, K, new, H, hk, hd):
+    """what a step captured once for the whole table passes: max_q and max_kv of tables and chunks far longer than what is there"""
+    g = torch.Generator().manual_seed(sum(new))
+    lens, page, cols, rows = [700, 33, 260], 32, 400, 2000
+    k, v, table = R.make_cache(lens, hk, hd, page, g, cols=cols)
+    T = sum(new)
+    q = torch.randn(rows, H * hd, generator=g).bfloat16()
+    w = torch.rand(3, hk, cols * page, generator=g)
+    want = R.attention(q, k, v, table, new, lens, hd ** -0.5, None, w)
+    cu = [0, new[0], new[0] + new[1], T]
+    wo = torch.full_like(w, -1.0).to(dev)
+    out = torch.full((rows, H * hd), 3.0, dtype=torch.bfloat16, device=dev)
+    _, lse = K.attn_paged(q.to(dev), k.to(dev), v.to(dev), table.to(dev), i32(cu, dev), i32(lens, dev), hd ** -0.5, rows, cols * page, weights=w.to(dev),
+                          weights_out=wo, out=out)
+    close(out[:T], want[0][:T], want[1][:T], 'out')
+    close(lse[:, :T], want[2][:, :T], want[3][:, :T], 'lse')
+    assert (out[T:] == 3.0).all()
+    for b, L in enumerate(lens):
+        close(wo[b, :, :L], want[4][b, :, :L], want[5][b, :, :L], 'weights')
+        assert (wo[b, :, L:] == -1.0).all()
