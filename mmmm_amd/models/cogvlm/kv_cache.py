@@ -184,8 +184,9 @@ class PagedKVCache:
 
     def reserve(self, tokens: int):
         """pages for `tokens` tokens of every sample (those it has counted), and rotary tables for positions that go on as far: later steps up
-        to that length upload nothing. The pages stay, over further turns and evictions, until tighten(); tables that have to grow for it do so in the next step, which then
-        must not be a captured one."""
+        to that length upload nothing. The pages stay, over further turns and evictions, until tighten(); tables that have to grow for it do
+        so in the next step, which then must not be a captured one. The replays of a step of one's own are not counted by the host: settle()
+        before the next call or eviction."""
         want = [tokens] * self.batch
         if not self._grant(want):
             raise self._overflow(want)
